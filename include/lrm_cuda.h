@@ -171,7 +171,8 @@ lrm_status lrm_op_set_device(int32_t device);
  * 0x2010 a decode-attention row whose seq_len is below 1 or needs more pages than its page-table row (the row is
  * not read and its output is zeros); 0x3010 a prefill-attention sequence whose cu_seqlens rows fall outside
  * total_tokens or exceed max_len, or whose cached-token count is negative (the sequence is not computed and its
- * output rows are left unwritten). */
+ * output rows are left unwritten); 0x4001-0x4013 the paged attention (0x4010-0x4013 a bounded wait that
+ * gave up); 0x5001-0x5014 the page plan and release; 0x6001 the q/k/v append (their codes stand with them). */
 lrm_status lrm_op_error_word(uint32_t *code, int32_t clear);
 
 /* Runs one kernel whose bounded in-kernel wait can never complete (an mbarrier nothing arrives on), with a limit of
@@ -284,6 +285,96 @@ lrm_status lrm_op_decode_attention(void *stream, const lrm_decode_attn_desc *des
  * the device's error word, so a process that resets a device must not call the library's operators on it again. */
 #define LRM_DECODE_ATTN_STATIC_SCRATCH_BYTES (16u << 20)
 lrm_status lrm_op_decode_attention_static(void *stream, const lrm_decode_attn_desc *desc);
+
+/* ---- a paged serving step on the device ------------------------------------------------------------------------
+ * For a caller that keeps its sequences' state on the device: lengths int32 [max_seqs], a page table int32
+ * [max_seqs][pages_per_seq], and a free list int32 [kv_pages] whose first free_count entries are the free pages (the
+ * top is entry free_count - 1). A slot of length L owns the first ceil(L / 16) entries of its page-table row. A step is
+ *   lrm_op_page_plan       takes pages for each request's new tokens; the step's cu_seqlens, kv_len, tok_pos, slot_map
+ *   lrm_op_qkv_append      per layer: QK-norm, RoPE, q out, k and v into the cache at slot_map
+ *   lrm_op_paged_attention per layer: the new tokens over everything cached, any mixture of single tokens and chunks
+ *   lrm_op_page_release    cuts slots back to a kept length (0 frees them)
+ * with no copy to or from the host, so it can be captured as a CUDA graph whose lengths change from replay to replay.
+ * The reference keeps its KV cache contiguous and on the host's plan (tests/Lrm.Tensor.Tests/TinyModel.fs:144-204); it
+ * has no counterpart of these. All pointers are device addresses; calls are asynchronous on `stream`. Arrays must not
+ * overlap unless a call says so. What only the device knows is checked there and reported in the error word
+ * (lrm_op_error_word). */
+
+/* Block tables and slot maps from request lengths. Request i adds new_len[i] >= 0 tokens to slot slots[i]; slots[i] =
+ * -1 is padding (no tokens, new_len[i] is not read). Pages come off the top of the free list in request order. Writes
+ *   page_table       the new pages' entries (others stay as they are)
+ *   cu_seqlens       int32 [requests + 1]: where each request's tokens start
+ *   kv_len           int32 [requests]: its keys, the new ones included (0 for padding)
+ *   tok_pos          int32 [max_tokens]: each token's position; 0 behind the last token
+ *   slot_map         int32 [max_tokens]: page * 16 + offset of each token; -1 behind the last token
+ *   seq_len_out      int32 [max_seqs]: the new lengths of the slots in slots (others stay); may be seq_len itself
+ *   free_count_out   int32 [1]; may be free_count itself.
+ * All or nothing: on a broken rule the error word gets its code, cu_seqlens and kv_len are all 0, tok_pos 0, slot_map
+ * -1 (so the step's other calls do nothing), and the lengths, the table and the count stay as they were. Codes:
+ *   0x5001 a slot outside 0 .. max_seqs - 1 or listed twice, a negative new_len, or a length (old or new) outside 0 ..
+ *          16 * pages_per_seq;  0x5002 not enough free pages;  0x5003 more than max_tokens tokens;  0x5004 free_count
+ *          outside 0 .. kv_pages, or a page id to be taken outside 0 .. kv_pages - 1.
+ * 0x5005 (alone not a refusal): a page that the slot held already has an id outside the pool; slot_map is -1 for that
+ * page's tokens. Limits: requests 1 .. 65535, max_seqs 1 .. 2^17, pages_per_seq 1 .. 2^20, kv_pages 1 .. 2^26,
+ * max_tokens 1 .. 2^24. */
+typedef struct lrm_page_plan_desc {
+    uint64_t slots, new_len, seq_len, page_table, free_list, free_count;
+    uint64_t cu_seqlens, kv_len, tok_pos, slot_map, seq_len_out, free_count_out;
+    int32_t requests, max_seqs, pages_per_seq, kv_pages, max_tokens;
+} lrm_page_plan_desc;
+lrm_status lrm_op_page_plan(void *stream, const lrm_page_plan_desc *desc);
+
+/* The plan's inverse: slot slots[i] keeps its first keep_len[i] tokens (0 .. its length; 0 frees the slot), and the
+ * pages behind them go back on top of the free list, in request and then page order. slots[i] = -1 is padding.
+ * seq_len_out and free_count_out as in the plan. All or nothing: on a broken rule nothing is written but the code:
+ *   0x5011 a slot outside 0 .. max_seqs - 1 or listed twice, a length outside 0 .. 16 * pages_per_seq, or a keep_len
+ *          outside 0 .. the slot's length;  0x5012 free_count outside 0 .. kv_pages or more pages than the list holds;
+ *          0x5014 a page id to be given back outside 0 .. kv_pages - 1. */
+typedef struct lrm_page_release_desc {
+    uint64_t slots, keep_len, seq_len, page_table, free_list, free_count, seq_len_out, free_count_out;
+    int32_t requests, max_seqs, pages_per_seq, kv_pages;
+} lrm_page_release_desc;
+lrm_status lrm_op_page_release(void *stream, const lrm_page_release_desc *desc);
+
+/* The operator form of the engine's q/k/v epilogue. qkv bf16 [tokens][ld_qkv]: q_heads, then kv_heads k, then kv_heads v
+ * heads of 128 a row. q and k: RMSNorm over the head with gains q_norm / k_norm (bf16 [128]; both 0: no norm), then the
+ * rotate-half RoPE of row tok_pos[t] of cos / sin (fp32 [rope_rows][64]; both 0: no rotation, and tok_pos is not read),
+ * in fp32 with one rounding at the end. q goes to q_out bf16 [tokens][ld_q] (q_out may be qkv's own q columns, with ld_q
+ * = ld_qkv), k and v to place slot_map[t] = page * 16 + offset of pool [kv_pages][kv_heads][2][16][128]. Rows whose
+ * slot_map is -1 are skipped: nothing of them is written. The places of a call must be distinct. A row whose slot_map
+ * is below -1 or past the pool, or whose tok_pos is outside 0 .. rope_rows - 1, is skipped too and the error word gets
+ * 0x6001. ld_qkv and ld_q are multiples of 8; qkv, q_out, pool, the gains and cos / sin are 16-byte aligned. */
+typedef struct lrm_qkv_append_desc {
+    uint64_t qkv, q_norm, k_norm, cos, sin, tok_pos, slot_map, q_out, pool;
+    int64_t ld_qkv, ld_q;
+    int32_t tokens, q_heads, kv_heads, head_dim, rope_rows, kv_pages;
+    float eps;
+} lrm_qkv_append_desc;
+lrm_status lrm_op_qkv_append(void *stream, const lrm_qkv_append_desc *desc);
+
+/* Causal GQA attention of each request's new tokens over its cached keys: rows cu_seqlens[i] .. cu_seqlens[i + 1] - 1 of
+ * q bf16 [tokens][ld_q] (q_heads heads of 128 a row) are the last tokens of the kv_len[i] keys of slot slots[i], which
+ * are read through page_table [max_seqs][pages_per_seq] from pool [kv_pages][kv_heads][2][16][128] (the new tokens' own
+ * k and v included). out bf16 [tokens][ld_out]. Any q_heads that kv_heads divides, up to 128 query heads a KV head;
+ * any mixture of chunk lengths, one token included; requests without tokens are skipped whatever their slot. Keys that a
+ * row does not see do not reach it, whatever they hold (NaN and infinities too). Rows outside every request, before
+ * cu_seqlens[0] or behind cu_seqlens[requests], are left as they were. Softmax statistics and accumulators are fp32.
+ * A request whose rows fall outside the tokens, whose slot is outside 0 .. max_seqs - 1, or whose kv_len is below its
+ * tokens or above 16 * pages_per_seq is not computed: its rows are left as they were and the error word gets 0x4001. A
+ * page id outside the pool is never read: its keys count as zeros and the error word gets 0x4002. `workspace`:
+ * lrm_op_paged_attention_workspace bytes, 16-byte aligned, any contents; calls that can run at the same time need one
+ * each. scale must be positive and finite; ld_q and ld_out multiples of 8; q, pool and out 16-byte aligned.
+ * Limits: requests 1 .. 65535, tokens 1 .. 2^24, max_seqs 1 .. 2^17, pages_per_seq 1 .. 2^20, kv_pages 1 .. 2^26 with
+ * kv_pages * kv_heads below 2^30. */
+typedef struct lrm_paged_attn_desc {
+    uint64_t q, pool, page_table, slots, cu_seqlens, kv_len, out, workspace;
+    int64_t ld_q, ld_out;
+    int32_t requests, tokens, q_heads, kv_heads, head_dim, max_seqs, pages_per_seq, kv_pages;
+    float scale;
+} lrm_paged_attn_desc;
+/* Bytes of workspace for calls of up to `tokens` rows on the current device; 0 for impossible sizes. */
+uint64_t lrm_op_paged_attention_workspace(int32_t tokens, int32_t q_heads, int32_t kv_heads);
+lrm_status lrm_op_paged_attention(void *stream, const lrm_paged_attn_desc *desc);
 
 /* ---- the Qwen3 forward engine (bf16 fast path) ---------------------------------------------------------------- */
 /*

@@ -32,6 +32,8 @@ SOURCES = [
     "flash_tc.cu",
     "qwen_engine.cu",
     "decode_attn_static.cu",
+    "paged_step.cu",
+    "paged_attn.cu",
     "safetensors.cpp",
     "tokenizer.cpp",
 ]

@@ -9,7 +9,7 @@ import ctypes
 
 from . import native as N
 
-P, I32, U32, U64 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_uint32, ctypes.c_uint64
+P, I32, U32, U64, I64 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_uint32, ctypes.c_uint64, ctypes.c_int64
 
 GEMM_F32, GEMM_RESID, GEMM_SWIGLU, GEMM_PARTIAL, GEMM_BF16 = range(5)
 
@@ -38,6 +38,33 @@ class DecodeGemmDesc(ctypes.Structure):
                 ("x", U64), ("gain", U64), ("u", U64), ("ss_out", U64), ("act", U64), ("ld_act", I32)]
 
 
+class PagePlanDesc(ctypes.Structure):
+    _fields_ = [("slots", U64), ("new_len", U64), ("seq_len", U64), ("page_table", U64), ("free_list", U64),
+                ("free_count", U64), ("cu_seqlens", U64), ("kv_len", U64), ("tok_pos", U64), ("slot_map", U64),
+                ("seq_len_out", U64), ("free_count_out", U64), ("requests", I32), ("max_seqs", I32),
+                ("pages_per_seq", I32), ("kv_pages", I32), ("max_tokens", I32)]
+
+
+class PageReleaseDesc(ctypes.Structure):
+    _fields_ = [("slots", U64), ("keep_len", U64), ("seq_len", U64), ("page_table", U64), ("free_list", U64),
+                ("free_count", U64), ("seq_len_out", U64), ("free_count_out", U64), ("requests", I32),
+                ("max_seqs", I32), ("pages_per_seq", I32), ("kv_pages", I32)]
+
+
+class QkvAppendDesc(ctypes.Structure):
+    _fields_ = [("qkv", U64), ("q_norm", U64), ("k_norm", U64), ("cos", U64), ("sin", U64), ("tok_pos", U64),
+                ("slot_map", U64), ("q_out", U64), ("pool", U64), ("ld_qkv", I64), ("ld_q", I64), ("tokens", I32),
+                ("q_heads", I32), ("kv_heads", I32), ("head_dim", I32), ("rope_rows", I32), ("kv_pages", I32),
+                ("eps", ctypes.c_float)]
+
+
+class PagedAttnDesc(ctypes.Structure):
+    _fields_ = [("q", U64), ("pool", U64), ("page_table", U64), ("slots", U64), ("cu_seqlens", U64), ("kv_len", U64),
+                ("out", U64), ("workspace", U64), ("ld_q", I64), ("ld_out", I64), ("requests", I32), ("tokens", I32),
+                ("q_heads", I32), ("kv_heads", I32), ("head_dim", I32), ("max_seqs", I32), ("pages_per_seq", I32),
+                ("kv_pages", I32), ("scale", ctypes.c_float)]
+
+
 DEC_SWIGLU, DEC_RESID = 1, 2
 
 N.extra_signatures({
@@ -51,7 +78,12 @@ N.extra_signatures({
     "lrm_op_wait_probe": [P, U32, U32],
     "lrm_op_argmax_rows": [P, P, I32, I32, P],
     "lrm_op_decode_gemm": [P, ctypes.POINTER(DecodeGemmDesc)],
-}, {"lrm_op_decode_attention_workspace": U64})
+    "lrm_op_page_plan": [P, ctypes.POINTER(PagePlanDesc)],
+    "lrm_op_page_release": [P, ctypes.POINTER(PageReleaseDesc)],
+    "lrm_op_qkv_append": [P, ctypes.POINTER(QkvAppendDesc)],
+    "lrm_op_paged_attention_workspace": [I32, I32, I32],
+    "lrm_op_paged_attention": [P, ctypes.POINTER(PagedAttnDesc)],
+}, {"lrm_op_decode_attention_workspace": U64, "lrm_op_paged_attention_workspace": U64})
 
 # Scratch built into liblrmcuda.so for lrm_op_decode_attention_static (LRM_DECODE_ATTN_STATIC_SCRATCH_BYTES).
 DECODE_ATTN_STATIC_SCRATCH_BYTES = 16 << 20
@@ -152,3 +184,195 @@ def decode_attention_static(q, pool, page_table, seq_len, slots, out, pages_per_
                        pages_per_split, scale)
     N.check(N.lib().lrm_op_decode_attention_static(_stream(stream), ctypes.byref(d)), None,
             "decode_attention_static")
+
+
+# ---- a paged serving step on the device (include/lrm_cuda.h, same heading) -----------------------------------------
+#
+# plan -> append -> attention -> release, with lengths, page table and free pages kept on the device and no copy to or
+# from the host. These take tensors of any CUDA device (all of a call on one) and launch on `stream`, or on that
+# device's current stream. What only the device knows (slots, lengths, page ids) is checked there: error_word().
+
+def _need(ok, what):
+    if not ok:
+        raise ValueError(what)
+
+
+def _same_device(call, tensors):
+    """The device index that all of a call's tensors are on."""
+    dev = tensors[0].get_device()
+    for t in tensors:
+        if t.get_device() != dev or dev < 0:
+            raise ValueError(f"{call}: all tensors must be on one CUDA device")
+    return dev
+
+
+def _int32(call, **tensors):
+    """The tensors are contiguous int32."""
+    import torch
+
+    for name, t in tensors.items():
+        if t.dtype is not torch.int32 or not t.is_contiguous():
+            raise ValueError(f"{call}: {name} must be a contiguous int32 tensor")
+
+
+def _pool(call, pool):
+    import torch
+
+    if pool.dtype is not torch.bfloat16 or pool.dim() != 5 or pool.shape[2:] != (2, 16, 128) or \
+            not pool.is_contiguous():
+        raise ValueError(f"{call}: pool must be contiguous bfloat16 [pages, kv_heads, 2, 16, 128]")
+
+
+def _rows_of_heads(t):
+    """Whether only the rows of [T, heads, 128] are strided."""
+    return t.stride(2) == 1 and (t.stride(1) == 128 or t.shape[1] == 1)
+
+
+def _launch(call, fn, desc, dev, stream):
+    import torch
+
+    if dev == torch.cuda.current_device():
+        s = torch.cuda.current_stream(dev) if stream is None else stream
+        N.check(fn(s.cuda_stream, ctypes.byref(desc)), None, call)
+    else:
+        with torch.cuda.device(dev):
+            s = torch.cuda.current_stream(dev) if stream is None else stream
+            N.check(fn(s.cuda_stream, ctypes.byref(desc)), None, call)
+
+
+def page_plan(slots, new_len, seq_len, page_table, free_list, free_count, cu_seqlens, kv_len, tok_pos, slot_map,
+              seq_len_out=None, free_count_out=None, stream=None):
+    """Takes pages for each request's new tokens and writes the step's cu_seqlens [requests + 1], kv_len [requests],
+    tok_pos and slot_map [max_tokens]; int32 tensors throughout. slots [requests] (-1: padding) with new_len tokens
+    each; seq_len [max_seqs], page_table [max_seqs, pages_per_seq], free_list [kv_pages] and free_count [1] are the
+    cache's state, updated in place unless seq_len_out / free_count_out are given. All or nothing: a step that breaks a
+    rule (error_word 0x5001 .. 0x5004) takes no page and becomes a step of no tokens."""
+    call = "page_plan"
+    seq_len_out = seq_len if seq_len_out is None else seq_len_out
+    free_count_out = free_count if free_count_out is None else free_count_out
+    _int32(call, slots=slots, new_len=new_len, seq_len=seq_len, page_table=page_table, free_list=free_list,
+           free_count=free_count, cu_seqlens=cu_seqlens, kv_len=kv_len, tok_pos=tok_pos, slot_map=slot_map,
+           seq_len_out=seq_len_out, free_count_out=free_count_out)
+    n, seqs, tokens = slots.numel(), seq_len.numel(), tok_pos.numel()
+    _need(page_table.dim() == 2 and page_table.shape[0] == seqs and seq_len_out.numel() == seqs,
+          "page_plan: page_table must be [max_seqs, pages_per_seq] and seq_len, seq_len_out [max_seqs]")
+    _need(new_len.numel() == n and kv_len.numel() == n and cu_seqlens.numel() == n + 1 and slot_map.numel() == tokens
+          and free_count.numel() == 1 and free_count_out.numel() == 1,
+          "page_plan: new_len and kv_len are [requests], cu_seqlens [requests + 1], tok_pos and slot_map one size, "
+          "free_count and free_count_out one element")
+    dev = _same_device(call, (slots, new_len, seq_len, page_table, free_list, free_count, cu_seqlens, kv_len, tok_pos,
+                              slot_map, seq_len_out, free_count_out))
+    d = PagePlanDesc(slots.data_ptr(), new_len.data_ptr(), seq_len.data_ptr(), page_table.data_ptr(),
+                     free_list.data_ptr(), free_count.data_ptr(), cu_seqlens.data_ptr(), kv_len.data_ptr(),
+                     tok_pos.data_ptr(), slot_map.data_ptr(), seq_len_out.data_ptr(), free_count_out.data_ptr(), n,
+                     seqs, page_table.shape[1], free_list.numel(), tokens)
+    _launch(call, N.lib().lrm_op_page_plan, d, dev, stream)
+
+
+def page_release(slots, keep_len, seq_len, page_table, free_list, free_count, seq_len_out=None, free_count_out=None,
+                 stream=None):
+    """Cuts slots [requests] (-1: padding) back to their first keep_len tokens (0 frees a slot) and puts the pages
+    behind them back on top of the free list. State and outputs as in page_plan. All or nothing: a call that breaks a
+    rule (error_word 0x5011, 0x5012, 0x5014) changes nothing."""
+    call = "page_release"
+    seq_len_out = seq_len if seq_len_out is None else seq_len_out
+    free_count_out = free_count if free_count_out is None else free_count_out
+    _int32(call, slots=slots, keep_len=keep_len, seq_len=seq_len, page_table=page_table, free_list=free_list,
+           free_count=free_count, seq_len_out=seq_len_out, free_count_out=free_count_out)
+    n, seqs = slots.numel(), seq_len.numel()
+    _need(page_table.dim() == 2 and page_table.shape[0] == seqs and seq_len_out.numel() == seqs,
+          "page_release: page_table must be [max_seqs, pages_per_seq] and seq_len, seq_len_out [max_seqs]")
+    _need(keep_len.numel() == n and free_count.numel() == 1 and free_count_out.numel() == 1,
+          "page_release: keep_len is [requests], free_count and free_count_out one element")
+    dev = _same_device(call, (slots, keep_len, seq_len, page_table, free_list, free_count, seq_len_out,
+                              free_count_out))
+    d = PageReleaseDesc(slots.data_ptr(), keep_len.data_ptr(), seq_len.data_ptr(), page_table.data_ptr(),
+                        free_list.data_ptr(), free_count.data_ptr(), seq_len_out.data_ptr(),
+                        free_count_out.data_ptr(), n, seqs, page_table.shape[1], free_list.numel())
+    _launch(call, N.lib().lrm_op_page_release, d, dev, stream)
+
+
+def qkv_append(qkv, q_norm, k_norm, eps, cos, sin, tok_pos, slot_map, q_out, pool, stream=None):
+    """QK-RMSNorm, RoPE and the paged append of one fused projection qkv [T, (q_heads + 2 kv_heads) * 128] (bfloat16,
+    rows may be strided): q to q_out [T, q_heads, 128] (rows may be strided; may be a view of qkv's q columns), k and v
+    to pool [pages, kv_heads, 2, 16, 128] at slot_map [T] (int32 page * 16 + offset; -1 skips the row). q_norm, k_norm:
+    bfloat16 [128], or both None for no norm. cos, sin: float32 [rows, 64] read at tok_pos [T], or all three None for
+    no rotation."""
+    import torch
+
+    call = "qkv_append"
+    _pool(call, pool)
+    bf16 = torch.bfloat16
+    _need(qkv.dtype is bf16 and q_out.dtype is bf16 and qkv.dim() == 2 and q_out.dim() == 3 and q_out.shape[2] == 128
+          and q_out.shape[0] == qkv.shape[0],
+          "qkv_append: qkv must be bfloat16 [T, columns] and q_out bfloat16 [T, q_heads, 128]")
+    tokens, q_heads, kv_heads = qkv.shape[0], q_out.shape[1], pool.shape[1]
+    _need(qkv.shape[1] == (q_heads + 2 * kv_heads) * 128, "qkv_append: qkv has (q_heads + 2 kv_heads) * 128 columns")
+    _need(qkv.stride(1) == 1 and _rows_of_heads(q_out),
+          "qkv_append: only the rows of qkv and q_out may be strided")
+    _int32(call, slot_map=slot_map)
+    _need(slot_map.numel() == tokens, "qkv_append: slot_map is [T]")
+    tensors = [qkv, slot_map, q_out, pool]
+    if q_norm is not None or k_norm is not None:
+        _need(q_norm is not None and k_norm is not None, "qkv_append: give both gains or none")
+        for g in (q_norm, k_norm):
+            _need(g.dtype is bf16 and g.numel() == 128 and g.is_contiguous(),
+                  "qkv_append: q_norm and k_norm are contiguous bfloat16 [128]")
+        tensors += (q_norm, k_norm)
+    rope_rows = 0
+    if cos is not None or sin is not None:
+        _need(cos is not None and sin is not None and tok_pos is not None,
+              "qkv_append: give cos, sin and tok_pos, or none of them")
+        _int32(call, tok_pos=tok_pos)
+        for c in (cos, sin):
+            _need(c.dtype is torch.float32 and c.dim() == 2 and c.shape[1] == 64 and c.is_contiguous(),
+                  "qkv_append: cos and sin are contiguous float32 [rows, 64]")
+        _need(cos.shape == sin.shape and tok_pos.numel() == tokens,
+              "qkv_append: cos and sin have one shape and tok_pos is [T]")
+        rope_rows = cos.shape[0]
+        tensors += (cos, sin, tok_pos)
+    dev = _same_device(call, tensors)
+
+    def ptr(t):
+        return 0 if t is None else t.data_ptr()
+
+    d = QkvAppendDesc(qkv.data_ptr(), ptr(q_norm), ptr(k_norm), ptr(cos), ptr(sin), ptr(tok_pos) if rope_rows else 0,
+                      slot_map.data_ptr(), q_out.data_ptr(), pool.data_ptr(),
+                      qkv.stride(0) if tokens > 1 else qkv.shape[1], q_out.stride(0) if tokens > 1 else q_heads * 128,
+                      tokens, q_heads, kv_heads, 128, rope_rows, pool.shape[0], eps)
+    _launch(call, N.lib().lrm_op_qkv_append, d, dev, stream)
+
+
+def paged_attention_workspace(tokens, q_heads, kv_heads) -> int:
+    """Bytes of workspace for paged_attention calls of up to `tokens` rows on the current device."""
+    return int(N.lib().lrm_op_paged_attention_workspace(tokens, q_heads, kv_heads))
+
+
+def paged_attention(q, pool, page_table, slots, cu_seqlens, kv_len, out, workspace, scale, stream=None):
+    """Causal GQA attention of new tokens over the paged cache: rows cu_seqlens[i] .. cu_seqlens[i + 1] - 1 of q
+    [T, q_heads, 128] (bfloat16, rows may be strided, as may out's) are the last tokens of the kv_len[i] keys of slot
+    slots[i], read through page_table [max_seqs, pages_per_seq] from pool [pages, kv_heads, 2, 16, 128]. Rows of no
+    request are left as they were. workspace: paged_attention_workspace(T, ...) bytes, any contents."""
+    import torch
+
+    call = "paged_attention"
+    _pool(call, pool)
+    bf16 = torch.bfloat16
+    _need(q.dtype is bf16 and out.dtype is bf16 and q.dim() == 3 and q.shape[2] == 128 and out.shape == q.shape,
+          "paged_attention: q and out must be bfloat16 [T, q_heads, 128]")
+    _need(_rows_of_heads(q) and _rows_of_heads(out),
+          "paged_attention: only the rows of q and out may be strided")
+    _int32(call, page_table=page_table, slots=slots, cu_seqlens=cu_seqlens, kv_len=kv_len)
+    tokens, q_heads, kv_heads, n = q.shape[0], q.shape[1], pool.shape[1], slots.numel()
+    _need(page_table.dim() == 2 and kv_len.numel() == n and cu_seqlens.numel() == n + 1,
+          "paged_attention: page_table is [max_seqs, pages_per_seq], kv_len [requests], cu_seqlens [requests + 1]")
+    _need(workspace.is_contiguous(), "paged_attention: the workspace must be contiguous")
+    dev = _same_device(call, (q, pool, page_table, slots, cu_seqlens, kv_len, out, workspace))
+    lib = N.lib()
+    _need(workspace.numel() * workspace.element_size() >= lib.lrm_op_paged_attention_workspace(tokens, q_heads, kv_heads),
+          "paged_attention: the workspace is smaller than paged_attention_workspace says")
+    d = PagedAttnDesc(q.data_ptr(), pool.data_ptr(), page_table.data_ptr(), slots.data_ptr(), cu_seqlens.data_ptr(),
+                      kv_len.data_ptr(), out.data_ptr(), workspace.data_ptr(),
+                      q.stride(0) if tokens > 1 else q_heads * 128, out.stride(0) if tokens > 1 else q_heads * 128, n,
+                      tokens, q_heads, kv_heads, 128, page_table.shape[0], page_table.shape[1], pool.shape[0], scale)
+    _launch(call, lib.lrm_op_paged_attention, d, dev, stream)
