@@ -1,7 +1,31 @@
-// paged_attn.cu -- attention of each request's new tokens over its cached keys (lrm_op_paged_attention).
+// paged_attn.cu -- attention of each request's new tokens over its cached keys (lrm_op_paged_attention), on the
+// 5th-generation tensor cores (tcgen05, TMEM, TMA).
 //
-// o = sum_j p_j v_j / sum_j p_j with p_j = 2^(scale log2(e) q.k_j - m), m the running maximum: one pass over the keys.
-// One warp a (token, query head): 4 dims a lane, a key at a time.
+//   o = sum_j p_j v_j / sum_j p_j,   p_j = 2^(scale log2(e) q.k_j - m),   m a running reference maximum:
+// one pass over the keys, with the statistics and the accumulator in fp32 and p rounded to bf16 for the product with v.
+//
+// The work is cut evenly over one persistent CTA an SM (paged_sched.h): single tokens, verify chunks and prefill chunks
+// of any lengths fill the GPU alike. An item is up to 2 * floor(128 / group) tokens of one request and KV head. Its rows
+// are (token, query head) pairs, token-major, so the query heads that share a KV head share its tiles whatever the group
+// size, and one TMA box brings their q. 128 rows make a "slot" (S and O, 128 x 128 fp32 each, in tensor memory):
+//   wide    (more than 128 rows): each 128-key tile of K and V is used by both slots' rows;
+//   narrow  (up to 128 rows): one set of rows; the even key tiles go to slot 0 and the odd ones to slot 1, so one
+//           slot's products run under the other's softmax; the two states merge at the end.
+// Warps of a CTA:
+//   0       TMA producer: q of an item, then K_0, V_0, K_1, V_1, ... through a ring of five 32 KiB stages (8 pages of 16
+//           tokens, one box a page and 64 dims; 16 lanes issue them), running ahead into the next item;
+//   1       tensor-core issuer (one thread);
+//   2       scheduler: walks the CTA's range and hands the items to the others through a ring of four;
+//   4..11   softmax, one warpgroup a slot, thread = row.
+// Keys that a row does not see: their scores are replaced before the maximum, and their v, which the product multiplies
+// by 0, must not be infinite or NaN. So in tiles where some row's mask bites (the last tokens' own tiles) the softmax
+// warps test v in shared memory and zero what is not finite; if a key of the request itself was hit, the epilogue adds
+// its original values to the rows that see it.
+// Items that a cut passes through leave (m, sum p, unnormalised o) in the workspace, at most two a CTA, and
+// paged_combine_kernel merges them. Within a range the last item is walked first: CTAs that share a head's keys then
+// all start at key 0 of an item and stream the same tiles at about the same time, from L2.
+// Every wait is bounded and reports to the error word.
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <math.h>
@@ -9,63 +33,786 @@
 
 #include "internal.h"
 #include "paged.h"
+#include "paged_sched.h"
 #include "ptx.cuh"
 
 namespace lrm {
 namespace {
 
-__global__ void __launch_bounds__(128) paged_attn_kernel(PagedAttnArgs a) {
-    const int lane = threadIdx.x & 31, h = blockIdx.y * 4 + (threadIdx.x >> 5);
-    const int t = blockIdx.x;
-    // the request of row t: the last one that starts at or before it (requests without tokens start where the next does)
-    int lo = 0, hi = a.requests;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (a.cu_seqlens[mid] <= t)
-            lo = mid;
-        else
-            hi = mid;
+constexpr int TK = sched::kTileKeys, KV_ST = 5, SLOTS = 2, ITEMS = 4;
+constexpr int SUB = 128 * 64 * 2;  // one [128 rows][64] bf16 swizzled sub-tile
+constexpr int TILE = 2 * SUB;      // [128 rows][128]
+constexpr int P_SPLIT = 48;        // P is announced in two parts: keys 0..95 (48 packed columns), then 96..127
+constexpr int kThreads = 384;
+constexpr int kRegsLaunch = 168;  // 65536 / 384, rounded down to the allocation unit of 8
+constexpr int kRegsControl = 72, kRegsSoftmax = 216;
+static_assert(128 * kRegsControl + 256 * kRegsSoftmax <= kThreads * kRegsLaunch, "register split exceeds the launch");
+constexpr float kRescaleThreshold = 8.0f;  // log2 units: the reference maximum moves only when a tile exceeds it by more
+constexpr int kLeastUnits = 2;
+constexpr int kSmallBoxRows = 16;  // items of up to this many rows load q with a small box
+constexpr uint32_t kErrWaitProducer = 0x4010, kErrWaitIssuer = 0x4011, kErrWaitSoftmax = 0x4012, kErrWaitScheduler = 0x4013;
+
+// One item's share of a CTA's range: key tiles [kb, ke) of it.
+struct Item {
+    int tok0, ntok;     // its token rows in q and out; ntok 0 ends the list
+    int kvh, pos0;      // KV head; position of its first token
+    int kb, ke;
+    int npages, dest;   // pages of the request; dest -1: the whole item, else the partial slot 0 or 1
+    int64_t table;      // the request's first page-table entry
+};
+
+// An item whose last keys lie in later CTAs' ranges, left by the CTA that holds its first: partial slot 1 of this CTA
+// and slots 0 of the next `follow` CTAs make it up. ntok 0: none.
+struct Record {
+    int tok0, ntok, kvh, follow;
+};
+
+struct Control {
+    uint64_t q_full, q_empty, fin, o_free;
+    uint64_t kv_full[KV_ST], kv_empty[KV_ST];
+    uint64_t s_full[SLOTS], p_part[SLOTS], p_full[SLOTS], o_done[SLOTS];
+    uint64_t item_full[ITEMS], item_empty[ITEMS];
+    Item items[ITEMS];
+    uint64_t warp_sum[kThreads / 32];
+    uint64_t start_off;
+    int start_req;
+    uint32_t tmem;
+    int poison[SLOTS][2];  // [slot][item parity]: the item (counted from 1) in which v of a visible key was zeroed
+    float ml[SLOTS][128][2];
+};
+constexpr int SMEM_BYTES = (SLOTS + KV_ST) * TILE + (int)sizeof(Control);
+static_assert(SMEM_BYTES <= 227 * 1024, "shared memory of one CTA");
+
+struct Params {
+    PagedAttnArgs a;
+    int group, tt, rows_cap;  // query heads a KV head; tokens a slot; rows of a partial slot
+    float *part_o, *part_ml;
+    Record *records;
+};
+
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<uint32_t *>(&h);
+}
+__device__ __forceinline__ void add2(float &d0, float &d1, float a0, float a1) {
+    asm("{\n\t.reg .b64 a, d;\n\tmov.b64 d, {%0, %1};\n\tmov.b64 a, {%2, %3};\n\t"
+        "add.rn.f32x2 d, d, a;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "+f"(d0), "+f"(d1)
+        : "f"(a0), "f"(a1));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ bool finite_bf16(uint32_t h) { return (h & 0x7F80u) != 0x7F80u; }
+
+// A request's tokens and keys when it is sound and has any, else n = 0.
+struct Request {
+    int start, n, kv, slot;
+};
+__device__ __forceinline__ Request load_request(const PagedAttnArgs &a, int r, bool report) {
+    Request q;
+    q.start = a.cu_seqlens[r];
+    const int end = a.cu_seqlens[r + 1];
+    q.kv = a.kv_len[r];
+    q.slot = a.slots[r];
+    const int64_t n = (int64_t)end - q.start;
+    const bool ok = q.start >= 0 && n > 0 && end <= a.tokens && q.slot >= 0 && q.slot < a.max_seqs && q.kv >= n &&
+                    q.kv <= (int64_t)a.pages_per_seq * kPageTokens;
+    if (report && !ok && n != 0) atomicCAS(a.err, 0u, kErrAttnRequest);
+    q.n = ok ? (int)n : 0;
+    return q;
+}
+
+// Tests v in this warp's quarter of a tile (32 keys, one a lane) and zeroes what is not finite. Keys up to
+// `last_seen` (relative to the tile) are seen by some row: if one of them is hit, `poison` is set.
+__device__ __forceinline__ void clean_v(uint8_t *tile, int key, int lane, int last_seen, volatile int *poison, int id) {
+    const uint32_t row = ptx::smem_u32(tile) + key * 128;
+    __nv_bfloat162 acc = __floats2bfloat162_rn(0.f, 0.f);
+    const __nv_bfloat162 zero = acc;
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {  // chunks in an order that differs by lane: no bank conflicts
+            uint4 v = ptx::ld_shared_v4(row + half * SUB + (((c + lane) & 7) << 4));
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)  // 0 * v + acc: NaN once v is infinite or NaN
+                acc = __hfma2(*reinterpret_cast<const __nv_bfloat162 *>(&w[e]), zero, acc);
+        }
+    const float2 f = __bfloat1622float2(acc);
+    const bool hit = f.x != f.x || f.y != f.y;
+    if (hit && key <= last_seen) {
+        *poison = id;
+        __threadfence_block();  // seen before the zeros below are (the other warpgroup may find only those)
     }
-    const int start = a.cu_seqlens[lo], end = a.cu_seqlens[lo + 1];
-    if (t < start || t >= end || h >= a.q_heads) return;
-    const int slot = a.slots[lo], kv = a.kv_len[lo];
-    if (start < 0 || end > a.tokens || slot < 0 || slot >= a.max_seqs || kv < end - start ||
-        kv > (int64_t)a.pages_per_seq * kPageTokens) {
-        if (lane == 0) atomicCAS(a.err, 0u, kErrAttnRequest);
+    if (hit)
+#pragma unroll 1
+        for (int c = 0; c < 16; ++c) {
+            const uint32_t at = row + (c >> 3) * SUB + ((c & 7) << 4);
+            uint4 v = ptx::ld_shared_v4(at);
+            uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (!finite_bf16(w[e])) w[e] &= 0xFFFF0000u;
+                if (!finite_bf16(w[e] >> 16)) w[e] &= 0x0000FFFFu;
+            }
+            ptx::st_shared_v4(at, w[0], w[1], w[2], w[3]);
+        }
+    ptx::fence_proxy_async();  // the tensor core reads the tile through the async proxy
+}
+
+// Adds the values that clean_v zeroed, from the cache, to dims [c, c + 32) of a row that sees keys lo .. hi.
+__device__ __noinline__ void add_poison(const PagedAttnArgs &a, const Item &it, int lo, int hi, int c, float *o) {
+    for (int key = lo; key <= hi; ++key) {
+        const int pg = a.page_table[it.table + key / kPageTokens];
+        if (pg < 0 || pg >= a.kv_pages) continue;
+        const __nv_bfloat16 *v = a.pool + (size_t)pg * kv_page_elems(a.kv_heads) +
+                                 (size_t)(it.kvh * 2 + 1) * (kPageTokens * kHeadDim) + (key % kPageTokens) * kHeadDim + c;
+        for (int e = 0; e < 32; ++e) {
+            const float x = __bfloat162float(v[e]);
+            if (!(fabsf(x) < INFINITY)) o[e] += x;
+        }
+    }
+}
+
+__global__ void __launch_bounds__(kThreads, 1)
+    paged_attn_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tq_small,
+                      const __grid_constant__ CUtensorMap tkv, const __grid_constant__ Params p) {
+    ptx::griddep_wait();
+    ptx::griddep_launch();
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint8_t *sQ = smem;                // SLOTS tiles
+    uint8_t *sKV = sQ + SLOTS * TILE;  // KV_ST tiles: ring item 2j is K_j, 2j + 1 is V_j
+    Control &c = *reinterpret_cast<Control *>(sKV + KV_ST * TILE);
+    const PagedAttnArgs &a = p.a;
+    uint32_t *err = a.err;
+    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+    const int cta = blockIdx.x, span = SLOTS * p.tt;
+    if (ptx::smem_u32(smem) & 1023) {  // the swizzled tiles and their descriptors need 1024-byte alignment
+        if (tid == 0) {
+            atomicCAS(err, 0u, kErrWaitScheduler);
+            p.records[cta] = Record{0, 0, 0, 0};
+        }
         return;
     }
-    const int pos = kv - (end - t);
-    const int kvh = h / (a.q_heads / a.kv_heads);
-    float q[4], o[4] = {}, m = -INFINITY, l = 0.f;
-    for (int e = 0; e < 4; ++e) q[e] = __bfloat162float(a.q[(size_t)t * a.ld_q + h * kHeadDim + 4 * lane + e]);
-    for (int j = 0; j <= pos; ++j) {
-        const int pg = a.page_table[(size_t)slot * a.pages_per_seq + j / kPageTokens];
-        const bool good = pg >= 0 && pg < a.kv_pages;
-        if (!good && lane == 0) atomicCAS(a.err, 0u, kErrAttnPage);
-        const __nv_bfloat16 *k = a.pool + (size_t)(good ? pg : 0) * kv_page_elems(a.kv_heads) +
-                                 (size_t)kvh * 2 * kPageTokens * kHeadDim + (j % kPageTokens) * kHeadDim + 4 * lane;
-        float s = 0.f;
-        for (int e = 0; e < 4; ++e) s += good ? q[e] * __bfloat162float(k[e]) : 0.f;
-        for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-        s *= a.scale_log2;
-        const float m2 = fmaxf(m, s), f = m == -INFINITY ? 0.f : exp2f(m - m2);
-        const float p = exp2f(s - (m2 == -INFINITY ? 0.f : m2));
-        m = m2;
-        l = l * f + p;
-        for (int e = 0; e < 4; ++e)
-            o[e] = o[e] * f + (good ? p * __bfloat162float(k[kPageTokens * kHeadDim + e]) : 0.f);
+
+    // ---- this CTA's range ----
+    // Units of each thread's requests, their exclusive sums over the threads, and the request of the range's last unit.
+    const int per = (a.requests + kThreads - 1) / kThreads;
+    const int r0 = min(a.requests, tid * per), r1 = min(a.requests, r0 + per);
+    uint64_t own = 0;
+    for (int r = r0; r < r1; ++r) {
+        const Request q = load_request(a, r, cta == 0);
+        if (q.n) own += sched::head_units(q.n, q.kv, span) * (uint64_t)a.kv_heads;
     }
-    for (int e = 0; e < 4; ++e)
-        a.out[(size_t)t * a.ld_out + h * kHeadDim + 4 * lane + e] = __float2bfloat16_rn(o[e] / l);
+    uint64_t incl = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint64_t x = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += x;
+    }
+    if (lane == 31) c.warp_sum[warp] = incl;
+    if (tid == 0) {
+        ptx::mbar_init(&c.q_full, 1);
+        ptx::mbar_init(&c.q_empty, 1);
+        ptx::mbar_init(&c.fin, 1);
+        ptx::mbar_init(&c.o_free, 8);
+        for (int s = 0; s < KV_ST; ++s) {
+            ptx::mbar_init(&c.kv_full[s], 1);
+            ptx::mbar_init(&c.kv_empty[s], 1);
+        }
+        for (int s = 0; s < SLOTS; ++s) {
+            ptx::mbar_init(&c.s_full[s], 1);
+            ptx::mbar_init(&c.p_part[s], 4);
+            ptx::mbar_init(&c.p_full[s], 4);
+            ptx::mbar_init(&c.o_done[s], 1);
+            c.poison[s][0] = c.poison[s][1] = 0;
+        }
+        for (int s = 0; s < ITEMS; ++s) {
+            ptx::mbar_init(&c.item_full[s], 1);
+            ptx::mbar_init(&c.item_empty[s], 10);  // producer, issuer, eight softmax warps
+        }
+        ptx::fence_barrier_init();
+        ptx::prefetch_tmap(&tq);
+        ptx::prefetch_tmap(&tq_small);
+        ptx::prefetch_tmap(&tkv);
+    }
+    if (warp == 1) {
+        ptx::tmem_alloc(&c.tmem, 512);
+        ptx::tmem_relinquish();
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    uint64_t before = incl - own, units = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) {
+        if (w < warp) before += c.warp_sum[w];
+        units += c.warp_sum[w];
+    }
+    const uint32_t tmem = c.tmem;
+    const int ctas = sched::ctas_of(units, (int)gridDim.x, kLeastUnits);
+    const bool idle = cta >= ctas;
+    const uint64_t u0 = idle ? 0 : sched::cut(units, ctas, cta), u1 = idle ? 0 : sched::cut(units, ctas, cta + 1);
+    if (!idle && before <= u1 - 1 && u1 - 1 < before + own) {
+        uint64_t at = before;
+        for (int r = r0; r < r1; ++r) {
+            const Request q = load_request(a, r, false);
+            if (!q.n) continue;
+            const uint64_t w = sched::head_units(q.n, q.kv, span) * (uint64_t)a.kv_heads;
+            if (u1 - 1 < at + w) {
+                c.start_req = r;
+                c.start_off = u1 - 1 - at;
+                break;
+            }
+            at += w;
+        }
+    }
+    __syncthreads();
+
+    if (idle) {
+        if (tid == 0) p.records[cta] = Record{0, 0, 0, 0};
+    } else if (warp < 4) {
+        ptx::setmaxnreg_dec<kRegsControl>();
+        if (warp == 2) {
+            // ---- scheduler ----
+            if (lane == 0) {
+                int r = c.start_req;
+                Request q = load_request(a, r, false);
+                uint64_t off = c.start_off, head = sched::head_units(q.n, q.kv, span), left = u1 - u0, u_end = u1;
+                int h = (int)(off / head), i = sched::item_at(q.n, q.kv, span, off % head);
+                int tiles = sched::item_tiles(q.n, q.kv, span, i);
+                int ke = (int)(off % head - sched::units_before(q.n, q.kv, span, i)) + 1;
+                Record rec = {0, 0, 0, 0};
+                int k = 0;
+                bool ok = true;
+                while (ok) {
+                    ok = ptx::mbar_wait(&c.item_empty[k % ITEMS], ((k / ITEMS) & 1) ^ 1, err, kErrWaitScheduler);
+                    if (!ok) break;
+                    Item it = {};
+                    if (left > 0) {
+                        it.kb = (uint64_t)ke > left ? ke - (int)left : 0;
+                        it.ke = ke;
+                        it.tok0 = q.start + i * span;
+                        it.ntok = min(span, q.n - i * span);
+                        it.kvh = h;
+                        it.pos0 = q.kv - q.n + i * span;
+                        it.npages = (q.kv + kPageTokens - 1) / kPageTokens;
+                        it.table = (int64_t)q.slot * a.pages_per_seq;
+                        it.dest = it.kb == 0 && ke == tiles ? -1 : (it.kb == 0 ? 1 : 0);
+                        if (it.dest == 1)  // the item ends at unit u_end + (tiles - ke)
+                            rec = Record{it.tok0, it.ntok, h,
+                                         sched::cta_of(units, ctas, u_end + (uint64_t)(tiles - ke) - 1) - cta};
+                    }
+                    c.items[k % ITEMS] = it;
+                    ptx::mbar_arrive(&c.item_full[k % ITEMS]);
+                    ++k;
+                    if (left == 0) break;
+                    left -= (uint64_t)(ke - it.kb);
+                    u_end -= (uint64_t)(ke - it.kb);
+                    if (left == 0) continue;
+                    // the item before: of this head, else of the head before, else of the request before
+                    if (i > 0) {
+                        --i;
+                    } else {
+                        if (h > 0) {
+                            --h;
+                        } else {
+                            do q = load_request(a, --r, false);
+                            while (!q.n);
+                            h = a.kv_heads - 1;
+                        }
+                        i = sched::items_of(q.n, span) - 1;
+                    }
+                    tiles = ke = sched::item_tiles(q.n, q.kv, span, i);
+                }
+                p.records[cta] = rec;
+            }
+        } else if (warp == 0) {
+            // ---- TMA producer ----
+            const int oob = a.kv_pages * a.kv_heads * 2;  // past the tensor map: read as zeros, without a memory access
+            int ring = 0;  // ring items issued so far
+            bool ok = true;
+            for (int k = 0; ok; ++k) {
+                if (lane == 0) ok = ptx::mbar_wait(&c.item_full[k % ITEMS], (k / ITEMS) & 1, err, kErrWaitProducer);
+                ok = __shfl_sync(0xffffffffu, ok, 0);
+                if (!ok) break;
+                const Item it = c.items[k % ITEMS];
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(&c.item_empty[k % ITEMS]);
+                if (it.ntok == 0) break;
+                // z coordinates (K block of page and head) of 4 tiles' pages, one a lane; the next 4 tiles' are fetched
+                // while these are issued
+                auto fetch = [&](int tile) {
+                    const int pg = tile * 8 + lane;
+                    if (pg >= it.npages) return oob;  // keys past the request, which no row sees
+                    const int id = a.page_table[it.table + pg];
+                    if ((uint32_t)id < (uint32_t)a.kv_pages) return (id * a.kv_heads + it.kvh) * 2;
+                    atomicCAS(err, 0u, kErrAttnPage);
+                    return oob;
+                };
+                int z = fetch(it.kb), z_next = it.kb + 4 < it.ke ? fetch(it.kb + 4) : oob;
+                if (lane == 0) {
+                    ok = ptx::mbar_wait(&c.q_empty, (k & 1) ^ 1, err, kErrWaitProducer);
+                    if (ok) {
+                        const bool small = it.ntok * p.group <= kSmallBoxRows;
+                        const int slots = it.ntok > p.tt ? 2 : 1;
+                        const int box_tok = small ? max(1, kSmallBoxRows / p.group) : p.tt;
+                        const CUtensorMap *map = small ? &tq_small : &tq;
+                        ptx::mbar_arrive_expect_tx(&c.q_full, slots * box_tok * p.group * 256);
+                        for (int s = 0; s < slots; ++s)
+                            for (int half = 0; half < 2; ++half)
+                                ptx::tma_load_3d(sQ + s * TILE + half * SUB, map, &c.q_full, 64 * half, it.kvh * p.group,
+                                                 it.tok0 + s * p.tt);
+                    }
+                }
+                ok = __shfl_sync(0xffffffffu, ok, 0);
+                for (int t = it.kb; ok && t < it.ke; ++t) {
+                    const int sub = (t - it.kb) & 3;
+                    if (sub == 0 && t != it.kb) {
+                        z = z_next;
+                        z_next = t + 4 < it.ke ? fetch(t + 4) : oob;
+                    }
+                    const int zt = __shfl_sync(0xffffffffu, z, sub * 8 + (lane >> 1));  // lanes 0..15: page lane / 2
+                    for (int kv = 0; ok && kv < 2; ++kv, ++ring) {
+                        const int st = ring % KV_ST;
+                        if (lane == 0) {
+                            ok = ptx::mbar_wait(&c.kv_empty[st], ((ring / KV_ST) & 1) ^ 1, err, kErrWaitProducer);
+                            if (ok) ptx::mbar_arrive_expect_tx(&c.kv_full[st], TILE);
+                        }
+                        ok = __shfl_sync(0xffffffffu, ok, 0);
+                        if (!ok) break;
+                        if (lane < 16)
+                            ptx::tma_load_3d(sKV + st * TILE + (lane & 1) * SUB + (lane >> 1) * 2048, &tkv, &c.kv_full[st],
+                                             64 * (lane & 1), 0, zt + kv);
+                    }
+                }
+            }
+            // Our own copies in flight must land before the CTA exits (this matters on the error path).
+            for (int x = ring > KV_ST ? ring - KV_ST : 0; x < ring; ++x)
+                ptx::mbar_wait(&c.kv_full[x % KV_ST], (x / KV_ST) & 1, err, kErrWaitProducer);
+        } else if (warp == 1) {
+            // ---- tensor-core issuer ----
+            if (ptx::elect_one()) {
+                constexpr uint32_t idesc_qk = ptx::idesc_bf16_f32(128, 128, false);
+                constexpr uint32_t idesc_pv = ptx::idesc_bf16_f32(128, 128, true);
+                int ring = 0;              // ring items of the items before this one
+                uint32_t steps[SLOTS] = {};  // P tiles consumed so far, a slot
+                bool ok = true;
+                auto wait = [&](uint64_t *bar, uint32_t parity) {
+                    if (ok) ok = ptx::mbar_wait(bar, parity, err, kErrWaitIssuer);
+                    ptx::tc_fence_after();
+                    return ok;
+                };
+                auto wait_ring = [&](int x) { return wait(&c.kv_full[x % KV_ST], (x / KV_ST) & 1); };
+                // S_s = Q_q K^T of the K tile in ring item x, announced on s_full[s]
+                auto qk = [&](int s, int q, int x) {
+                    const uint32_t aQ = ptx::smem_u32(sQ + q * TILE), aK = ptx::smem_u32(sKV + (x % KV_ST) * TILE);
+#pragma unroll
+                    for (int kk = 0; kk < 8; ++kk) {
+                        const uint32_t o = (kk >> 2) * SUB + (kk & 3) * 32;
+                        ptx::mma_bf16(tmem + 256 * s, ptx::sw128_kmajor_desc(aQ + o), ptx::sw128_kmajor_desc(aK + o),
+                                      idesc_qk, kk > 0 ? 1u : 0u);
+                    }
+                    ptx::mma_commit(&c.s_full[s]);
+                };
+                // O_s (+)= P_s V of the V tile in ring item x, as P's two parts are written
+                auto pv = [&](int s, int x, bool first) {
+                    const uint32_t tO = tmem + 256 * s + 128, tP = tmem + 256 * s;
+                    const uint32_t aV = ptx::smem_u32(sKV + (x % KV_ST) * TILE);
+                    if (!wait(&c.p_part[s], steps[s] & 1)) return;
+#pragma unroll
+                    for (int kk = 0; kk < 6; ++kk)
+                        ptx::mma_bf16_ts(tO, tP + kk * 8, ptx::sw128_mnmajor_desc(aV + kk * 2048, SUB, 1024), idesc_pv,
+                                         (!first || kk > 0) ? 1u : 0u);
+                    if (!wait(&c.p_full[s], steps[s] & 1)) return;
+#pragma unroll
+                    for (int kk = 6; kk < 8; ++kk)
+                        ptx::mma_bf16_ts(tO, tP + kk * 8, ptx::sw128_mnmajor_desc(aV + kk * 2048, SUB, 1024), idesc_pv, 1u);
+                    ++steps[s];
+                };
+                for (int k = 0; ok; ++k) {
+                    if (!wait(&c.item_full[k % ITEMS], (k / ITEMS) & 1)) break;
+                    const int ntok = c.items[k % ITEMS].ntok;
+                    const int nt = c.items[k % ITEMS].ke - c.items[k % ITEMS].kb;
+                    ptx::mbar_arrive(&c.item_empty[k % ITEMS]);
+                    if (ntok == 0) break;
+                    const bool wide = ntok > p.tt;
+                    if (!wait(&c.q_full, k & 1) || !wait_ring(ring)) break;
+                    // The first scores. The tensor core runs this thread's MMAs in order, so they overwrite P of the
+                    // item before only after its last product has read it.
+                    qk(0, 0, ring);
+                    if (wide) qk(1, 1, ring);
+                    ptx::mma_commit(&c.kv_empty[ring % KV_ST]);
+                    if (!wide && nt > 1) {
+                        if (!wait_ring(ring + 2)) break;
+                        qk(1, 0, ring + 2);
+                        ptx::mma_commit(&c.kv_empty[(ring + 2) % KV_ST]);
+                    }
+                    if (nt <= (wide ? 1 : 2)) ptx::mma_commit(&c.q_empty);
+                    // O may be overwritten once the item before has been read out
+                    if (k > 0 && !wait(&c.o_free, (k - 1) & 1)) break;
+                    if (wide) {
+                        for (int j = 0; ok && j < nt; ++j) {
+                            const int xv = ring + 2 * j + 1;
+                            if (!wait_ring(xv)) break;
+                            for (int s = 0; s < 2; ++s) {
+                                pv(s, xv, j == 0);
+                                if (!ok) break;
+                                if (s == 1) ptx::mma_commit(&c.kv_empty[xv % KV_ST]);
+                                if (j + 1 == nt) {
+                                    ptx::mma_commit(&c.o_done[s]);
+                                    continue;
+                                }
+                                if (s == 0 && !wait_ring(xv + 1)) break;
+                                qk(s, s, xv + 1);
+                                if (s == 1) ptx::mma_commit(&c.kv_empty[(xv + 1) % KV_ST]);
+                                if (s == 1 && j + 2 == nt) ptx::mma_commit(&c.q_empty);
+                            }
+                        }
+                    } else {
+                        for (int j = 0; ok && j < nt; ++j) {
+                            const int xv = ring + 2 * j + 1, s = j & 1;
+                            if (!wait_ring(xv)) break;
+                            pv(s, xv, j < 2);
+                            if (!ok) break;
+                            ptx::mma_commit(&c.kv_empty[xv % KV_ST]);
+                            if (j + 2 >= nt) {
+                                ptx::mma_commit(&c.o_done[s]);
+                                continue;
+                            }
+                            if (!wait_ring(xv + 3)) break;
+                            qk(s, 0, xv + 3);
+                            ptx::mma_commit(&c.kv_empty[(xv + 3) % KV_ST]);
+                            if (j + 3 == nt) ptx::mma_commit(&c.q_empty);
+                        }
+                    }
+                    ring += 2 * nt;
+                }
+                // No MMA may still be writing TMEM when it is freed (this matters on the error path).
+                ptx::mma_commit(&c.fin);
+                ptx::mbar_wait(&c.fin, 0, err, kErrWaitIssuer);
+            }
+        }
+    } else {
+        // ---- softmax ----
+        ptx::setmaxnreg_inc<kRegsSoftmax>();
+        const int s = (warp - 4) >> 2;  // slot
+        const int quarter = warp & 3;   // TMEM lanes this warp may access
+        const int rl = quarter * 32 + lane;
+        const int tl = rl / p.group, hl = rl - tl * p.group;  // this row's token (of the slot) and query head (of the group)
+        const int warp_tl = (quarter * 32) / p.group;         // the warp's first token
+        const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+        const uint32_t tS = tmem + 256 * s + lanes;
+        const float sc = a.scale_log2;
+        int ring = 0;
+        uint32_t steps = 0, done[SLOTS] = {};  // S tiles taken from this slot; items that used each slot
+        bool ok = true;
+        for (int k = 0; ok; ++k) {
+            if (!ptx::mbar_wait(&c.item_full[k % ITEMS], (k / ITEMS) & 1, err, kErrWaitSoftmax)) break;
+            const Item it = c.items[k % ITEMS];
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(&c.item_empty[k % ITEMS]);
+            if (it.ntok == 0) break;
+            const bool wide = it.ntok > p.tt;
+            const int token = wide ? s * p.tt + tl : tl;  // of the item
+            const bool valid = tl < p.tt && token < it.ntok;
+            const int warp_token = wide ? s * p.tt + warp_tl : warp_tl;
+            const bool active = warp_tl < p.tt && warp_token < it.ntok;  // some row of the warp is real
+            const int nt = it.ke - it.kb;
+            float m_ref = -INFINITY, l = 0.f;
+            bool first = true;
+            for (int j = wide ? 0 : s; j < nt; j += wide ? 1 : 2, ++steps) {
+                if (!ptx::mbar_wait(&c.s_full[s], steps & 1, err, kErrWaitSoftmax)) {
+                    ok = false;
+                    break;
+                }
+                ptx::tc_fence_after();
+                const int key0 = (it.kb + j) * TK;
+                const bool dirty = key0 + TK - 1 > it.pos0;  // some row of the item does not see the whole tile
+                uint32_t pk[64];
+                if (active) {
+                    float x[128];
+                    ptx::tmem_ld32(tS, reinterpret_cast<uint32_t *>(x));
+                    ptx::tmem_ld32(tS + 32, reinterpret_cast<uint32_t *>(x) + 32);
+                    ptx::tmem_ld32(tS + 64, reinterpret_cast<uint32_t *>(x) + 64);
+                    ptx::tmem_ld32(tS + 96, reinterpret_cast<uint32_t *>(x) + 96);
+                    ptx::tmem_ld_wait();
+                    if (key0 + TK - 1 > it.pos0 + warp_token) {
+                        const int lim = it.pos0 + token - key0;  // keys 0..lim of the tile are visible
+#pragma unroll
+                        for (int e = 0; e < 128; ++e) x[e] = e <= lim ? x[e] : -INFINITY;
+                    }
+                    float mx[8];
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) mx[u] = fmaxf(x[u], x[u + 8]);
+#pragma unroll
+                    for (int e = 16; e < 128; e += 16) {
+#pragma unroll
+                        for (int u = 0; u < 8; ++u) mx[u] = max3(mx[u], x[e + u], x[e + 8 + u]);
+                    }
+                    const float tmax =
+                        fmaxf(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], max3(mx[5], mx[6], mx[7]))) * sc;
+                    bool rescale = false;
+                    float alpha = 1.f;
+                    if (first) {
+                        m_ref = tmax;
+                    } else if (valid && tmax > m_ref + kRescaleThreshold) {
+                        alpha = ptx::ex2(m_ref - tmax);  // 0 when nothing was visible before
+                        m_ref = tmax;
+                        rescale = true;
+                    }
+                    if (__any_sync(0xffffffffu, rescale)) {
+                        // this S was issued behind the slot's last product, so O is quiescent
+                        l *= alpha;
+#pragma unroll 1
+                        for (int col = 0; col < 128; col += 32) {
+                            uint32_t u[32];
+                            ptx::tmem_ld32(tS + 128 + col, u);
+                            ptx::tmem_ld_wait();
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) u[e] = __float_as_uint(__uint_as_float(u[e]) * alpha);
+                            ptx::tmem_st32(tS + 128 + col, u);
+                        }
+                    }
+                    const float nm = m_ref == -INFINITY ? 0.f : -m_ref;  // a row that has seen no key yet: p = 0
+                    float la = 0.f, lb = 0.f, lc = 0.f, ld = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 64; ++e) {
+                        float u, v;
+                        ptx::fma_x2(u, v, x[2 * e], x[2 * e + 1], sc, sc, nm, nm);
+                        u = ptx::ex2(u);
+                        v = ptx::ex2(v);
+                        if (e & 1)
+                            add2(lc, ld, u, v);
+                        else
+                            add2(la, lb, u, v);
+                        pk[e] = pack2(u, v);
+                    }
+                    l += (la + lb) + (lc + ld);
+                    ptx::tmem_st32(tS, pk);
+                    ptx::tmem_st16(tS + 32, *reinterpret_cast<const uint32_t(*)[16]>(pk + 32));
+                }
+                first = false;
+                if (dirty) {
+                    const int xv = ring + 2 * j + 1;
+                    if (!ptx::mbar_wait(&c.kv_full[xv % KV_ST], (xv / KV_ST) & 1, err, kErrWaitSoftmax)) {
+                        ok = false;
+                        break;
+                    }
+                    clean_v(sKV + (xv % KV_ST) * TILE, rl, lane, it.pos0 + it.ntok - 1 - key0, &c.poison[s][k & 1], k + 1);
+                }
+                if (active) ptx::tmem_st_wait();
+                ptx::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(&c.p_part[s]);
+                if (active) {
+                    ptx::tmem_st16(tS + P_SPLIT, *reinterpret_cast<const uint32_t(*)[16]>(pk + P_SPLIT));
+                    ptx::tmem_st_wait();
+                }
+                ptx::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(&c.p_full[s]);
+            }
+            if (!ok) break;
+            ring += 2 * nt;
+
+            // ---- epilogue ----
+            const bool used1 = wide || nt > 1;
+            auto wait_done = [&](int slot) {
+                if (!ptx::mbar_wait(&c.o_done[slot], done[slot] & 1, err, kErrWaitSoftmax)) ok = false;
+                ++done[slot];
+                ptx::tc_fence_after();
+                return ok;
+            };
+            if (wide && s == 1) {
+                if (!wait_done(0) || !wait_done(1)) break;
+            } else {
+                if (!wait_done(0)) break;
+                if (!wide && used1 && !wait_done(1)) break;
+            }
+            float w[SLOTS] = {1.f, 0.f};  // weights of the two slots' states (narrow)
+            if (!wide) {
+                // both warpgroups hold the same rows: exchange the states, then each takes half of the dims
+                c.ml[s][rl][0] = m_ref;
+                c.ml[s][rl][1] = l;
+                ptx::named_barrier(1, 256);
+                const float m0 = c.ml[0][rl][0], l0 = c.ml[0][rl][1];
+                const float m1 = c.ml[1][rl][0], l1 = used1 ? c.ml[1][rl][1] : 0.f;
+                m_ref = l0 == 0.f ? m1 : (l1 == 0.f ? m0 : fmaxf(m0, m1));
+                w[0] = l0 == 0.f ? 0.f : ptx::ex2(m0 - m_ref);
+                w[1] = l1 == 0.f ? 0.f : ptx::ex2(m1 - m_ref);
+                l = (l0 == 0.f ? 0.f : w[0] * l0) + (l1 == 0.f ? 0.f : w[1] * l1);
+            }
+            const bool poisoned = c.poison[0][k & 1] == k + 1 || c.poison[1][k & 1] == k + 1;
+            if (active) {
+                const int row = token * p.group + hl;
+                const size_t part = ((size_t)cta * 2 + (it.dest > 0)) * p.rows_cap + row;
+                const float inv = 1.f / l;
+                const int c0 = wide ? 0 : 64 * s, c1 = wide ? 128 : 64 * s + 64;
+#pragma unroll 1
+                for (int col = c0; col < c1; col += 32) {
+                    float o[32];
+                    if (wide) {
+                        ptx::tmem_ld32(tS + 128 + col, reinterpret_cast<uint32_t *>(o));
+                        ptx::tmem_ld_wait();
+                    } else {
+                        uint32_t o1[32];
+                        ptx::tmem_ld32(tmem + lanes + 128 + col, reinterpret_cast<uint32_t *>(o));
+                        if (used1) ptx::tmem_ld32(tmem + lanes + 256 + 128 + col, o1);
+                        ptx::tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            o[e] = w[0] == 0.f ? 0.f : w[0] * o[e];
+                            if (used1 && w[1] != 0.f) o[e] += w[1] * __uint_as_float(o1[e]);
+                        }
+                    }
+                    if (poisoned && valid)
+                        add_poison(a, it, max(it.kb * TK, it.pos0 / TK * TK), min(it.pos0 + token, it.ke * TK - 1), col, o);
+                    if (!valid) continue;
+                    if (it.dest < 0) {
+                        uint4 *d = reinterpret_cast<uint4 *>(a.out + (size_t)(it.tok0 + token) * a.ld_out +
+                                                             (size_t)(it.kvh * p.group + hl) * kHeadDim + col);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            d[e] = make_uint4(pack2(o[8 * e] * inv, o[8 * e + 1] * inv),
+                                              pack2(o[8 * e + 2] * inv, o[8 * e + 3] * inv),
+                                              pack2(o[8 * e + 4] * inv, o[8 * e + 5] * inv),
+                                              pack2(o[8 * e + 6] * inv, o[8 * e + 7] * inv));
+                    } else {
+                        float4 *d = reinterpret_cast<float4 *>(p.part_o + part * kHeadDim + col);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            d[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                        if (col == 0) *reinterpret_cast<float2 *>(p.part_ml + part * 2) = make_float2(m_ref, l);
+                    }
+                }
+            }
+            ptx::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(&c.o_free);
+            if (wide && s == 0 && !wait_done(1)) break;  // keeps in step with the slot's barrier
+        }
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    if (warp == 1) ptx::tmem_dealloc(tmem, 512);
+}
+
+// Merges the partial results of the items that a cut passes through: o = sum 2^(m_i - m) o_i / sum 2^(m_i - m) l_i in the
+// order of their keys. Block (CTA, 8 rows), a warp a row, 4 dims a lane.
+__global__ void __launch_bounds__(256) paged_combine_kernel(Params p) {
+    ptx::griddep_wait();
+    const Record rec = p.records[blockIdx.x];
+    const int row = blockIdx.y * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
+    if (row >= rec.ntok * p.group) return;
+    const int n = rec.follow + 1;
+    // partial i: slot 1 of the record's CTA, then slot 0 of each CTA behind it
+    auto at = [&](int i) { return ((size_t)(blockIdx.x + i) * 2 + (i == 0)) * p.rows_cap + row; };
+    float m = -INFINITY;
+    for (int i = lane; i < n; i += 32) {
+        const float2 ml = *reinterpret_cast<const float2 *>(p.part_ml + at(i) * 2);
+        if (ml.y != 0.f) m = fmaxf(m, ml.x);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+        const float2 ml = *reinterpret_cast<const float2 *>(p.part_ml + at(i) * 2);
+        const float4 o = *reinterpret_cast<const float4 *>(p.part_o + at(i) * kHeadDim + 4 * lane);
+        if (ml.y == 0.f) continue;  // the row saw none of this part's keys
+        const float w = ptx::ex2(ml.x - m);
+        l += w * ml.y;
+        acc.x += w * o.x;
+        acc.y += w * o.y;
+        acc.z += w * o.z;
+        acc.w += w * o.w;
+    }
+    const float inv = 1.f / l;
+    const int token = row / p.group, h = row - token * p.group;
+    *reinterpret_cast<uint2 *>(p.a.out + (size_t)(rec.tok0 + token) * p.a.ld_out +
+                               (size_t)(rec.kvh * p.group + h) * kHeadDim + 4 * lane) =
+        make_uint2(pack2(acc.x * inv, acc.y * inv), pack2(acc.z * inv, acc.w * inv));
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                  const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_tiled_fn() {
+    static const EncodeTiledFn fn = [] {
+        void *ptr = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            return (EncodeTiledFn)ptr;
+        return (EncodeTiledFn) nullptr;
+    }();
+    return fn;
+}
+
+// bf16 [z][y][128] with the given y and z strides (bytes), boxes of 64 x by x bz, 128-byte swizzle.
+bool make_tmap(CUtensorMap *map, const void *ptr, uint64_t y, uint64_t z, uint64_t ystride, uint64_t zstride, uint32_t by,
+               uint32_t bz) {
+    EncodeTiledFn enc = encode_tiled_fn();
+    if (!enc) return false;
+    const cuuint64_t dims[3] = {128, y, z}, strides[2] = {ystride, zstride};
+    const cuuint32_t box[3] = {64, by, bz}, estr[3] = {1, 1, 1};
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(ptr), dims, strides, box, estr,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Rows of a partial slot: those of an item, which a call of `tokens` rows bounds too.
+int partial_rows(int tokens, int q_heads, int kv_heads) {
+    const int group = q_heads / kv_heads, span = 2 * (sched::kTileRows / group);
+    return (tokens < span ? tokens : span) * group;
 }
 
 }  // namespace
 
-uint64_t paged_attention_workspace(int tokens, int q_heads, int kv_heads, int sms) { return 16; }
+uint64_t paged_attention_workspace(int tokens, int q_heads, int kv_heads, int sms) {
+    return (uint64_t)sms * (2 * (uint64_t)partial_rows(tokens, q_heads, kv_heads) * (kHeadDim + 2) * sizeof(float) +
+                            sizeof(Record));
+}
 
 cudaError_t launch_paged_attention(const PagedAttnArgs &a, int sms, cudaStream_t st) {
-    paged_attn_kernel<<<dim3(a.tokens, (a.q_heads + 3) / 4), 128, 0, st>>>(a);
-    return cudaGetLastError();
+    Params p;
+    p.a = a;
+    p.group = a.q_heads / a.kv_heads;
+    p.tt = sched::kTileRows / p.group;
+    p.rows_cap = partial_rows(a.tokens, a.q_heads, a.kv_heads);
+    p.records = reinterpret_cast<Record *>(a.workspace);
+    p.part_o = reinterpret_cast<float *>(p.records + sms);
+    p.part_ml = p.part_o + (size_t)sms * 2 * p.rows_cap * kHeadDim;
+    const uint32_t small = kSmallBoxRows / p.group > 0 ? kSmallBoxRows / p.group : 1;
+    CUtensorMap tq, tq_small, tkv;
+    const uint64_t qrow = (uint64_t)a.ld_q * 2;
+    if (!make_tmap(&tq, a.q, a.q_heads, a.tokens, kHeadDim * 2, qrow, p.group, p.tt) ||
+        !make_tmap(&tq_small, a.q, a.q_heads, a.tokens, kHeadDim * 2, qrow, p.group, small) ||
+        !make_tmap(&tkv, a.pool, kPageTokens, (uint64_t)a.kv_pages * a.kv_heads * 2, kHeadDim * 2,
+                   kPageTokens * kHeadDim * 2, kPageTokens, 1))
+        return cudaErrorInvalidValue;
+    static SmemOptIn opt;
+    if (cudaError_t e = opt.set((const void *)paged_attn_kernel, SMEM_BYTES)) return e;
+    cudaError_t e = launch_kernel(paged_attn_kernel, dim3(sms), dim3(kThreads), SMEM_BYTES, st, tq, tq_small, tkv, p);
+    if (e != cudaSuccess) return e;
+    // The merge launches under the attention kernel's tail; its own wait orders it behind that kernel's writes.
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(sms, (p.rows_cap + 7) / 8);
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, paged_combine_kernel, p);
 }
 
 }  // namespace lrm

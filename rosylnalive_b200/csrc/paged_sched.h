@@ -1,0 +1,91 @@
+// paged_sched.h -- how the paged attention's work is counted and cut (host and device: the kernels use it, and it can
+// be checked on the CPU).
+//
+// A request has n new tokens, the last of its kv keys, and `group` query heads a KV head. An item is up to `span`
+// consecutive tokens of one request and KV head, all their query heads; its unit of work is a tile of 128 keys, and it
+// has as many as its last token sees. All units of a call, ordered by (request, KV head, item, key), are cut into
+// `ctas` ranges of equal length, one a CTA, so every mixture of lengths is balanced; an item that a cut passes through
+// is merged from its CTAs' partial results.
+#pragma once
+
+#include <stdint.h>
+
+#ifdef __CUDACC__
+#define LRM_HD __host__ __device__ __forceinline__
+#else
+#define LRM_HD inline
+#endif
+
+namespace lrm {
+namespace sched {
+
+constexpr int kTileKeys = 128;
+constexpr int kTileRows = 128;
+
+// sum over i in [0, n) of floor((a i + b) / m), by Euclid's steps on (a, m); a, b >= 0, m > 0.
+LRM_HD uint64_t floor_sum(uint64_t n, uint32_t m, uint32_t a, uint64_t b) {
+    uint64_t sum = 0;
+    for (;;) {
+        if (n == 0) return sum;
+        sum += (n * (n - 1) / 2) * (a / m) + n * (b / m);
+        a %= m;
+        b %= m;
+        const uint64_t y = (uint64_t)a * n + b;
+        if (y < m) return sum;
+        n = y / m;
+        b = y % m;
+        const uint32_t t = m;
+        m = a;
+        a = t;
+    }
+}
+
+LRM_HD int items_of(int n, int span) { return (n + span - 1) / span; }
+
+// Key tiles of item i.
+LRM_HD int item_tiles(int n, int kv, int span, int i) {
+    const int last = (i + 1) * span < n ? (i + 1) * span : n;  // (i + 1) * span <= n + span: no overflow at 2^24 tokens
+    return (kv - n + last - 1) / kTileKeys + 1;
+}
+
+// Units of the items before item i (i <= items - 1) of one head.
+LRM_HD uint64_t units_before(int n, int kv, int span, int i) {
+    if (i == 0) return 0;
+    return floor_sum((uint64_t)i, kTileKeys, (uint32_t)span, (uint64_t)(kv - n + span - 1)) + (uint64_t)i;
+}
+
+// Units of one head.
+LRM_HD uint64_t head_units(int n, int kv, int span) {
+    const int items = items_of(n, span);
+    return units_before(n, kv, span, items - 1) + (uint64_t)item_tiles(n, kv, span, items - 1);
+}
+
+// The item of a head that holds its unit `off`.
+LRM_HD int item_at(int n, int kv, int span, uint64_t off) {
+    int lo = 0, hi = items_of(n, span);  // units_before(lo) <= off < units_before(hi)
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (units_before(n, kv, span, mid) <= off)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    return lo;
+}
+
+// CTAs that take part: at least `least` units each, so that short work is not cut into pieces that cost more to merge
+// than they save.
+LRM_HD int ctas_of(uint64_t units, int ctas, int least) {
+    const uint64_t want = (units + (uint64_t)least - 1) / (uint64_t)least;
+    return want < (uint64_t)ctas ? (int)want : ctas;
+}
+
+LRM_HD uint64_t cut(uint64_t units, int ctas, int c) { return units * (uint64_t)c / (uint64_t)ctas; }
+
+// The CTA whose range holds unit u.
+LRM_HD int cta_of(uint64_t units, int ctas, uint64_t u) {
+    return (int)(((u + 1) * (uint64_t)ctas - 1) / units);
+}
+
+}  // namespace sched
+}  // namespace lrm
