@@ -12,8 +12,8 @@
 //   narrow  (up to 128 rows): one set of rows; the even key tiles go to slot 0 and the odd ones to slot 1, so one
 //           slot's products run under the other's softmax; the two states merge at the end.
 // Warps of a CTA:
-//   0       TMA producer: q of an item, then K_0, V_0, K_1, V_1, ... through a ring of five 32 KiB stages (8 pages of 16
-//           tokens, one box a page and 64 dims; 16 lanes issue them), running ahead into the next item;
+//   0, 3    TMA producers, half of the dims each: q of an item, then K_0, V_0, K_1, V_1, ... through a ring of five 32 KiB
+//           stages (8 pages of 16 tokens, one box a page and 64 dims), running ahead into the next item;
 //   1       tensor-core issuer (one thread);
 //   2       scheduler: walks the CTA's range and hands the items to the others through a ring of four;
 //   4..11   softmax, one warpgroup a slot, thread = row.
@@ -67,6 +67,10 @@ struct Record {
     int tok0, ntok, kvh, follow;
 };
 
+// A request's tokens and keys when it is sound and has any, else n = 0.
+struct Request {
+    int start, n, kv, slot;
+};
 struct Control {
     uint64_t q_full, q_empty, fin, o_free;
     uint64_t kv_full[KV_ST], kv_empty[KV_ST];
@@ -74,7 +78,8 @@ struct Control {
     uint64_t item_full[ITEMS], item_empty[ITEMS];
     Item items[ITEMS];
     uint64_t warp_sum[kThreads / 32];
-    uint64_t start_off;
+    uint64_t start_off, start_head;  // the range's last unit within its request, and that request's units a head
+    Request start;
     int start_req;
     uint32_t tmem;
     int poison[SLOTS][2];  // [slot][item parity]: the item (counted from 1) in which v of a visible key was zeroed
@@ -105,12 +110,18 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
+// ptx::mbar_wait with its loop kept small: the kernel has some thirty waits, and its warps' loops together have to fit
+// the SM's instruction cache (unrolled waits alone were 60 KB of code, and every role then stalled on fetches).
+__device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, uint32_t *err, uint32_t code) {
+#pragma unroll 1
+    for (uint32_t i = 0; i < ptx::kWaitLimit; ++i)
+        if (ptx::mbar_try_wait(bar, parity)) return true;
+    atomicCAS(err, 0u, code);
+    return false;
+}
+
 __device__ __forceinline__ bool finite_bf16(uint32_t h) { return (h & 0x7F80u) != 0x7F80u; }
 
-// A request's tokens and keys when it is sound and has any, else n = 0.
-struct Request {
-    int start, n, kv, slot;
-};
 __device__ __forceinline__ Request load_request(const PagedAttnArgs &a, int r, bool report) {
     Request q;
     q.start = a.cu_seqlens[r];
@@ -129,50 +140,83 @@ __device__ __forceinline__ Request load_request(const PagedAttnArgs &a, int r, b
 // `last_seen` (relative to the tile) are seen by some row: if one of them is hit, `poison` is set.
 __device__ __forceinline__ void clean_v(uint8_t *tile, int key, int lane, int last_seen, volatile int *poison, int id) {
     const uint32_t row = ptx::smem_u32(tile) + key * 128;
-    __nv_bfloat162 acc = __floats2bfloat162_rn(0.f, 0.f);
-    const __nv_bfloat162 zero = acc;
+    __nv_bfloat162 acc[4];
+    const __nv_bfloat162 zero = __floats2bfloat162_rn(0.f, 0.f);
 #pragma unroll
-    for (int half = 0; half < 2; ++half)
+    for (int e = 0; e < 4; ++e) acc[e] = zero;
+#pragma unroll 4
+    for (int i = 0; i < 16; ++i) {  // 16-byte chunks in an order that differs by lane: no bank conflicts
+        const uint4 v = ptx::ld_shared_v4(row + (i >> 3) * SUB + (((i + lane) & 7) << 4));
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {  // chunks in an order that differs by lane: no bank conflicts
-            uint4 v = ptx::ld_shared_v4(row + half * SUB + (((c + lane) & 7) << 4));
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e)  // 0 * v + acc: NaN once v is infinite or NaN
-                acc = __hfma2(*reinterpret_cast<const __nv_bfloat162 *>(&w[e]), zero, acc);
-        }
-    const float2 f = __bfloat1622float2(acc);
-    const bool hit = f.x != f.x || f.y != f.y;
-    if (hit && key <= last_seen) {
-        *poison = id;
-        __threadfence_block();  // seen before the zeros below are (the other warpgroup may find only those)
+        for (int e = 0; e < 4; ++e)  // 0 * v + acc: NaN once v is infinite or NaN
+            acc[e] = __hfma2(*reinterpret_cast<const __nv_bfloat162 *>(&w[e]), zero, acc[e]);
     }
-    if (hit)
-#pragma unroll 1
-        for (int c = 0; c < 16; ++c) {
-            const uint32_t at = row + (c >> 3) * SUB + ((c & 7) << 4);
-            uint4 v = ptx::ld_shared_v4(at);
-            uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (!finite_bf16(w[e])) w[e] &= 0xFFFF0000u;
-                if (!finite_bf16(w[e] >> 16)) w[e] &= 0x0000FFFFu;
-            }
-            ptx::st_shared_v4(at, w[0], w[1], w[2], w[3]);
+    const float2 f = __bfloat1622float2(__hadd2(__hadd2(acc[0], acc[1]), __hadd2(acc[2], acc[3])));
+    if (f.x != f.x || f.y != f.y) {
+        if (key <= last_seen) {
+            *poison = id;
+            __threadfence_block();  // seen before the zeros below are (the other warpgroup may find only those)
         }
+#pragma unroll 1
+        for (int i = 0; i < 64; ++i) {
+            const uint32_t at = row + (i >> 5) * SUB + (i & 31) * 4;
+            uint32_t w;
+            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(at) : "memory");
+            if (!finite_bf16(w)) w &= 0xFFFF0000u;
+            if (!finite_bf16(w >> 16)) w &= 0x0000FFFFu;
+            asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(w) : "memory");
+        }
+    }
     ptx::fence_proxy_async();  // the tensor core reads the tile through the async proxy
 }
 
-// Adds the values that clean_v zeroed, from the cache, to dims [c, c + 32) of a row that sees keys lo .. hi.
-__device__ __noinline__ void add_poison(const PagedAttnArgs &a, const Item &it, int lo, int hi, int c, float *o) {
-    for (int key = lo; key <= hi; ++key) {
-        const int pg = a.page_table[it.table + key / kPageTokens];
-        if (pg < 0 || pg >= a.kv_pages) continue;
-        const __nv_bfloat16 *v = a.pool + (size_t)pg * kv_page_elems(a.kv_heads) +
-                                 (size_t)(it.kvh * 2 + 1) * (kPageTokens * kHeadDim) + (key % kPageTokens) * kHeadDim + c;
-        for (int e = 0; e < 32; ++e) {
-            const float x = __bfloat162float(v[e]);
-            if (!(fabsf(x) < INFINITY)) o[e] += x;
+// Adds the values that clean_v zeroed to one slot's O (128 columns at `t`, this warp's lanes), from the cache: this
+// lane's row sees keys lo .. hi, of which the slot has those of tiles tile0, tile0 + step, ... Rare, so it is kept out of the kernel's instruction stream.
+__device__ __noinline__ void add_poison(const PagedAttnArgs &a, int64_t table, int kvh, int lo, int hi, int tile0, int step,
+                                        uint32_t t) {
+#pragma unroll 1
+    for (int c = 0; c < kHeadDim; c += 16) {
+        uint32_t o[16];
+        ptx::tmem_ld16(t + c, o);
+        ptx::tmem_ld_wait();
+#pragma unroll 1
+        for (int key = lo; key <= hi; ++key) {
+            if ((key / TK - tile0) % step != 0) continue;  // the other slot's tile
+            const int pg = a.page_table[table + key / kPageTokens];
+            if (pg < 0 || pg >= a.kv_pages) continue;
+            const __nv_bfloat16 *v = a.pool + (size_t)pg * kv_page_elems(a.kv_heads) +
+                                     (size_t)(kvh * 2 + 1) * (kPageTokens * kHeadDim) + (key % kPageTokens) * kHeadDim + c;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const float x = __bfloat162float(v[e]);
+                if (!(fabsf(x) < INFINITY)) o[e] = __float_as_uint(__uint_as_float(o[e]) + x);
+            }
+        }
+        __syncwarp();
+        ptx::tmem_st16(t + c, o);
+    }
+    ptx::tmem_st_wait();
+}
+
+// Within each group of four lanes: v[j] becomes lane j's v[own lane]. A thread holds 64 bytes of its own row; after
+// this, v[j] is 16 bytes of row j of the group, and the four lanes' 16 bytes are 64 contiguous ones.
+__device__ __forceinline__ void quad_transpose(uint4 (&v)[4], int lane) {
+#pragma unroll
+    for (int step = 1; step <= 2; step *= 2) {
+        const bool up = lane & step;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int x = step == 1 ? 2 * i : i, y = x + step;
+            uint4 t = up ? v[x] : v[y];
+            t.x = __shfl_xor_sync(0xffffffffu, t.x, step);
+            t.y = __shfl_xor_sync(0xffffffffu, t.y, step);
+            t.z = __shfl_xor_sync(0xffffffffu, t.z, step);
+            t.w = __shfl_xor_sync(0xffffffffu, t.w, step);
+            if (up)
+                v[x] = t;
+            else
+                v[y] = t;
         }
     }
 }
@@ -188,7 +232,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     Control &c = *reinterpret_cast<Control *>(sKV + KV_ST * TILE);
     const PagedAttnArgs &a = p.a;
     uint32_t *err = a.err;
-    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+    // (the shuffle tells the compiler that the warp index, and so the role, is the same in all lanes)
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid / 32, 0), lane = tid % 32;
     const int cta = blockIdx.x, span = SLOTS * p.tt;
     if (ptx::smem_u32(smem) & 1023) {  // the swizzled tiles and their descriptors need 1024-byte alignment
         if (tid == 0) {
@@ -198,11 +243,44 @@ __global__ void __launch_bounds__(kThreads, 1)
         return;
     }
 
+    if (warp == 2) {
+        if (lane == 0) {
+            ptx::mbar_init(&c.q_full, 2);  // the two producer warps
+            ptx::mbar_init(&c.q_empty, 1);
+            ptx::mbar_init(&c.fin, 1);
+            ptx::mbar_init(&c.o_free, 8);
+            for (int s = 0; s < KV_ST; ++s) {
+                ptx::mbar_init(&c.kv_full[s], 2);
+                ptx::mbar_init(&c.kv_empty[s], 1);
+            }
+            for (int s = 0; s < SLOTS; ++s) {
+                ptx::mbar_init(&c.s_full[s], 1);
+                ptx::mbar_init(&c.p_part[s], 4);
+                ptx::mbar_init(&c.p_full[s], 4);
+                ptx::mbar_init(&c.o_done[s], 1);
+                c.poison[s][0] = c.poison[s][1] = 0;
+            }
+            for (int s = 0; s < ITEMS; ++s) {
+                ptx::mbar_init(&c.item_full[s], 1);
+                ptx::mbar_init(&c.item_empty[s], 11);  // two producers, the issuer, eight softmax warps
+            }
+            ptx::fence_barrier_init();
+        }
+    } else if (warp == 1) {
+        ptx::tmem_alloc(&c.tmem, 512);
+        ptx::tmem_relinquish();
+    } else if (warp == 0 && lane == 0) {
+        ptx::prefetch_tmap(&tq);
+        ptx::prefetch_tmap(&tq_small);
+        ptx::prefetch_tmap(&tkv);
+    }
+
     // ---- this CTA's range ----
     // Units of each thread's requests, their exclusive sums over the threads, and the request of the range's last unit.
     const int per = (a.requests + kThreads - 1) / kThreads;
     const int r0 = min(a.requests, tid * per), r1 = min(a.requests, r0 + per);
     uint64_t own = 0;
+#pragma unroll 1
     for (int r = r0; r < r1; ++r) {
         const Request q = load_request(a, r, cta == 0);
         if (q.n) own += sched::head_units(q.n, q.kv, span) * (uint64_t)a.kv_heads;
@@ -214,35 +292,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane >= o) incl += x;
     }
     if (lane == 31) c.warp_sum[warp] = incl;
-    if (tid == 0) {
-        ptx::mbar_init(&c.q_full, 1);
-        ptx::mbar_init(&c.q_empty, 1);
-        ptx::mbar_init(&c.fin, 1);
-        ptx::mbar_init(&c.o_free, 8);
-        for (int s = 0; s < KV_ST; ++s) {
-            ptx::mbar_init(&c.kv_full[s], 1);
-            ptx::mbar_init(&c.kv_empty[s], 1);
-        }
-        for (int s = 0; s < SLOTS; ++s) {
-            ptx::mbar_init(&c.s_full[s], 1);
-            ptx::mbar_init(&c.p_part[s], 4);
-            ptx::mbar_init(&c.p_full[s], 4);
-            ptx::mbar_init(&c.o_done[s], 1);
-            c.poison[s][0] = c.poison[s][1] = 0;
-        }
-        for (int s = 0; s < ITEMS; ++s) {
-            ptx::mbar_init(&c.item_full[s], 1);
-            ptx::mbar_init(&c.item_empty[s], 10);  // producer, issuer, eight softmax warps
-        }
-        ptx::fence_barrier_init();
-        ptx::prefetch_tmap(&tq);
-        ptx::prefetch_tmap(&tq_small);
-        ptx::prefetch_tmap(&tkv);
-    }
-    if (warp == 1) {
-        ptx::tmem_alloc(&c.tmem, 512);
-        ptx::tmem_relinquish();
-    }
     ptx::tc_fence_before();
     __syncthreads();
     ptx::tc_fence_after();
@@ -258,6 +307,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint64_t u0 = idle ? 0 : sched::cut(units, ctas, cta), u1 = idle ? 0 : sched::cut(units, ctas, cta + 1);
     if (!idle && before <= u1 - 1 && u1 - 1 < before + own) {
         uint64_t at = before;
+#pragma unroll 1
         for (int r = r0; r < r1; ++r) {
             const Request q = load_request(a, r, false);
             if (!q.n) continue;
@@ -265,6 +315,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (u1 - 1 < at + w) {
                 c.start_req = r;
                 c.start_off = u1 - 1 - at;
+                c.start_head = sched::head_units(q.n, q.kv, span);
+                c.start = q;
                 break;
             }
             at += w;
@@ -280,16 +332,18 @@ __global__ void __launch_bounds__(kThreads, 1)
             // ---- scheduler ----
             if (lane == 0) {
                 int r = c.start_req;
-                Request q = load_request(a, r, false);
-                uint64_t off = c.start_off, head = sched::head_units(q.n, q.kv, span), left = u1 - u0, u_end = u1;
-                int h = (int)(off / head), i = sched::item_at(q.n, q.kv, span, off % head);
+                Request q = c.start;
+                uint64_t left = u1 - u0;
+                int h = (int)sched::quotient(c.start_off, c.start_head);
+                const uint64_t off = c.start_off - (uint64_t)h * c.start_head;
+                int i = sched::item_at(q.n, q.kv, span, off);
                 int tiles = sched::item_tiles(q.n, q.kv, span, i);
-                int ke = (int)(off % head - sched::units_before(q.n, q.kv, span, i)) + 1;
+                int ke = (int)(off - sched::units_before(q.n, q.kv, span, i)) + 1;
                 Record rec = {0, 0, 0, 0};
                 int k = 0;
                 bool ok = true;
                 while (ok) {
-                    ok = ptx::mbar_wait(&c.item_empty[k % ITEMS], ((k / ITEMS) & 1) ^ 1, err, kErrWaitScheduler);
+                    ok = wait_bar(&c.item_empty[k % ITEMS], ((k / ITEMS) & 1) ^ 1, err, kErrWaitScheduler);
                     if (!ok) break;
                     Item it = {};
                     if (left > 0) {
@@ -302,16 +356,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                         it.npages = (q.kv + kPageTokens - 1) / kPageTokens;
                         it.table = (int64_t)q.slot * a.pages_per_seq;
                         it.dest = it.kb == 0 && ke == tiles ? -1 : (it.kb == 0 ? 1 : 0);
-                        if (it.dest == 1)  // the item ends at unit u_end + (tiles - ke)
-                            rec = Record{it.tok0, it.ntok, h,
-                                         sched::cta_of(units, ctas, u_end + (uint64_t)(tiles - ke) - 1) - cta};
                     }
                     c.items[k % ITEMS] = it;
                     ptx::mbar_arrive(&c.item_full[k % ITEMS]);
+                    if (it.dest == 1)  // the range's last item, begun here: it ends (tiles - ke) units behind the range
+                        rec = Record{it.tok0, it.ntok, h, sched::cta_of(units, ctas, u1 - 1 + (uint64_t)(tiles - ke)) - cta};
                     ++k;
                     if (left == 0) break;
                     left -= (uint64_t)(ke - it.kb);
-                    u_end -= (uint64_t)(ke - it.kb);
                     if (left == 0) continue;
                     // the item before: of this head, else of the head before, else of the request before
                     if (i > 0) {
@@ -330,13 +382,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 p.records[cta] = rec;
             }
-        } else if (warp == 0) {
-            // ---- TMA producer ----
+        } else if (warp == 0 || warp == 3) {
+            // ---- TMA producers: warp 0 the first 64 dims of every tile, warp 3 the others ----
+            const int half = warp == 3;
             const int oob = a.kv_pages * a.kv_heads * 2;  // past the tensor map: read as zeros, without a memory access
             int ring = 0;  // ring items issued so far
             bool ok = true;
             for (int k = 0; ok; ++k) {
-                if (lane == 0) ok = ptx::mbar_wait(&c.item_full[k % ITEMS], (k / ITEMS) & 1, err, kErrWaitProducer);
+                if (lane == 0) ok = wait_bar(&c.item_full[k % ITEMS], (k / ITEMS) & 1, err, kErrWaitProducer);
                 ok = __shfl_sync(0xffffffffu, ok, 0);
                 if (!ok) break;
                 const Item it = c.items[k % ITEMS];
@@ -355,17 +408,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                 };
                 int z = fetch(it.kb), z_next = it.kb + 4 < it.ke ? fetch(it.kb + 4) : oob;
                 if (lane == 0) {
-                    ok = ptx::mbar_wait(&c.q_empty, (k & 1) ^ 1, err, kErrWaitProducer);
+                    ok = wait_bar(&c.q_empty, (k & 1) ^ 1, err, kErrWaitProducer);
                     if (ok) {
                         const bool small = it.ntok * p.group <= kSmallBoxRows;
                         const int slots = it.ntok > p.tt ? 2 : 1;
                         const int box_tok = small ? max(1, kSmallBoxRows / p.group) : p.tt;
                         const CUtensorMap *map = small ? &tq_small : &tq;
-                        ptx::mbar_arrive_expect_tx(&c.q_full, slots * box_tok * p.group * 256);
+                        ptx::mbar_arrive_expect_tx(&c.q_full, slots * box_tok * p.group * 128);
                         for (int s = 0; s < slots; ++s)
-                            for (int half = 0; half < 2; ++half)
-                                ptx::tma_load_3d(sQ + s * TILE + half * SUB, map, &c.q_full, 64 * half, it.kvh * p.group,
-                                                 it.tok0 + s * p.tt);
+                            ptx::tma_load_3d(sQ + s * TILE + half * SUB, map, &c.q_full, 64 * half, it.kvh * p.group,
+                                             it.tok0 + s * p.tt);
                     }
                 }
                 ok = __shfl_sync(0xffffffffu, ok, 0);
@@ -375,24 +427,30 @@ __global__ void __launch_bounds__(kThreads, 1)
                         z = z_next;
                         z_next = t + 4 < it.ke ? fetch(t + 4) : oob;
                     }
-                    const int zt = __shfl_sync(0xffffffffu, z, sub * 8 + (lane >> 1));  // lanes 0..15: page lane / 2
-                    for (int kv = 0; ok && kv < 2; ++kv, ++ring) {
-                        const int st = ring % KV_ST;
-                        if (lane == 0) {
-                            ok = ptx::mbar_wait(&c.kv_empty[st], ((ring / KV_ST) & 1) ^ 1, err, kErrWaitProducer);
-                            if (ok) ptx::mbar_arrive_expect_tx(&c.kv_full[st], TILE);
+                    int zp[8];
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) zp[u] = __shfl_sync(0xffffffffu, z, sub * 8 + u);
+                    if (ptx::elect_one()) {
+#pragma unroll 1
+                        for (int kv = 0; ok && kv < 2; ++kv) {
+                            const int x = ring + kv, st = x % KV_ST;
+                            ok = wait_bar(&c.kv_empty[st], ((x / KV_ST) & 1) ^ 1, err, kErrWaitProducer);
+                            if (!ok) break;
+                            ptx::mbar_arrive_expect_tx(&c.kv_full[st], SUB);
+                            uint8_t *dst = sKV + st * TILE + half * SUB;
+#pragma unroll
+                            for (int u = 0; u < 8; ++u)
+                                ptx::tma_load_3d(dst + u * 2048, &tkv, &c.kv_full[st], 64 * half, 0, zp[u] + kv);
                         }
-                        ok = __shfl_sync(0xffffffffu, ok, 0);
-                        if (!ok) break;
-                        if (lane < 16)
-                            ptx::tma_load_3d(sKV + st * TILE + (lane & 1) * SUB + (lane >> 1) * 2048, &tkv, &c.kv_full[st],
-                                             64 * (lane & 1), 0, zt + kv);
                     }
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (ok) ring += 2;
                 }
             }
-            // Our own copies in flight must land before the CTA exits (this matters on the error path).
+            // Copies in flight must land before the CTA exits (this matters on the error path; a fill of which only
+            // one half was issued is waited for until the wait's limit).
             for (int x = ring > KV_ST ? ring - KV_ST : 0; x < ring; ++x)
-                ptx::mbar_wait(&c.kv_full[x % KV_ST], (x / KV_ST) & 1, err, kErrWaitProducer);
+                wait_bar(&c.kv_full[x % KV_ST], (x / KV_ST) & 1, err, kErrWaitProducer);
         } else if (warp == 1) {
             // ---- tensor-core issuer ----
             if (ptx::elect_one()) {
@@ -402,37 +460,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 uint32_t steps[SLOTS] = {};  // P tiles consumed so far, a slot
                 bool ok = true;
                 auto wait = [&](uint64_t *bar, uint32_t parity) {
-                    if (ok) ok = ptx::mbar_wait(bar, parity, err, kErrWaitIssuer);
+                    if (ok) ok = wait_bar(bar, parity, err, kErrWaitIssuer);
                     ptx::tc_fence_after();
                     return ok;
                 };
                 auto wait_ring = [&](int x) { return wait(&c.kv_full[x % KV_ST], (x / KV_ST) & 1); };
-                // S_s = Q_q K^T of the K tile in ring item x, announced on s_full[s]
-                auto qk = [&](int s, int q, int x) {
-                    const uint32_t aQ = ptx::smem_u32(sQ + q * TILE), aK = ptx::smem_u32(sKV + (x % KV_ST) * TILE);
-#pragma unroll
-                    for (int kk = 0; kk < 8; ++kk) {
-                        const uint32_t o = (kk >> 2) * SUB + (kk & 3) * 32;
-                        ptx::mma_bf16(tmem + 256 * s, ptx::sw128_kmajor_desc(aQ + o), ptx::sw128_kmajor_desc(aK + o),
-                                      idesc_qk, kk > 0 ? 1u : 0u);
-                    }
-                    ptx::mma_commit(&c.s_full[s]);
-                };
-                // O_s (+)= P_s V of the V tile in ring item x, as P's two parts are written
-                auto pv = [&](int s, int x, bool first) {
-                    const uint32_t tO = tmem + 256 * s + 128, tP = tmem + 256 * s;
-                    const uint32_t aV = ptx::smem_u32(sKV + (x % KV_ST) * TILE);
-                    if (!wait(&c.p_part[s], steps[s] & 1)) return;
-#pragma unroll
-                    for (int kk = 0; kk < 6; ++kk)
-                        ptx::mma_bf16_ts(tO, tP + kk * 8, ptx::sw128_mnmajor_desc(aV + kk * 2048, SUB, 1024), idesc_pv,
-                                         (!first || kk > 0) ? 1u : 0u);
-                    if (!wait(&c.p_full[s], steps[s] & 1)) return;
-#pragma unroll
-                    for (int kk = 6; kk < 8; ++kk)
-                        ptx::mma_bf16_ts(tO, tP + kk * 8, ptx::sw128_mnmajor_desc(aV + kk * 2048, SUB, 1024), idesc_pv, 1u);
-                    ++steps[s];
-                };
                 for (int k = 0; ok; ++k) {
                     if (!wait(&c.item_full[k % ITEMS], (k / ITEMS) & 1)) break;
                     const int ntok = c.items[k % ITEMS].ntok;
@@ -440,60 +472,55 @@ __global__ void __launch_bounds__(kThreads, 1)
                     ptx::mbar_arrive(&c.item_empty[k % ITEMS]);
                     if (ntok == 0) break;
                     const bool wide = ntok > p.tt;
-                    if (!wait(&c.q_full, k & 1) || !wait_ring(ring)) break;
-                    // The first scores. The tensor core runs this thread's MMAs in order, so they overwrite P of the
-                    // item before only after its last product has read it.
-                    qk(0, 0, ring);
-                    if (wide) qk(1, 1, ring);
-                    ptx::mma_commit(&c.kv_empty[ring % KV_ST]);
-                    if (!wide && nt > 1) {
-                        if (!wait_ring(ring + 2)) break;
-                        qk(1, 0, ring + 2);
-                        ptx::mma_commit(&c.kv_empty[(ring + 2) % KV_ST]);
-                    }
-                    if (nt <= (wide ? 1 : 2)) ptx::mma_commit(&c.q_empty);
-                    // O may be overwritten once the item before has been read out
-                    if (k > 0 && !wait(&c.o_free, (k - 1) & 1)) break;
-                    if (wide) {
-                        for (int j = 0; ok && j < nt; ++j) {
-                            const int xv = ring + 2 * j + 1;
-                            if (!wait_ring(xv)) break;
-                            for (int s = 0; s < 2; ++s) {
-                                pv(s, xv, j == 0);
-                                if (!ok) break;
-                                if (s == 1) ptx::mma_commit(&c.kv_empty[xv % KV_ST]);
-                                if (j + 1 == nt) {
-                                    ptx::mma_commit(&c.o_done[s]);
-                                    continue;
-                                }
-                                if (s == 0 && !wait_ring(xv + 1)) break;
-                                qk(s, s, xv + 1);
-                                if (s == 1) ptx::mma_commit(&c.kv_empty[(xv + 1) % KV_ST]);
-                                if (s == 1 && j + 2 == nt) ptx::mma_commit(&c.q_empty);
-                            }
+                    if (!wait(&c.q_full, k & 1)) break;
+                    // Products n = 0 .. count - 1: slot n & 1, key tile n / 2 (wide) or n (narrow). Step n issues
+                    // O += P V of product n - 2, then S = Q K^T of product n in the same slot. The tensor core runs one
+                    // thread's MMAs in order, so S overwrites P only after its product with V has read it.
+                    const int count = wide ? 2 * nt : nt;
+#pragma unroll 1
+                    for (int n = 0; ok && n < count + 2; ++n) {
+                        const int s = n & 1;
+                        const uint32_t tS = tmem + 256 * s;
+                        if (n >= 2 && n - 2 < count) {
+                            const int x = ring + 2 * (wide ? (n - 2) >> 1 : n - 2) + 1;
+                            if (!wait_ring(x)) break;
+                            // O may be overwritten once the item before has been read out
+                            if (n == 2 && k > 0 && !wait(&c.o_free, (k - 1) & 1)) break;
+                            const uint32_t keep = n - 2 >= 2 ? 1u : 0u;  // the slot's first product overwrites O
+                            const uint64_t v = ptx::sw128_mnmajor_desc(ptx::smem_u32(sKV + (x % KV_ST) * TILE), SUB, 1024);
+                            if (!wait(&c.p_part[s], steps[s] & 1)) break;
+                            ptx::mma_bf16_ts(tS + 128, tS, v, idesc_pv, keep);
+#pragma unroll
+                            for (int kk = 1; kk < 6; ++kk)
+                                ptx::mma_bf16_ts(tS + 128, tS + kk * 8, v + kk * (2048 >> 4), idesc_pv, 1u);
+                            if (!wait(&c.p_full[s], steps[s] & 1)) break;
+#pragma unroll
+                            for (int kk = 6; kk < 8; ++kk)
+                                ptx::mma_bf16_ts(tS + 128, tS + kk * 8, v + kk * (2048 >> 4), idesc_pv, 1u);
+                            ++steps[s];
+                            if (!wide || s == 1) ptx::mma_commit(&c.kv_empty[x % KV_ST]);
+                            if (n >= count) ptx::mma_commit(&c.o_done[s]);
                         }
-                    } else {
-                        for (int j = 0; ok && j < nt; ++j) {
-                            const int xv = ring + 2 * j + 1, s = j & 1;
-                            if (!wait_ring(xv)) break;
-                            pv(s, xv, j < 2);
-                            if (!ok) break;
-                            ptx::mma_commit(&c.kv_empty[xv % KV_ST]);
-                            if (j + 2 >= nt) {
-                                ptx::mma_commit(&c.o_done[s]);
-                                continue;
+                        if (n < count) {
+                            const int x = ring + 2 * (wide ? n >> 1 : n);
+                            if (!wait_ring(x)) break;
+                            const uint64_t q = ptx::sw128_kmajor_desc(ptx::smem_u32(sQ + (wide ? s : 0) * TILE));
+                            const uint64_t kt = ptx::sw128_kmajor_desc(ptx::smem_u32(sKV + (x % KV_ST) * TILE));
+#pragma unroll
+                            for (int kk = 0; kk < 8; ++kk) {
+                                const int o = ((kk >> 2) * SUB + (kk & 3) * 32) >> 4;
+                                ptx::mma_bf16(tS, q + o, kt + o, idesc_qk, kk > 0 ? 1u : 0u);
                             }
-                            if (!wait_ring(xv + 3)) break;
-                            qk(s, 0, xv + 3);
-                            ptx::mma_commit(&c.kv_empty[(xv + 3) % KV_ST]);
-                            if (j + 3 == nt) ptx::mma_commit(&c.q_empty);
+                            ptx::mma_commit(&c.s_full[s]);
+                            if (!wide || s == 1) ptx::mma_commit(&c.kv_empty[x % KV_ST]);
+                            if (n == count - 1) ptx::mma_commit(&c.q_empty);
                         }
                     }
                     ring += 2 * nt;
                 }
                 // No MMA may still be writing TMEM when it is freed (this matters on the error path).
                 ptx::mma_commit(&c.fin);
-                ptx::mbar_wait(&c.fin, 0, err, kErrWaitIssuer);
+                wait_bar(&c.fin, 0, err, kErrWaitIssuer);
             }
         }
     } else {
@@ -504,6 +531,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int rl = quarter * 32 + lane;
         const int tl = rl / p.group, hl = rl - tl * p.group;  // this row's token (of the slot) and query head (of the group)
         const int warp_tl = (quarter * 32) / p.group;         // the warp's first token
+        int rows4[4];  // token << 8 | query head of the four rows that this lane helps to write
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int r = quarter * 32 + (lane & ~3) + j;
+            rows4[j] = (r / p.group) << 8 | (r % p.group);
+        }
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         const uint32_t tS = tmem + 256 * s + lanes;
         const float sc = a.scale_log2;
@@ -511,7 +544,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t steps = 0, done[SLOTS] = {};  // S tiles taken from this slot; items that used each slot
         bool ok = true;
         for (int k = 0; ok; ++k) {
-            if (!ptx::mbar_wait(&c.item_full[k % ITEMS], (k / ITEMS) & 1, err, kErrWaitSoftmax)) break;
+            if (!wait_bar(&c.item_full[k % ITEMS], (k / ITEMS) & 1, err, kErrWaitSoftmax)) break;
             const Item it = c.items[k % ITEMS];
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(&c.item_empty[k % ITEMS]);
@@ -525,7 +558,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             float m_ref = -INFINITY, l = 0.f;
             bool first = true;
             for (int j = wide ? 0 : s; j < nt; j += wide ? 1 : 2, ++steps) {
-                if (!ptx::mbar_wait(&c.s_full[s], steps & 1, err, kErrWaitSoftmax)) {
+                if (!wait_bar(&c.s_full[s], steps & 1, err, kErrWaitSoftmax)) {
                     ok = false;
                     break;
                 }
@@ -598,7 +631,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 first = false;
                 if (dirty) {
                     const int xv = ring + 2 * j + 1;
-                    if (!ptx::mbar_wait(&c.kv_full[xv % KV_ST], (xv / KV_ST) & 1, err, kErrWaitSoftmax)) {
+                    if (!wait_bar(&c.kv_full[xv % KV_ST], (xv / KV_ST) & 1, err, kErrWaitSoftmax)) {
                         ok = false;
                         break;
                     }
@@ -622,7 +655,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             // ---- epilogue ----
             const bool used1 = wide || nt > 1;
             auto wait_done = [&](int slot) {
-                if (!ptx::mbar_wait(&c.o_done[slot], done[slot] & 1, err, kErrWaitSoftmax)) ok = false;
+                if (!wait_bar(&c.o_done[slot], done[slot] & 1, err, kErrWaitSoftmax)) ok = false;
                 ++done[slot];
                 ptx::tc_fence_after();
                 return ok;
@@ -648,45 +681,72 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             const bool poisoned = c.poison[0][k & 1] == k + 1 || c.poison[1][k & 1] == k + 1;
             if (active) {
-                const int row = token * p.group + hl;
-                const size_t part = ((size_t)cta * 2 + (it.dest > 0)) * p.rows_cap + row;
-                const float inv = 1.f / l;
+                // o = w[0] O_0 + w[1] O_1 (wide: this slot's O alone), 16 dims at a time
+                const uint32_t tO = (wide ? tS : tmem + lanes) + 128;
+                const bool two = !wide && used1;
+                if (poisoned) {
+                    const int lo = max(it.kb * TK, it.pos0 / TK * TK);
+                    const int hi = valid ? min(it.pos0 + token, it.ke * TK - 1) : -1;
+                    if (wide || nt > s)
+                        add_poison(a, it.table, it.kvh, lo, hi, it.kb + (wide ? 0 : s), wide ? 1 : 2, tS + 128);
+                    if (!wide) {  // the other warpgroup's warp of these lanes reads this slot's O too
+                        ptx::tc_fence_before();
+                        ptx::named_barrier(2 + quarter, 64);
+                        ptx::tc_fence_after();
+                    }
+                }
+                const float inv = it.dest < 0 ? 1.f / l : 1.f;
+                const float w0 = w[0] * inv, w1 = w[1] * inv;
+                const size_t part = ((size_t)cta * 2 + (it.dest > 0)) * p.rows_cap;
                 const int c0 = wide ? 0 : 64 * s, c1 = wide ? 128 : 64 * s + 64;
+                if (it.dest >= 0 && valid && c0 == 0)
+                    *reinterpret_cast<float2 *>(p.part_ml + (part + token * p.group + hl) * 2) = make_float2(m_ref, l);
 #pragma unroll 1
                 for (int col = c0; col < c1; col += 32) {
-                    float o[32];
-                    if (wide) {
-                        ptx::tmem_ld32(tS + 128 + col, reinterpret_cast<uint32_t *>(o));
-                        ptx::tmem_ld_wait();
-                    } else {
-                        uint32_t o1[32];
-                        ptx::tmem_ld32(tmem + lanes + 128 + col, reinterpret_cast<uint32_t *>(o));
-                        if (used1) ptx::tmem_ld32(tmem + lanes + 256 + 128 + col, o1);
+                    uint4 v[4];
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+                        uint32_t o[16];
+                        ptx::tmem_ld16(tO + col + 16 * b, o);
                         ptx::tmem_ld_wait();
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            o[e] = w[0] == 0.f ? 0.f : w[0] * o[e];
-                            if (used1 && w[1] != 0.f) o[e] += w[1] * __uint_as_float(o1[e]);
+                        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * w0);
+                        if (two) {
+                            uint32_t o1[16];
+                            ptx::tmem_ld16(tO + 256 + col + 16 * b, o1);
+                            ptx::tmem_ld_wait();
+#pragma unroll
+                            for (int e = 0; e < 16; ++e)
+                                o[e] = __float_as_uint(fmaf(__uint_as_float(o1[e]), w1, __uint_as_float(o[e])));
+                        }
+                        if (it.dest < 0) {
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const uint32_t *x = o + 8 * e;
+                                v[2 * b + e] = make_uint4(pack2(__uint_as_float(x[0]), __uint_as_float(x[1])),
+                                                          pack2(__uint_as_float(x[2]), __uint_as_float(x[3])),
+                                                          pack2(__uint_as_float(x[4]), __uint_as_float(x[5])),
+                                                          pack2(__uint_as_float(x[6]), __uint_as_float(x[7])));
+                            }
+                        } else if (valid) {
+                            float4 *d = reinterpret_cast<float4 *>(p.part_o + (part + token * p.group + hl) * kHeadDim + col + 16 * b);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                d[e] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]),
+                                                   __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
                         }
                     }
-                    if (poisoned && valid)
-                        add_poison(a, it, max(it.kb * TK, it.pos0 / TK * TK), min(it.pos0 + token, it.ke * TK - 1), col, o);
-                    if (!valid) continue;
                     if (it.dest < 0) {
-                        uint4 *d = reinterpret_cast<uint4 *>(a.out + (size_t)(it.tok0 + token) * a.ld_out +
-                                                             (size_t)(it.kvh * p.group + hl) * kHeadDim + col);
+                        // four lanes write 64 contiguous bytes of each of their four rows
+                        quad_transpose(v, lane);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            d[e] = make_uint4(pack2(o[8 * e] * inv, o[8 * e + 1] * inv),
-                                              pack2(o[8 * e + 2] * inv, o[8 * e + 3] * inv),
-                                              pack2(o[8 * e + 4] * inv, o[8 * e + 5] * inv),
-                                              pack2(o[8 * e + 6] * inv, o[8 * e + 7] * inv));
-                    } else {
-                        float4 *d = reinterpret_cast<float4 *>(p.part_o + part * kHeadDim + col);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            d[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-                        if (col == 0) *reinterpret_cast<float2 *>(p.part_ml + part * 2) = make_float2(m_ref, l);
+                        for (int j = 0; j < 4; ++j) {
+                            const int tj = rows4[j] >> 8, hj = rows4[j] & 255, tok = wide ? s * p.tt + tj : tj;
+                            if (tj < p.tt && tok < it.ntok)
+                                *reinterpret_cast<uint4 *>(a.out + (size_t)(it.tok0 + tok) * a.ld_out +
+                                                           (size_t)(it.kvh * p.group + hj) * kHeadDim + col +
+                                                           8 * (lane & 3)) = v[j];
+                        }
                     }
                 }
             }

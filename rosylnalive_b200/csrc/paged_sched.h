@@ -12,8 +12,10 @@
 
 #ifdef __CUDACC__
 #define LRM_HD __host__ __device__ __forceinline__
+#define LRM_HD_FAR static __host__ __device__ __noinline__  // one copy: instruction space is scarce in the kernel
 #else
 #define LRM_HD inline
+#define LRM_HD_FAR inline
 #endif
 
 namespace lrm {
@@ -23,7 +25,7 @@ constexpr int kTileKeys = 128;
 constexpr int kTileRows = 128;
 
 // sum over i in [0, n) of floor((a i + b) / m), by Euclid's steps on (a, m); a, b >= 0, m > 0.
-LRM_HD uint64_t floor_sum(uint64_t n, uint32_t m, uint32_t a, uint64_t b) {
+LRM_HD_FAR uint64_t floor_sum(uint64_t n, uint32_t m, uint32_t a, uint64_t b) {
     uint64_t sum = 0;
     for (;;) {
         if (n == 0) return sum;
@@ -76,15 +78,25 @@ LRM_HD int item_at(int n, int kv, int span, uint64_t off) {
 // CTAs that take part: at least `least` units each, so that short work is not cut into pieces that cost more to merge
 // than they save.
 LRM_HD int ctas_of(uint64_t units, int ctas, int least) {
-    const uint64_t want = (units + (uint64_t)least - 1) / (uint64_t)least;
-    return want < (uint64_t)ctas ? (int)want : ctas;
+    if (units >= (uint64_t)ctas * (uint64_t)least) return ctas;
+    const uint32_t want = ((uint32_t)units + (uint32_t)least - 1) / (uint32_t)least;
+    return want < (uint32_t)ctas ? (int)want : ctas;
 }
 
-LRM_HD uint64_t cut(uint64_t units, int ctas, int c) { return units * (uint64_t)c / (uint64_t)ctas; }
+// Where CTA c's range starts. (32-bit arithmetic where it fits: a 64-bit division costs the start of a short call.)
+LRM_HD uint64_t cut(uint64_t units, int ctas, int c) {
+    if (units < (1u << 20) && ctas <= 4096) return (uint32_t)units * (uint32_t)c / (uint32_t)ctas;
+    return units * (uint64_t)c / (uint64_t)ctas;
+}
 
 // The CTA whose range holds unit u.
 LRM_HD int cta_of(uint64_t units, int ctas, uint64_t u) {
+    if (units < (1u << 20) && ctas <= 4096) return (int)((((uint32_t)u + 1) * (uint32_t)ctas - 1) / (uint32_t)units);
     return (int)(((u + 1) * (uint64_t)ctas - 1) / units);
+}
+
+LRM_HD uint64_t quotient(uint64_t a, uint64_t b) {
+    return (a | b) >> 32 ? a / b : (uint64_t)((uint32_t)a / (uint32_t)b);
 }
 
 }  // namespace sched
