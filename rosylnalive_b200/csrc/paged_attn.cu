@@ -29,6 +29,7 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <math.h>
+#include <stddef.h>
 #include <stdint.h>
 
 #include "internal.h"
@@ -49,7 +50,8 @@ constexpr int kRegsControl = 72, kRegsSoftmax = 216;
 static_assert(128 * kRegsControl + 256 * kRegsSoftmax <= kThreads * kRegsLaunch, "register split exceeds the launch");
 constexpr float kRescaleThreshold = 8.0f;  // log2 units: the reference maximum moves only when a tile exceeds it by more
 constexpr int kLeastUnits = 2;
-constexpr int kSmallBoxRows = 16;  // items of up to this many rows load q with a small box
+constexpr int kFewRows = 32;    // items of up to this many rows run with keys and rows swapped
+constexpr int FEW_SUB = kFewRows * 128;  // half of the dims (q) or keys (P) of up to 32 rows
 constexpr uint32_t kErrWaitProducer = 0x4010, kErrWaitIssuer = 0x4011, kErrWaitSoftmax = 0x4012, kErrWaitScheduler = 0x4013;
 
 // One item's share of a CTA's range: key tiles [kb, ke) of it.
@@ -72,7 +74,7 @@ struct Request {
     int start, n, kv, slot;
 };
 struct Control {
-    uint64_t q_full, q_empty, fin, o_free;
+    uint64_t q_full[2], q_empty[2], fin, o_free;  // q: even and odd items
     uint64_t kv_full[KV_ST], kv_empty[KV_ST];
     uint64_t s_full[SLOTS], p_part[SLOTS], p_full[SLOTS], o_done[SLOTS];
     uint64_t item_full[ITEMS], item_empty[ITEMS];
@@ -83,14 +85,25 @@ struct Control {
     int start_req;
     uint32_t tmem;
     int poison[SLOTS][2];  // [slot][item parity]: the item (counted from 1) in which v of a visible key was zeroed
-    float ml[SLOTS][128][2];
+    union {
+        float ml[SLOTS][128][2];  // narrow: the slots' states
+        struct {                  // few
+            union {
+                alignas(16) float max[SLOTS][kFewRows][4];  // a tile's maxima, by row and warp (read as float4)
+                float l[SLOTS][4][kFewRows];    // sums of p, by warp and row
+            };
+            float m[SLOTS][kFewRows], neg[SLOTS][kFewRows], alpha[SLOTS][kFewRows];
+        } few;
+    };
 };
+static_assert(offsetof(Control, few) % 16 == 0, "few.max is read as float4");
 constexpr int SMEM_BYTES = (SLOTS + KV_ST) * TILE + (int)sizeof(Control);
 static_assert(SMEM_BYTES <= 227 * 1024, "shared memory of one CTA");
 
 struct Params {
     PagedAttnArgs a;
     int group, tt, rows_cap;  // query heads a KV head; tokens a slot; rows of a partial slot
+    int few_tok;              // tokens of a few-row item's q box
     float *part_o, *part_ml;
     Record *records;
 };
@@ -112,9 +125,10 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 // ptx::mbar_wait with its loop kept small: the kernel has some thirty waits, and its warps' loops together have to fit
 // the SM's instruction cache (unrolled waits alone were 60 KB of code, and every role then stalled on fetches).
+constexpr uint32_t kPolls = 1u << 20;  // a second or so; waits are microseconds
 __device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, uint32_t *err, uint32_t code) {
 #pragma unroll 1
-    for (uint32_t i = 0; i < ptx::kWaitLimit; ++i)
+    for (uint32_t i = 0; i < kPolls; ++i)
         if (ptx::mbar_try_wait(bar, parity)) return true;
     atomicCAS(err, 0u, code);
     return false;
@@ -221,8 +235,280 @@ __device__ __forceinline__ void quad_transpose(uint4 (&v)[4], int lane) {
     }
 }
 
+// ---- items of few rows ------------------------------------------------------------------------------------------
+//
+// With 1 to 32 rows (single tokens, short drafts) most of a 128-row tile would be empty and a thread would walk 128
+// scores alone. So keys and rows change places: the keys fill the MMA's 128 rows, S^T = K Q^T has 16 or 32 columns, one a
+// row, and a thread holds one key's scores. The running maximum of a row is the same in all threads of a slot's
+// warpgroup and moves only when some score exceeds it by 2^8, which one barrier with an OR finds out; only then (and at
+// an item's first tile) are the tile's maxima reduced over threads. P goes to shared memory as the B operand of
+// O^T = V^T P^T; sums of p stay per thread until the end. A tile costs some 500 cycles beside its MMAs' 512, which hides
+// under the 2,600 that its K and V take from HBM.
+struct RoleState {
+    Control *c;
+    const Params *p;
+    uint8_t *kv, *pt;  // K/V ring; this slot's P
+    uint32_t tmem;
+    int s, quarter, lane, cta, k, ring;
+};
+
+__device__ __forceinline__ bool barrier_or(int id, int count, bool x) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, %2, %3, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r)
+        : "r"((int)x), "r"(id), "r"(count)
+        : "memory");
+    return r != 0;
+}
+__device__ __forceinline__ float warp_max(float x) {
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ void tmem_ld8(uint32_t t, float (&x)[8]) {
+    uint32_t *r = reinterpret_cast<uint32_t *>(x);
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(t));
+}
+__device__ __forceinline__ void tmem_st8(uint32_t t, const float (&x)[8]) {
+    const uint32_t *r = reinterpret_cast<const uint32_t *>(x);
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(t), "r"(r[0]),
+                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+
+// The sum of the values that clean_v zeroed in dim d of keys lo .. hi in tiles tile0, tile0 + step, ... (infinite or NaN, or
+// 0 if there are none).
+__device__ __noinline__ float poison_sum(const PagedAttnArgs &a, int64_t table, int kvh, int lo, int hi, int tile0, int step,
+                                         int d) {
+    float sum = 0.f;
+#pragma unroll 1
+    for (int key = lo; key <= hi; ++key) {
+        if ((key / TK - tile0) % step != 0) continue;  // the other slot's tile
+        const int pg = a.page_table[table + key / kPageTokens];
+        if (pg < 0 || pg >= a.kv_pages) continue;
+        const float x = __bfloat162float(a.pool[(size_t)pg * kv_page_elems(a.kv_heads) +
+                                                (size_t)(kvh * 2 + 1) * (kPageTokens * kHeadDim) +
+                                                (key % kPageTokens) * kHeadDim + d]);
+        if (!(fabsf(x) < INFINITY)) sum += x;
+    }
+    return sum;
+}
+
+// Eight rows' scores of this thread's key; rows that do not see it (those before `from`) as -inf.
+__device__ __forceinline__ void load_scores(uint32_t t, int from, float (&x)[8]) {
+    tmem_ld8(t, x);
+    ptx::tmem_ld_wait();
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = e >= from ? x[e] : -INFINITY;
+}
+
+// An item's tiles in one slot and its epilogue, eight rows at a time in rolled loops (code that the instruction cache
+// holds). Columns of the slot's tensor memory: S^T at 0, O^T at 128, the thread's sums of p at 192 (not beside S^T, which the
+// next item's first scores may overwrite while this item is still read out).
+__device__ __forceinline__ bool few_item(const RoleState &r, const Item &it, uint32_t &steps, uint32_t (&done)[SLOTS]) {
+    Control &c = *r.c;
+    const PagedAttnArgs &a = r.p->a;
+    const int s = r.s, lane = r.lane, group = r.p->group, nt = it.ke - it.kb, rows = it.ntok * group;
+    const int key = r.quarter * 32 + lane;
+    const uint32_t lanes = (uint32_t)(r.quarter * 32) << 16, tS = r.tmem + 256 * s + lanes, tO = tS + 128, tL = tS + 192;
+    const float sc = a.scale_log2;
+    // P[row][key] with keys contiguous, 64 a 128-byte swizzled line
+    const uint32_t pt = ptx::smem_u32(r.pt) + (key >> 6) * FEW_SUB, pk = (key & 63) * 2;
+#pragma unroll 1
+    for (int j = s; j < nt; j += 2, ++steps) {
+        if (!wait_bar(&c.s_full[s], steps & 1, a.err, kErrWaitSoftmax)) return false;
+        ptx::tc_fence_after();
+        const int key0 = (it.kb + j) * TK;
+        const bool first = j == s, dirty = key0 + TK - 1 > it.pos0;  // dirty: some row does not see the whole tile
+        // rows are token-major, so the key is seen from this row on
+        const int from = dirty ? min(max(key0 + key - it.pos0, 0), 64) * group : 0;
+        bool over = first;
+        if (!first) {
+#pragma unroll 1
+            for (int g = 0; g < rows; g += 8) {
+                float x[8];
+                load_scores(tS + g, from - g, x);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) over |= g + e < rows && x[e] * sc > c.few.m[s][g + e] + kRescaleThreshold;
+            }
+        }
+        if (barrier_or(6 + s, 128, over)) {
+#pragma unroll 1
+            for (int g = 0; g < rows; g += 8) {
+                float x[8];
+                load_scores(tS + g, from - g, x);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float w = warp_max(x[e]);
+                    if (lane == e) c.few.max[s][g + e][r.quarter] = w;
+                }
+            }
+            ptx::named_barrier(6 + s, 128);
+            if (key < kFewRows) {  // thread = row
+                const float4 w = *reinterpret_cast<const float4 *>(c.few.max[s][key]);
+                const float mx = fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w)) * sc, old = c.few.m[s][key];
+                const bool up = first || mx > old + kRescaleThreshold;
+                c.few.alpha[s][key] = up ? ptx::ex2(old - mx) : 1.f;  // 0 when no key was seen before
+                if (up) {
+                    c.few.m[s][key] = mx;
+                    c.few.neg[s][key] = mx == -INFINITY ? 0.f : -mx;  // a row that has seen no key yet: p = 0
+                }
+            }
+            ptx::named_barrier(6 + s, 128);
+            if (!first) {  // this S was issued behind the slot's last product, so O is quiescent
+#pragma unroll 1
+                for (int g = 0; g < rows; g += 8) {
+                    float o[8], l[8];
+                    tmem_ld8(tO + g, o);
+                    tmem_ld8(tL + g, l);
+                    ptx::tmem_ld_wait();
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float alpha = c.few.alpha[s][g + e];
+                        o[e] *= alpha;
+                        l[e] *= alpha;
+                    }
+                    tmem_st8(tO + g, o);
+                    tmem_st8(tL + g, l);
+                }
+                ptx::tmem_st_wait();
+            }
+        }
+#pragma unroll 1
+        for (int g = 0; g < rows; g += 8) {
+            float x[8], l[8];
+            tmem_ld8(tL + g, l);
+            load_scores(tS + g, from - g, x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float w = ptx::ex2(fmaf(x[e], sc, c.few.neg[s][g + e]));
+                l[e] = first ? w : l[e] + w;
+                const __nv_bfloat16 h = __float2bfloat16_rn(w);
+                asm volatile("st.shared.b16 [%0], %1;" ::"r"(pt + (g + e) * 128 + (pk ^ (e << 4))),
+                             "h"(*reinterpret_cast<const uint16_t *>(&h))
+                             : "memory");
+            }
+            tmem_st8(tL + g, l);
+        }
+        if (dirty) {
+            const int xv = r.ring + 2 * j + 1;
+            if (!wait_bar(&c.kv_full[xv % KV_ST], (xv / KV_ST) & 1, a.err, kErrWaitSoftmax)) return false;
+            clean_v(r.kv + (xv % KV_ST) * TILE, key, lane, it.pos0 + it.ntok - 1 - key0, &c.poison[s][r.k & 1], r.k + 1);
+        } else {
+            ptx::fence_proxy_async();  // P is read through the async proxy
+        }
+        ptx::tmem_st_wait();
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+            ptx::mbar_arrive(&c.p_part[s]);
+            ptx::mbar_arrive(&c.p_full[s]);
+        }
+    }
+
+    const bool two = nt > 1;  // the second slot has a state
+    bool ok = wait_bar(&c.o_done[0], done[0]++ & 1, a.err, kErrWaitSoftmax);
+    if (ok && two) ok = wait_bar(&c.o_done[1], done[1]++ & 1, a.err, kErrWaitSoftmax);
+    if (!ok) return false;
+    ptx::tc_fence_after();
+    if (c.poison[0][r.k & 1] == r.k + 1 || c.poison[1][r.k & 1] == r.k + 1) {
+        if (nt > s)
+#pragma unroll 1
+            for (int e = 0; e < rows; ++e) {
+                uint32_t o;
+                asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(o) : "r"(tO + e));
+                ptx::tmem_ld_wait();
+                o = __float_as_uint(__uint_as_float(o) +
+                                    poison_sum(a, it.table, it.kvh, max(it.kb * TK, it.pos0 / TK * TK),
+                                               min(it.pos0 + e / group, it.ke * TK - 1), it.kb + s, 2, key));
+                asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(tO + e), "r"(o) : "memory");
+            }
+        ptx::tmem_st_wait();
+        ptx::tc_fence_before();
+        ptx::named_barrier(1, 256);
+        ptx::tc_fence_after();
+    }
+    // This warp's sums of each row's p: eight rows over 32 lanes, each step halving the rows that a lane holds.
+    if (nt > s) {
+#pragma unroll 1
+        for (int g = 0; g < rows; g += 8) {
+            float l[8];
+            tmem_ld8(tL + g, l);
+            ptx::tmem_ld_wait();
+#pragma unroll
+            for (int o = 4; o > 0; o /= 2) {
+                const bool up = lane & o;
+#pragma unroll
+                for (int e = 0; e < o; ++e) {
+                    const float give = up ? l[e] : l[e + o], keep = up ? l[e + o] : l[e];
+                    l[e] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+                }
+            }
+            l[0] += __shfl_xor_sync(0xffffffffu, l[0], 8);
+            l[0] += __shfl_xor_sync(0xffffffffu, l[0], 16);
+            if (lane < 8) c.few.l[s][r.quarter][g + lane] = l[0];
+        }
+    }
+    ptx::named_barrier(1, 256);
+    // Lane e: row e's place in the output and its weights of the two slots' O.
+    const float m0 = c.few.m[0][lane], m1 = c.few.m[1][lane];
+    float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        l0 += c.few.l[0][q][lane];
+        l1 += c.few.l[1][q][lane];
+    }
+    ptx::named_barrier(1, 256);  // read by both before either may write there again
+    if (!two) l1 = 0.f;
+    const float mt = l0 == 0.f ? m1 : (l1 == 0.f ? m0 : fmaxf(m0, m1));
+    float w0 = l0 == 0.f ? 0.f : ptx::ex2(m0 - mt), w1 = l1 == 0.f ? 0.f : ptx::ex2(m1 - mt);
+    const float lt = (l0 == 0.f ? 0.f : w0 * l0) + (l1 == 0.f ? 0.f : w1 * l1);
+    const size_t part = ((size_t)r.cta * 2 + (it.dest > 0)) * r.p->rows_cap;
+    const int tok = lane / group;
+    int64_t at;  // of the row in out, or in the partial results
+    if (it.dest < 0) {
+        const float inv = 1.f / lt;
+        w0 *= inv;
+        w1 *= inv;
+        at = (int64_t)(it.tok0 + tok) * a.ld_out + (int64_t)(it.kvh * group + lane - tok * group) * kHeadDim;
+    } else {
+        at = (int64_t)(part + lane) * kHeadDim;
+        if (s == 0 && r.quarter == 0 && lane < rows)
+            *reinterpret_cast<float2 *>(r.p->part_ml + (part + lane) * 2) = make_float2(mt, lt);
+    }
+    // Every other eight rows are this warpgroup's to write; thread = dim.
+#pragma unroll 1
+    for (int g = 8 * s; g < rows; g += 16) {
+        float o[8], o1[8];
+        tmem_ld8(r.tmem + lanes + 128 + g, o);
+        if (two) tmem_ld8(r.tmem + lanes + 256 + 128 + g, o1);
+        ptx::tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            o[e] *= __shfl_sync(0xffffffffu, w0, g + e);
+            const float v1 = __shfl_sync(0xffffffffu, w1, g + e);
+            if (two) o[e] = fmaf(o1[e], v1, o[e]);
+            const int64_t to = __shfl_sync(0xffffffffu, at, g + e) + key;
+            if (g + e < rows) {
+                if (it.dest < 0)
+                    a.out[to] = __float2bfloat16_rn(o[e]);
+                else
+                    r.p->part_o[to] = o[e];
+            }
+        }
+    }
+    ptx::tc_fence_before();
+    __syncwarp();
+    if (lane == 0) ptx::mbar_arrive(&c.o_free);
+    return true;
+}
+
 __global__ void __launch_bounds__(kThreads, 1)
-    paged_attn_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tq_small,
+    paged_attn_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tq_few,
                       const __grid_constant__ CUtensorMap tkv, const __grid_constant__ Params p) {
     ptx::griddep_wait();
     ptx::griddep_launch();
@@ -245,8 +531,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if (warp == 2) {
         if (lane == 0) {
-            ptx::mbar_init(&c.q_full, 2);  // the two producer warps
-            ptx::mbar_init(&c.q_empty, 1);
+            ptx::mbar_init(&c.q_full[0], 2);  // the two producer warps
+            ptx::mbar_init(&c.q_full[1], 2);
+            ptx::mbar_init(&c.q_empty[0], 1);
+            ptx::mbar_init(&c.q_empty[1], 1);
             ptx::mbar_init(&c.fin, 1);
             ptx::mbar_init(&c.o_free, 8);
             for (int s = 0; s < KV_ST; ++s) {
@@ -271,7 +559,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         ptx::tmem_relinquish();
     } else if (warp == 0 && lane == 0) {
         ptx::prefetch_tmap(&tq);
-        ptx::prefetch_tmap(&tq_small);
+        ptx::prefetch_tmap(&tq_few);
         ptx::prefetch_tmap(&tkv);
     }
 
@@ -386,8 +674,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             // ---- TMA producers: warp 0 the first 64 dims of every tile, warp 3 the others ----
             const int half = warp == 3;
             const int oob = a.kv_pages * a.kv_heads * 2;  // past the tensor map: read as zeros, without a memory access
-            int ring = 0;  // ring items issued so far
-            bool ok = true;
+            int ring = 0;    // ring items issued so far
+            int q_free = 0;  // items known to be through with q
+            bool ok = true, few_before = false;
             for (int k = 0; ok; ++k) {
                 if (lane == 0) ok = wait_bar(&c.item_full[k % ITEMS], (k / ITEMS) & 1, err, kErrWaitProducer);
                 ok = __shfl_sync(0xffffffffu, ok, 0);
@@ -407,19 +696,24 @@ __global__ void __launch_bounds__(kThreads, 1)
                     return oob;
                 };
                 int z = fetch(it.kb), z_next = it.kb + 4 < it.ke ? fetch(it.kb + 4) : oob;
+                const bool few = it.ntok * p.group <= kFewRows;
                 if (lane == 0) {
-                    ok = wait_bar(&c.q_empty, (k & 1) ^ 1, err, kErrWaitProducer);
+                    // Two few-row items in a row use different places for q, so the second one's q is loaded while the
+                    // first still runs; otherwise q's place is free once the item before is through. Even and odd items
+                    // have a barrier each: one that is waited for late, behind two items, would have lost its phase.
+                    for (const int need = few && few_before ? k - 1 : k; ok && q_free < need; ++q_free)
+                        ok = wait_bar(&c.q_empty[q_free & 1], (q_free >> 1) & 1, err, kErrWaitProducer);
                     if (ok) {
-                        const bool small = it.ntok * p.group <= kSmallBoxRows;
-                        const int slots = it.ntok > p.tt ? 2 : 1;
-                        const int box_tok = small ? max(1, kSmallBoxRows / p.group) : p.tt;
-                        const CUtensorMap *map = small ? &tq_small : &tq;
-                        ptx::mbar_arrive_expect_tx(&c.q_full, slots * box_tok * p.group * 128);
+                        const int slots = it.ntok > p.tt ? 2 : 1, rows = (few ? p.few_tok : p.tt) * p.group;
+                        uint64_t *bar = &c.q_full[k & 1];
+                        uint8_t *dst = few ? sQ + (k & 1) * 2 * FEW_SUB + half * FEW_SUB : sQ + half * SUB;
+                        ptx::mbar_arrive_expect_tx(bar, slots * rows * 128);
                         for (int s = 0; s < slots; ++s)
-                            ptx::tma_load_3d(sQ + s * TILE + half * SUB, map, &c.q_full, 64 * half, it.kvh * p.group,
+                            ptx::tma_load_3d(dst + s * TILE, few ? &tq_few : &tq, bar, 64 * half, it.kvh * p.group,
                                              it.tok0 + s * p.tt);
                     }
                 }
+                few_before = few;
                 ok = __shfl_sync(0xffffffffu, ok, 0);
                 for (int t = it.kb; ok && t < it.ke; ++t) {
                     const int sub = (t - it.kb) & 3;
@@ -471,8 +765,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const int nt = c.items[k % ITEMS].ke - c.items[k % ITEMS].kb;
                     ptx::mbar_arrive(&c.item_empty[k % ITEMS]);
                     if (ntok == 0) break;
-                    const bool wide = ntok > p.tt;
-                    if (!wait(&c.q_full, k & 1)) break;
+                    const bool wide = ntok > p.tt, few = ntok * p.group <= kFewRows;
+                    // few: S^T = K Q^T (128 keys x 16 or 32 rows) and O^T = V^T P^T (128 dims x rows)
+                    const int nrow = ntok * p.group <= 16 ? 16 : 32;
+                    const uint32_t idesc_s = few ? ptx::idesc_bf16_f32(128, nrow) : idesc_qk;
+                    const uint32_t idesc_o = ptx::idesc_bf16_f32(128, nrow) | 1u << 15;  // A (V) MN-major
+                    if (!wait(&c.q_full[k & 1], (k >> 1) & 1)) break;
                     // Products n = 0 .. count - 1: slot n & 1, key tile n / 2 (wide) or n (narrow). Step n issues
                     // O += P V of product n - 2, then S = Q K^T of product n in the same slot. The tensor core runs one
                     // thread's MMAs in order, so S overwrites P only after its product with V has read it.
@@ -489,14 +787,24 @@ __global__ void __launch_bounds__(kThreads, 1)
                             const uint32_t keep = n - 2 >= 2 ? 1u : 0u;  // the slot's first product overwrites O
                             const uint64_t v = ptx::sw128_mnmajor_desc(ptx::smem_u32(sKV + (x % KV_ST) * TILE), SUB, 1024);
                             if (!wait(&c.p_part[s], steps[s] & 1)) break;
-                            ptx::mma_bf16_ts(tS + 128, tS, v, idesc_pv, keep);
+                            if (few) {
+                                const uint64_t pt = ptx::sw128_kmajor_desc(ptx::smem_u32(sQ + TILE + s * 2 * FEW_SUB));
+                                if (!wait(&c.p_full[s], steps[s] & 1)) break;
 #pragma unroll
-                            for (int kk = 1; kk < 6; ++kk)
-                                ptx::mma_bf16_ts(tS + 128, tS + kk * 8, v + kk * (2048 >> 4), idesc_pv, 1u);
-                            if (!wait(&c.p_full[s], steps[s] & 1)) break;
+                                for (int kk = 0; kk < 8; ++kk)
+                                    ptx::mma_bf16(tS + 128, v + kk * (2048 >> 4),
+                                                  pt + (((kk >> 2) * FEW_SUB + (kk & 3) * 32) >> 4), idesc_o,
+                                                  kk > 0 ? 1u : keep);
+                            } else {
 #pragma unroll
-                            for (int kk = 6; kk < 8; ++kk)
-                                ptx::mma_bf16_ts(tS + 128, tS + kk * 8, v + kk * (2048 >> 4), idesc_pv, 1u);
+                                for (int kk = 0; kk < 6; ++kk)
+                                    ptx::mma_bf16_ts(tS + 128, tS + kk * 8, v + kk * (2048 >> 4), idesc_pv,
+                                                     kk > 0 ? 1u : keep);
+                                if (!wait(&c.p_full[s], steps[s] & 1)) break;
+#pragma unroll
+                                for (int kk = 6; kk < 8; ++kk)
+                                    ptx::mma_bf16_ts(tS + 128, tS + kk * 8, v + kk * (2048 >> 4), idesc_pv, 1u);
+                            }
                             ++steps[s];
                             if (!wide || s == 1) ptx::mma_commit(&c.kv_empty[x % KV_ST]);
                             if (n >= count) ptx::mma_commit(&c.o_done[s]);
@@ -504,18 +812,21 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (n < count) {
                             const int x = ring + 2 * (wide ? n >> 1 : n);
                             if (!wait_ring(x)) break;
-                            const uint64_t q = ptx::sw128_kmajor_desc(ptx::smem_u32(sQ + (wide ? s : 0) * TILE));
                             const uint64_t kt = ptx::sw128_kmajor_desc(ptx::smem_u32(sKV + (x % KV_ST) * TILE));
+                            const uint64_t q = ptx::sw128_kmajor_desc(
+                                ptx::smem_u32(sQ + (few ? (k & 1) * 2 * FEW_SUB : (wide ? s : 0) * TILE)));
+                            const uint64_t x0 = few ? kt : q, y0 = few ? q : kt;  // the operand of 128 rows, and the other
+                            const uint32_t half = (few ? FEW_SUB : SUB) >> 4, xhalf = SUB >> 4;
 #pragma unroll
-                            for (int kk = 0; kk < 8; ++kk) {
-                                const int o = ((kk >> 2) * SUB + (kk & 3) * 32) >> 4;
-                                ptx::mma_bf16(tS, q + o, kt + o, idesc_qk, kk > 0 ? 1u : 0u);
-                            }
+                            for (int kk = 0; kk < 8; ++kk)
+                                ptx::mma_bf16(tS, x0 + (kk >> 2) * xhalf + (kk & 3) * 2,
+                                              y0 + (kk >> 2) * half + (kk & 3) * 2, idesc_s, kk > 0 ? 1u : 0u);
                             ptx::mma_commit(&c.s_full[s]);
                             if (!wide || s == 1) ptx::mma_commit(&c.kv_empty[x % KV_ST]);
-                            if (n == count - 1) ptx::mma_commit(&c.q_empty);
+                            if (n == count - 1 && !few) ptx::mma_commit(&c.q_empty[k & 1]);
                         }
                     }
+                    if (few) ptx::mma_commit(&c.q_empty[k & 1]);  // P lies beside q
                     ring += 2 * nt;
                 }
                 // No MMA may still be writing TMEM when it is freed (this matters on the error path).
@@ -549,6 +860,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(&c.item_empty[k % ITEMS]);
             if (it.ntok == 0) break;
+            if (it.ntok * p.group <= kFewRows) {
+                const RoleState r = {&c, &p, sKV, sQ + TILE + s * 2 * FEW_SUB, tmem, s, quarter, lane, cta, k, ring};
+                ok = few_item(r, it, steps, done);
+                ring += 2 * (it.ke - it.kb);
+                if (!ok) break;
+                continue;
+            }
             const bool wide = it.ntok > p.tt;
             const int token = wide ? s * p.tt + tl : tl;  // of the item
             const bool valid = tl < p.tt && token < it.ntok;
@@ -557,6 +875,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int nt = it.ke - it.kb;
             float m_ref = -INFINITY, l = 0.f;
             bool first = true;
+#pragma unroll 1
             for (int j = wide ? 0 : s; j < nt; j += wide ? 1 : 2, ++steps) {
                 if (!wait_bar(&c.s_full[s], steps & 1, err, kErrWaitSoftmax)) {
                     ok = false;
@@ -678,6 +997,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 w[0] = l0 == 0.f ? 0.f : ptx::ex2(m0 - m_ref);
                 w[1] = l1 == 0.f ? 0.f : ptx::ex2(m1 - m_ref);
                 l = (l0 == 0.f ? 0.f : w[0] * l0) + (l1 == 0.f ? 0.f : w[1] * l1);
+                ptx::named_barrier(1, 256);  // read by both before either may write there again
             }
             const bool poisoned = c.poison[0][k & 1] == k + 1 || c.poison[1][k & 1] == k + 1;
             if (active) {
@@ -850,17 +1170,17 @@ cudaError_t launch_paged_attention(const PagedAttnArgs &a, int sms, cudaStream_t
     p.records = reinterpret_cast<Record *>(a.workspace);
     p.part_o = reinterpret_cast<float *>(p.records + sms);
     p.part_ml = p.part_o + (size_t)sms * 2 * p.rows_cap * kHeadDim;
-    const uint32_t small = kSmallBoxRows / p.group > 0 ? kSmallBoxRows / p.group : 1;
-    CUtensorMap tq, tq_small, tkv;
+    p.few_tok = kFewRows / p.group > 0 ? kFewRows / p.group : 1;
+    CUtensorMap tq, tq_few, tkv;
     const uint64_t qrow = (uint64_t)a.ld_q * 2;
     if (!make_tmap(&tq, a.q, a.q_heads, a.tokens, kHeadDim * 2, qrow, p.group, p.tt) ||
-        !make_tmap(&tq_small, a.q, a.q_heads, a.tokens, kHeadDim * 2, qrow, p.group, small) ||
+        !make_tmap(&tq_few, a.q, a.q_heads, a.tokens, kHeadDim * 2, qrow, p.group, p.few_tok) ||
         !make_tmap(&tkv, a.pool, kPageTokens, (uint64_t)a.kv_pages * a.kv_heads * 2, kHeadDim * 2,
                    kPageTokens * kHeadDim * 2, kPageTokens, 1))
         return cudaErrorInvalidValue;
     static SmemOptIn opt;
     if (cudaError_t e = opt.set((const void *)paged_attn_kernel, SMEM_BYTES)) return e;
-    cudaError_t e = launch_kernel(paged_attn_kernel, dim3(sms), dim3(kThreads), SMEM_BYTES, st, tq, tq_small, tkv, p);
+    cudaError_t e = launch_kernel(paged_attn_kernel, dim3(sms), dim3(kThreads), SMEM_BYTES, st, tq, tq_few, tkv, p);
     if (e != cudaSuccess) return e;
     // The merge launches under the attention kernel's tail; its own wait orders it behind that kernel's writes.
     cudaLaunchConfig_t cfg = {};
