@@ -49,7 +49,7 @@ constexpr int kRegsLaunch = 168;  // 65536 / 384, rounded down to the allocation
 constexpr int kRegsControl = 72, kRegsSoftmax = 216;
 static_assert(128 * kRegsControl + 256 * kRegsSoftmax <= kThreads * kRegsLaunch, "register split exceeds the launch");
 constexpr float kRescaleThreshold = 8.0f;  // log2 units: the reference maximum moves only when a tile exceeds it by more
-constexpr int kLeastUnits = 2;
+constexpr int kLeastUnits = 4;
 constexpr int kFewRows = 32;    // items of up to this many rows run with keys and rows swapped
 constexpr int FEW_SUB = kFewRows * 128;  // half of the dims (q) or keys (P) of up to 32 rows
 constexpr uint32_t kErrWaitProducer = 0x4010, kErrWaitIssuer = 0x4011, kErrWaitSoftmax = 0x4012, kErrWaitScheduler = 0x4013;
@@ -298,6 +298,11 @@ __device__ __noinline__ float poison_sum(const PagedAttnArgs &a, int64_t table, 
     return sum;
 }
 
+__device__ __forceinline__ void load8(const float *shared, float (&x)[8]) {
+    const float4 a = reinterpret_cast<const float4 *>(shared)[0], b = reinterpret_cast<const float4 *>(shared)[1];
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+}
+
 // Eight rows' scores of this thread's key; rows that do not see it (those before `from`) as -inf.
 __device__ __forceinline__ void load_scores(uint32_t t, int from, float (&x)[8]) {
     tmem_ld8(t, x);
@@ -330,10 +335,11 @@ __device__ __forceinline__ bool few_item(const RoleState &r, const Item &it, uin
         if (!first) {
 #pragma unroll 1
             for (int g = 0; g < rows; g += 8) {
-                float x[8];
+                float x[8], m[8];
+                load8(&c.few.m[s][g], m);
                 load_scores(tS + g, from - g, x);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) over |= g + e < rows && x[e] * sc > c.few.m[s][g + e] + kRescaleThreshold;
+                for (int e = 0; e < 8; ++e) over |= g + e < rows && x[e] * sc > m[e] + kRescaleThreshold;
             }
         }
         if (barrier_or(6 + s, 128, over)) {
@@ -362,15 +368,15 @@ __device__ __forceinline__ bool few_item(const RoleState &r, const Item &it, uin
             if (!first) {  // this S was issued behind the slot's last product, so O is quiescent
 #pragma unroll 1
                 for (int g = 0; g < rows; g += 8) {
-                    float o[8], l[8];
+                    float o[8], l[8], alpha[8];
+                    load8(&c.few.alpha[s][g], alpha);
                     tmem_ld8(tO + g, o);
                     tmem_ld8(tL + g, l);
                     ptx::tmem_ld_wait();
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        const float alpha = c.few.alpha[s][g + e];
-                        o[e] *= alpha;
-                        l[e] *= alpha;
+                        o[e] *= alpha[e];
+                        l[e] *= alpha[e];
                     }
                     tmem_st8(tO + g, o);
                     tmem_st8(tL + g, l);
@@ -380,18 +386,23 @@ __device__ __forceinline__ bool few_item(const RoleState &r, const Item &it, uin
         }
 #pragma unroll 1
         for (int g = 0; g < rows; g += 8) {
-            float x[8], l[8];
+            float x[8], l[8], neg[8];
+            load8(&c.few.neg[s][g], neg);
             tmem_ld8(tL + g, l);
             load_scores(tS + g, from - g, x);
+            uint32_t w[4];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float w = ptx::ex2(fmaf(x[e], sc, c.few.neg[s][g + e]));
-                l[e] = first ? w : l[e] + w;
-                const __nv_bfloat16 h = __float2bfloat16_rn(w);
-                asm volatile("st.shared.b16 [%0], %1;" ::"r"(pt + (g + e) * 128 + (pk ^ (e << 4))),
-                             "h"(*reinterpret_cast<const uint16_t *>(&h))
-                             : "memory");
+                x[e] = ptx::ex2(fmaf(x[e], sc, neg[e]));
+                l[e] = first ? x[e] : l[e] + x[e];
             }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = pack2(x[2 * e], x[2 * e + 1]);
+            const uint32_t row = pt + g * 128;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                asm volatile("st.shared.b16 [%0], %1;" ::"r"(row + e * 128 + (pk ^ (e << 4))),
+                             "h"((uint16_t)(w[e / 2] >> (e & 1 ? 16 : 0))));
             tmem_st8(tL + g, l);
         }
         if (dirty) {
@@ -404,10 +415,7 @@ __device__ __forceinline__ bool few_item(const RoleState &r, const Item &it, uin
         ptx::tmem_st_wait();
         ptx::tc_fence_before();
         __syncwarp();
-        if (lane == 0) {
-            ptx::mbar_arrive(&c.p_part[s]);
-            ptx::mbar_arrive(&c.p_full[s]);
-        }
+        if (lane == 0) ptx::mbar_arrive(&c.p_full[s]);
     }
 
     const bool two = nt > 1;  // the second slot has a state
@@ -626,32 +634,38 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const uint64_t off = c.start_off - (uint64_t)h * c.start_head;
                 int i = sched::item_at(q.n, q.kv, span, off);
                 int tiles = sched::item_tiles(q.n, q.kv, span, i);
-                int ke = (int)(off - sched::units_before(q.n, q.kv, span, i)) + 1;
+                sched::Cost cost = sched::item_cost(q.n, span, i);
+                // the share's end within the item, in units
+                int end = (int)(off - sched::units_before(q.n, q.kv, span, i)) + 1;
                 Record rec = {0, 0, 0, 0};
                 int k = 0;
-                bool ok = true;
-                while (ok) {
-                    ok = wait_bar(&c.item_empty[k % ITEMS], ((k / ITEMS) & 1) ^ 1, err, kErrWaitScheduler);
-                    if (!ok) break;
+                for (;;) {
                     Item it = {};
+                    int begin = 0;
                     if (left > 0) {
-                        it.kb = (uint64_t)ke > left ? ke - (int)left : 0;
-                        it.ke = ke;
+                        begin = (uint64_t)end > left ? end - (int)left : 0;
+                        it.kb = sched::tile_at(cost, begin);
+                        it.ke = sched::tile_at(cost, end);
                         it.tok0 = q.start + i * span;
                         it.ntok = min(span, q.n - i * span);
                         it.kvh = h;
                         it.pos0 = q.kv - q.n + i * span;
                         it.npages = (q.kv + kPageTokens - 1) / kPageTokens;
                         it.table = (int64_t)q.slot * a.pages_per_seq;
-                        it.dest = it.kb == 0 && ke == tiles ? -1 : (it.kb == 0 ? 1 : 0);
+                        it.dest = it.kb == 0 && it.ke == tiles ? -1 : (it.kb == 0 ? 1 : 0);
                     }
-                    c.items[k % ITEMS] = it;
-                    ptx::mbar_arrive(&c.item_full[k % ITEMS]);
-                    if (it.dest == 1)  // the range's last item, begun here: it ends (tiles - ke) units behind the range
-                        rec = Record{it.tok0, it.ntok, h, sched::cta_of(units, ctas, u1 - 1 + (uint64_t)(tiles - ke)) - cta};
-                    ++k;
+                    if (it.ke > it.kb || left == 0) {  // a share of the item's own cost alone has no tiles
+                        if (!wait_bar(&c.item_empty[k % ITEMS], ((k / ITEMS) & 1) ^ 1, err, kErrWaitScheduler)) break;
+                        c.items[k % ITEMS] = it;
+                        ptx::mbar_arrive(&c.item_full[k % ITEMS]);
+                        ++k;
+                        if (it.dest == 1)  // the range's last item, begun here: the rest of it lies behind the range
+                            rec = Record{it.tok0, it.ntok, h,
+                                         sched::cta_of(units, ctas, u1 - 1 + (uint64_t)(cost.own + cost.tile * tiles - end)) -
+                                             cta};
+                    }
                     if (left == 0) break;
-                    left -= (uint64_t)(ke - it.kb);
+                    left -= (uint64_t)(end - begin);
                     if (left == 0) continue;
                     // the item before: of this head, else of the head before, else of the request before
                     if (i > 0) {
@@ -666,7 +680,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                         i = sched::items_of(q.n, span) - 1;
                     }
-                    tiles = ke = sched::item_tiles(q.n, q.kv, span, i);
+                    tiles = sched::item_tiles(q.n, q.kv, span, i);
+                    cost = sched::item_cost(q.n, span, i);
+                    end = cost.own + cost.tile * tiles;
                 }
                 p.records[cta] = rec;
             }
@@ -751,7 +767,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 constexpr uint32_t idesc_qk = ptx::idesc_bf16_f32(128, 128, false);
                 constexpr uint32_t idesc_pv = ptx::idesc_bf16_f32(128, 128, true);
                 int ring = 0;              // ring items of the items before this one
-                uint32_t steps[SLOTS] = {};  // P tiles consumed so far, a slot
+                uint32_t steps[SLOTS] = {}, parts[SLOTS] = {};  // P tiles consumed so far, a slot; those in two parts
                 bool ok = true;
                 auto wait = [&](uint64_t *bar, uint32_t parity) {
                     if (ok) ok = wait_bar(bar, parity, err, kErrWaitIssuer);
@@ -786,7 +802,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                             if (n == 2 && k > 0 && !wait(&c.o_free, (k - 1) & 1)) break;
                             const uint32_t keep = n - 2 >= 2 ? 1u : 0u;  // the slot's first product overwrites O
                             const uint64_t v = ptx::sw128_mnmajor_desc(ptx::smem_u32(sKV + (x % KV_ST) * TILE), SUB, 1024);
-                            if (!wait(&c.p_part[s], steps[s] & 1)) break;
                             if (few) {
                                 const uint64_t pt = ptx::sw128_kmajor_desc(ptx::smem_u32(sQ + TILE + s * 2 * FEW_SUB));
                                 if (!wait(&c.p_full[s], steps[s] & 1)) break;
@@ -796,6 +811,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                                                   pt + (((kk >> 2) * FEW_SUB + (kk & 3) * 32) >> 4), idesc_o,
                                                   kk > 0 ? 1u : keep);
                             } else {
+                                if (!wait(&c.p_part[s], parts[s] & 1)) break;
+                                ++parts[s];
 #pragma unroll
                                 for (int kk = 0; kk < 6; ++kk)
                                     ptx::mma_bf16_ts(tS + 128, tS + kk * 8, v + kk * (2048 >> 4), idesc_pv,

@@ -2,10 +2,12 @@
 // be checked on the CPU).
 //
 // A request has n new tokens, the last of its kv keys, and `group` query heads a KV head. An item is up to `span`
-// consecutive tokens of one request and KV head, all their query heads; its unit of work is a tile of 128 keys, and it
-// has as many as its last token sees. All units of a call, ordered by (request, KV head, item, key), are cut into
-// `ctas` ranges of equal length, one a CTA, so every mixture of lengths is balanced; an item that a cut passes through
-// is merged from its CTAs' partial results.
+// consecutive tokens of one request and KV head, all their query heads, and reads as many tiles of 128 keys as its last
+// token sees. A wide item (more than half a span: both slots' rows) counts 2 units of work a tile and 3 for itself, a
+// narrow one 1 a tile and 2 for itself: about 2,500 cycles each, as measured. All units of a call, ordered by (request,
+// KV head, item, key), are cut into `ctas` ranges of equal length, one a CTA, so every mixture of lengths is balanced; an
+// item that a cut passes through is merged from its CTAs' partial results. (Counting tiles alone left 32 requests of 5
+// tokens over 100 to 6000 keys at 64 us against 43, and 8 chunks of 511 tokens among 56 decodes at 103 against 73.)
 #pragma once
 
 #include <stdint.h>
@@ -50,16 +52,30 @@ LRM_HD int item_tiles(int n, int kv, int span, int i) {
     return (kv - n + last - 1) / kTileKeys + 1;
 }
 
-// Units of the items before item i (i <= items - 1) of one head.
+// An item's units: `own` for its start and end, then `tile` a tile.
+struct Cost {
+    int own, tile;
+};
+LRM_HD Cost item_cost(int n, int span, int i) {
+    const bool wide = n - i * span > span / 2;
+    return wide ? Cost{3, 2} : Cost{2, 1};
+}
+// The first tile that lies behind `units` of an item's units (neighbouring shares round to the same tile).
+LRM_HD int tile_at(Cost c, int units) { return units > c.own ? (units - c.own) / c.tile : 0; }
+
+// Units of the items before item i (i <= items - 1, so all of them are wide) of one head.
 LRM_HD uint64_t units_before(int n, int kv, int span, int i) {
     if (i == 0) return 0;
-    return floor_sum((uint64_t)i, kTileKeys, (uint32_t)span, (uint64_t)(kv - n + span - 1)) + (uint64_t)i;
+    const Cost c = item_cost(n, span, 0);
+    return (floor_sum((uint64_t)i, kTileKeys, (uint32_t)span, (uint64_t)(kv - n + span - 1)) + (uint64_t)i) *
+               (uint64_t)c.tile + (uint64_t)i * c.own;
 }
 
 // Units of one head.
 LRM_HD uint64_t head_units(int n, int kv, int span) {
-    const int items = items_of(n, span);
-    return units_before(n, kv, span, items - 1) + (uint64_t)item_tiles(n, kv, span, items - 1);
+    const int last = items_of(n, span) - 1;
+    const Cost c = item_cost(n, span, last);
+    return units_before(n, kv, span, last) + (uint64_t)(item_tiles(n, kv, span, last) * c.tile + c.own);
 }
 
 // The item of a head that holds its unit `off`.
@@ -75,12 +91,12 @@ LRM_HD int item_at(int n, int kv, int span, uint64_t off) {
     return lo;
 }
 
-// CTAs that take part: at least `least` units each, so that short work is not cut into pieces that cost more to merge
-// than they save.
+// CTAs that take part: at least `least` units each (2 or more, so that a share within an item holds a tile), so that
+// short work is not cut into pieces that cost more to merge than they save.
 LRM_HD int ctas_of(uint64_t units, int ctas, int least) {
     if (units >= (uint64_t)ctas * (uint64_t)least) return ctas;
-    const uint32_t want = ((uint32_t)units + (uint32_t)least - 1) / (uint32_t)least;
-    return want < (uint32_t)ctas ? (int)want : ctas;
+    const int want = (int)((uint32_t)units / (uint32_t)least);
+    return want > 0 ? want : (units > 0 ? 1 : 0);
 }
 
 // Where CTA c's range starts. (32-bit arithmetic where it fits: a 64-bit division costs the start of a short call.)

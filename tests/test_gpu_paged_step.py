@@ -446,6 +446,8 @@ MIXES = {
     "one long, few rows": [(3, 20000)],
     "long chunk": [(700, 5000)],
     "many short": [(1, 1 + 7 * i % 300) for i in range(200)],
+    "many long": [(1, 2500 + 37 * i) for i in range(40)],
+    "all kinds in turn": [x for i in range(6) for x in ((1, 700 + i), (150, 900), (20, 400 + i), (3, 30), (40, 45), (1, 2))],
 }
 
 
