@@ -597,7 +597,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (w < warp) before += c.warp_sum[w];
         units += c.warp_sum[w];
     }
-    const uint32_t tmem = c.tmem;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, c.tmem, 0);
     const int ctas = sched::ctas_of(units, (int)gridDim.x, kLeastUnits);
     const bool idle = cta >= ctas;
     const uint64_t u0 = idle ? 0 : sched::cut(units, ctas, cta), u1 = idle ? 0 : sched::cut(units, ctas, cta + 1);
@@ -763,93 +763,117 @@ __global__ void __launch_bounds__(kThreads, 1)
                 wait_bar(&c.kv_full[x % KV_ST], (x / KV_ST) & 1, err, kErrWaitProducer);
         } else if (warp == 1) {
             // ---- tensor-core issuer ----
-            if (ptx::elect_one()) {
-                constexpr uint32_t idesc_qk = ptx::idesc_bf16_f32(128, 128, false);
-                constexpr uint32_t idesc_pv = ptx::idesc_bf16_f32(128, 128, true);
-                int ring = 0;              // ring items of the items before this one
-                uint32_t steps[SLOTS] = {}, parts[SLOTS] = {};  // P tiles consumed so far, a slot; those in two parts
-                bool ok = true;
-                auto wait = [&](uint64_t *bar, uint32_t parity) {
-                    if (ok) ok = wait_bar(bar, parity, err, kErrWaitIssuer);
-                    ptx::tc_fence_after();
-                    return ok;
-                };
-                auto wait_ring = [&](int x) { return wait(&c.kv_full[x % KV_ST], (x / KV_ST) & 1); };
-                for (int k = 0; ok; ++k) {
-                    if (!wait(&c.item_full[k % ITEMS], (k / ITEMS) & 1)) break;
-                    const int ntok = c.items[k % ITEMS].ntok;
-                    const int nt = c.items[k % ITEMS].ke - c.items[k % ITEMS].kb;
-                    ptx::mbar_arrive(&c.item_empty[k % ITEMS]);
-                    if (ntok == 0) break;
-                    const bool wide = ntok > p.tt, few = ntok * p.group <= kFewRows;
-                    // few: S^T = K Q^T (128 keys x 16 or 32 rows) and O^T = V^T P^T (128 dims x rows)
-                    const int nrow = ntok * p.group <= 16 ? 16 : 32;
-                    const uint32_t idesc_s = few ? ptx::idesc_bf16_f32(128, nrow) : idesc_qk;
-                    const uint32_t idesc_o = ptx::idesc_bf16_f32(128, nrow) | 1u << 15;  // A (V) MN-major
-                    if (!wait(&c.q_full[k & 1], (k >> 1) & 1)) break;
-                    // Products n = 0 .. count - 1: slot n & 1, key tile n / 2 (wide) or n (narrow). Step n issues
-                    // O += P V of product n - 2, then S = Q K^T of product n in the same slot. The tensor core runs one
-                    // thread's MMAs in order, so S overwrites P only after its product with V has read it.
-                    const int count = wide ? 2 * nt : nt;
+            // The whole warp runs this, with everything it goes by the same in all lanes, and one lane issues: so the
+            // descriptors are computed once a warp (in uniform registers), 5 instructions an MMA. (Inside one lane's
+            // branch an MMA took 110 cycles to issue, more than the 64 that it runs.)
+            constexpr uint32_t idesc_qk = ptx::idesc_bf16_f32(128, 128, false);
+            constexpr uint32_t idesc_pv = ptx::idesc_bf16_f32(128, 128, true);
+            constexpr uint32_t kHi = 1u << 14 | 2u << 29;  // descriptor bits 32-63: version 1, 128-byte swizzle
+            const uint32_t bQ = ptx::smem_u32(sQ) >> 4, bKV = ptx::smem_u32(sKV) >> 4;
+            int ring = 0;                // ring items of the items before this one
+            uint32_t steps[SLOTS] = {}, parts[SLOTS] = {};  // P tiles consumed so far, a slot; those in two parts
+            bool ok = true;
+            auto wait = [&](uint64_t *bar, uint32_t parity) {
+                ok = __all_sync(0xffffffffu, ok && wait_bar(bar, parity, err, kErrWaitIssuer));
+                ptx::tc_fence_after();
+                return ok;
+            };
+            auto wait_ring = [&](int x) { return wait(&c.kv_full[x % KV_ST], (x / KV_ST) & 1); };
+            // K-major: rows of 128 bytes, 8-row groups 1024 apart; MN-major (V): 64-dim halves SUB apart, the same groups
+            auto kmajor = [](uint32_t at) { return (uint64_t)(kHi | 1024 >> 4) << 32 | (1u << 16 | at); };
+            auto mnmajor = [](uint32_t at) { return (uint64_t)(kHi | 1024 >> 4) << 32 | ((uint32_t)(SUB >> 4) << 16 | at); };
+            for (int k = 0; ok; ++k) {
+                if (!wait(&c.item_full[k % ITEMS], (k / ITEMS) & 1)) break;
+                const int ntok = __shfl_sync(0xffffffffu, c.items[k % ITEMS].ntok, 0);
+                const int nt = __shfl_sync(0xffffffffu, c.items[k % ITEMS].ke - c.items[k % ITEMS].kb, 0);
+                if (lane == 0) ptx::mbar_arrive(&c.item_empty[k % ITEMS]);
+                if (ntok == 0) break;
+                const bool wide = ntok > p.tt, few = ntok * p.group <= kFewRows;
+                // few: S^T = K Q^T (128 keys x 16 or 32 rows) and O^T = V^T P^T (128 dims x rows)
+                const int nrow = ntok * p.group <= 16 ? 16 : 32;
+                const uint32_t idesc_s = few ? ptx::idesc_bf16_f32(128, nrow) : idesc_qk;
+                const uint32_t idesc_o = ptx::idesc_bf16_f32(128, nrow) | 1u << 15;  // A (V) MN-major
+                if (!wait(&c.q_full[k & 1], (k >> 1) & 1)) break;
+                // Products n = 0 .. count - 1: slot n & 1, key tile n / 2 (wide) or n (narrow, few). Step n issues
+                // O += P V of product n - 2, then S = Q K^T of product n in the same slot. The tensor core runs one
+                // thread's MMAs in order, so S overwrites P only after its product with V has read it.
+                const int count = wide ? 2 * nt : nt;
 #pragma unroll 1
-                    for (int n = 0; ok && n < count + 2; ++n) {
-                        const int s = n & 1;
-                        const uint32_t tS = tmem + 256 * s;
-                        if (n >= 2 && n - 2 < count) {
-                            const int x = ring + 2 * (wide ? (n - 2) >> 1 : n - 2) + 1;
-                            if (!wait_ring(x)) break;
-                            // O may be overwritten once the item before has been read out
-                            if (n == 2 && k > 0 && !wait(&c.o_free, (k - 1) & 1)) break;
-                            const uint32_t keep = n - 2 >= 2 ? 1u : 0u;  // the slot's first product overwrites O
-                            const uint64_t v = ptx::sw128_mnmajor_desc(ptx::smem_u32(sKV + (x % KV_ST) * TILE), SUB, 1024);
-                            if (few) {
-                                const uint64_t pt = ptx::sw128_kmajor_desc(ptx::smem_u32(sQ + TILE + s * 2 * FEW_SUB));
-                                if (!wait(&c.p_full[s], steps[s] & 1)) break;
+                for (int n = 0; ok && n < count + 2; ++n) {
+                    const int s = n & 1;
+                    const uint32_t tS = tmem + 256 * s;
+                    if (n >= 2 && n - 2 < count) {
+                        const int x = ring + 2 * (wide ? (n - 2) >> 1 : n - 2) + 1, st = x % KV_ST;
+                        if (!wait_ring(x)) break;
+                        // O may be overwritten once the item before has been read out
+                        if (n == 2 && k > 0 && !wait(&c.o_free, (k - 1) & 1)) break;
+                        const uint32_t keep = n - 2 >= 2 ? 1u : 0u;  // the slot's first product overwrites O
+                        const uint32_t v = bKV + st * (TILE >> 4);
+                        if (few) {
+                            const uint32_t pt = bQ + ((TILE + s * 2 * FEW_SUB) >> 4);
+                            if (!wait(&c.p_full[s], steps[s] & 1)) break;
+                            if (ptx::elect_one()) {
 #pragma unroll
                                 for (int kk = 0; kk < 8; ++kk)
-                                    ptx::mma_bf16(tS + 128, v + kk * (2048 >> 4),
-                                                  pt + (((kk >> 2) * FEW_SUB + (kk & 3) * 32) >> 4), idesc_o,
+                                    ptx::mma_bf16(tS + 128, mnmajor(v + kk * (2048 >> 4)),
+                                                  kmajor(pt + (((kk >> 2) * FEW_SUB + (kk & 3) * 32) >> 4)), idesc_o,
                                                   kk > 0 ? 1u : keep);
-                            } else {
-                                if (!wait(&c.p_part[s], parts[s] & 1)) break;
-                                ++parts[s];
+                            }
+                        } else {
+                            if (!wait(&c.p_part[s], parts[s] & 1)) break;
+                            ++parts[s];
+                            if (ptx::elect_one()) {
 #pragma unroll
                                 for (int kk = 0; kk < 6; ++kk)
-                                    ptx::mma_bf16_ts(tS + 128, tS + kk * 8, v + kk * (2048 >> 4), idesc_pv,
+                                    ptx::mma_bf16_ts(tS + 128, tS + kk * 8, mnmajor(v + kk * (2048 >> 4)), idesc_pv,
                                                      kk > 0 ? 1u : keep);
-                                if (!wait(&c.p_full[s], steps[s] & 1)) break;
+                            }
+                            if (!wait(&c.p_full[s], steps[s] & 1)) break;
+                            if (ptx::elect_one()) {
 #pragma unroll
                                 for (int kk = 6; kk < 8; ++kk)
-                                    ptx::mma_bf16_ts(tS + 128, tS + kk * 8, v + kk * (2048 >> 4), idesc_pv, 1u);
+                                    ptx::mma_bf16_ts(tS + 128, tS + kk * 8, mnmajor(v + kk * (2048 >> 4)), idesc_pv, 1u);
                             }
-                            ++steps[s];
-                            if (!wide || s == 1) ptx::mma_commit(&c.kv_empty[x % KV_ST]);
+                        }
+                        ++steps[s];
+                        if (ptx::elect_one()) {
+                            if (!wide || s == 1) ptx::mma_commit(&c.kv_empty[st]);
                             if (n >= count) ptx::mma_commit(&c.o_done[s]);
                         }
-                        if (n < count) {
-                            const int x = ring + 2 * (wide ? n >> 1 : n);
-                            if (!wait_ring(x)) break;
-                            const uint64_t kt = ptx::sw128_kmajor_desc(ptx::smem_u32(sKV + (x % KV_ST) * TILE));
-                            const uint64_t q = ptx::sw128_kmajor_desc(
-                                ptx::smem_u32(sQ + (few ? (k & 1) * 2 * FEW_SUB : (wide ? s : 0) * TILE)));
-                            const uint64_t x0 = few ? kt : q, y0 = few ? q : kt;  // the operand of 128 rows, and the other
-                            const uint32_t half = (few ? FEW_SUB : SUB) >> 4, xhalf = SUB >> 4;
+                    }
+                    if (n < count) {
+                        const int x = ring + 2 * (wide ? n >> 1 : n), st = x % KV_ST;
+                        if (!wait_ring(x)) break;
+                        const uint32_t kt = bKV + st * (TILE >> 4);
+                        const uint32_t q = bQ + (few ? (k & 1) * (2 * FEW_SUB >> 4) : (wide ? s : 0) * (TILE >> 4));
+                        if (few) {
+                            if (ptx::elect_one()) {
+#pragma unroll
+                                for (int kk = 0; kk < 8; ++kk)
+                                    ptx::mma_bf16(tS, kmajor(kt + (((kk >> 2) * SUB + (kk & 3) * 32) >> 4)),
+                                                  kmajor(q + (((kk >> 2) * FEW_SUB + (kk & 3) * 32) >> 4)), idesc_s,
+                                                  kk > 0 ? 1u : 0u);
+                            }
+                        } else if (ptx::elect_one()) {
 #pragma unroll
                             for (int kk = 0; kk < 8; ++kk)
-                                ptx::mma_bf16(tS, x0 + (kk >> 2) * xhalf + (kk & 3) * 2,
-                                              y0 + (kk >> 2) * half + (kk & 3) * 2, idesc_s, kk > 0 ? 1u : 0u);
+                                ptx::mma_bf16(tS, kmajor(q + (((kk >> 2) * SUB + (kk & 3) * 32) >> 4)),
+                                              kmajor(kt + (((kk >> 2) * SUB + (kk & 3) * 32) >> 4)), idesc_qk,
+                                              kk > 0 ? 1u : 0u);
+                        }
+                        if (ptx::elect_one()) {
                             ptx::mma_commit(&c.s_full[s]);
-                            if (!wide || s == 1) ptx::mma_commit(&c.kv_empty[x % KV_ST]);
+                            if (!wide || s == 1) ptx::mma_commit(&c.kv_empty[st]);
                             if (n == count - 1 && !few) ptx::mma_commit(&c.q_empty[k & 1]);
                         }
                     }
-                    if (few) ptx::mma_commit(&c.q_empty[k & 1]);  // P lies beside q
-                    ring += 2 * nt;
                 }
-                // No MMA may still be writing TMEM when it is freed (this matters on the error path).
-                ptx::mma_commit(&c.fin);
-                wait_bar(&c.fin, 0, err, kErrWaitIssuer);
+                if (few && ptx::elect_one()) ptx::mma_commit(&c.q_empty[k & 1]);  // P lies beside q
+                ring += 2 * nt;
             }
+            // No MMA may still be writing TMEM when it is freed (this matters on the error path).
+            if (ptx::elect_one()) ptx::mma_commit(&c.fin);
+            wait_bar(&c.fin, 0, err, kErrWaitIssuer);
         }
     } else {
         // ---- softmax ----
