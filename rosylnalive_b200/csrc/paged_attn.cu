@@ -12,8 +12,8 @@
 //   narrow  (up to 128 rows): one set of rows; the even key tiles go to slot 0 and the odd ones to slot 1, so one
 //           slot's products run under the other's softmax; the two states merge at the end.
 // Warps of a CTA:
-//   0, 3    TMA producers, half of the dims each: q of an item, then K_0, V_0, K_1, V_1, ... through a ring of five 32 KiB
-//           stages (8 pages of 16 tokens, one box a page and 64 dims), running ahead into the next item;
+//   0, 3    TMA producers: q of an item and K's tiles, and V's tiles, in the order of their use through a ring of five
+//           32 KiB stages (5 or 8 pages of 16 tokens, one box a page and 64 dims), running ahead into the next item;
 //   1       tensor-core issuer (one thread);
 //   2       scheduler: walks the CTA's range and hands the items to the others through a ring of four;
 //   4..11   softmax, one warpgroup a slot, thread = row.
@@ -40,17 +40,18 @@
 namespace lrm {
 namespace {
 
-constexpr int TK = sched::kTileKeys, KV_ST = 5, SLOTS = 2, ITEMS = 4;
+constexpr int TK = sched::kTileKeys, TKF = sched::kFewTileKeys, KV_ST = 5, SLOTS = 2, ITEMS = 4;
+constexpr int P_COL = 80;  // P's columns in tensor memory, behind S's (two bf16 a column): 80 + 40 of the slot's first 128
 constexpr int SUB = 128 * 64 * 2;  // one [128 rows][64] bf16 swizzled sub-tile
 constexpr int TILE = 2 * SUB;      // [128 rows][128]
-constexpr int P_SPLIT = 48;        // P is announced in two parts: keys 0..95 (48 packed columns), then 96..127
+static_assert(TK + TK / 2 <= 128 && TK % kPageTokens == 0 && TK % 16 == 0, "S and P of a tile lie side by side");
 constexpr int kThreads = 384;
 constexpr int kRegsLaunch = 168;  // 65536 / 384, rounded down to the allocation unit of 8
 constexpr int kRegsControl = 72, kRegsSoftmax = 216;
 static_assert(128 * kRegsControl + 256 * kRegsSoftmax <= kThreads * kRegsLaunch, "register split exceeds the launch");
 constexpr float kRescaleThreshold = 8.0f;  // log2 units: the reference maximum moves only when a tile exceeds it by more
-constexpr int kLeastUnits = 4;
-constexpr int kFewRows = 32;    // items of up to this many rows run with keys and rows swapped
+constexpr int kLeastUnits = 12;
+constexpr int kFewRows = sched::kFewRows;  // items of up to this many rows run with keys and rows swapped
 constexpr int FEW_SUB = kFewRows * 128;  // half of the dims (q) or keys (P) of up to 32 rows
 constexpr uint32_t kErrWaitProducer = 0x4010, kErrWaitIssuer = 0x4011, kErrWaitSoftmax = 0x4012, kErrWaitScheduler = 0x4013;
 
@@ -69,6 +70,15 @@ struct Record {
     int tok0, ntok, kvh, follow;
 };
 
+// The ring order of an item's tiles is the order in which the issuer first uses them. Step m of an item issues product m's
+// S = Q K^T and then O += P V of product m - lag. Wide: products 2t and 2t + 1 are tile t's two slots, and lag is 3; else
+// product t is tile t, in slot t & 1, and lag is 2. So K_t comes before V_{t - lead + 1}, lead being 2 or 3.
+__device__ __forceinline__ int products_lag(bool wide) { return wide ? 3 : 2; }
+__device__ __forceinline__ int ring_of_v(int t, int nt, bool wide) { return min(nt, t + (wide ? 2 : 3)) + t; }
+
+// A value that is the same in all lanes, so that the compiler knows it is.
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+
 // A request's tokens and keys when it is sound and has any, else n = 0.
 struct Request {
     int start, n, kv, slot;
@@ -76,8 +86,9 @@ struct Request {
 struct Control {
     uint64_t q_full[2], q_empty[2], fin, o_free;  // q: even and odd items
     uint64_t kv_full[KV_ST], kv_empty[KV_ST];
-    uint64_t s_full[SLOTS], p_part[SLOTS], p_full[SLOTS], o_done[SLOTS];
+    uint64_t s_full[SLOTS], s_free[SLOTS], p_full[SLOTS], o_done[SLOTS];  // a phase each product of the slot
     uint64_t item_full[ITEMS], item_empty[ITEMS];
+    int z[2][32], z_pad[8];  // the producers': z coordinates of a window of pages
     Item items[ITEMS];
     uint64_t warp_sum[kThreads / 32];
     uint64_t start_off, start_head;  // the range's last unit within its request, and that request's units a head
@@ -123,15 +134,40 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-// ptx::mbar_wait with its loop kept small: the kernel has some thirty waits, and its warps' loops together have to fit
-// the SM's instruction cache (unrolled waits alone were 60 KB of code, and every role then stalled on fetches).
+// ptx::mbar_wait with the first poll (which by itself waits some time) on the straight path and the loop behind it out of
+// the way. Three roles' code shares an SM sub-partition's instruction buffers, so code that is not straight costs some 5
+// cycles an instruction in fetches: with the polls unrolled (60 KB of code for thirty waits) every role stalled on them.
 constexpr uint32_t kPolls = 1u << 20;  // a second or so; waits are microseconds
-__device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, uint32_t *err, uint32_t code) {
+__device__ __forceinline__ bool try_wait(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, uint32_t *err, uint32_t code) {
+    if (__builtin_expect(try_wait(bar, parity), 1)) return true;
 #pragma unroll 1
     for (uint32_t i = 0; i < kPolls; ++i)
-        if (ptx::mbar_try_wait(bar, parity)) return true;
+        if (try_wait(bar, parity)) return true;
     atomicCAS(err, 0u, code);
     return false;
+}
+__device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, uint32_t *err, uint32_t code) {
+    return wait_bar(ptx::smem_u32(bar), parity, err, code);
+}
+
+// tma_load_3d of a page's 64 dims from `x` on, with shared addresses as they are.
+__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], "
+        "[%2];" ::"r"(dst),
+        "l"((uint64_t)map), "r"(bar), "r"(x), "r"(0), "r"(z)
+        : "memory");
 }
 
 __device__ __forceinline__ bool finite_bf16(uint32_t h) { return (h & 0x7F80u) != 0x7F80u; }
@@ -187,7 +223,7 @@ __device__ __forceinline__ void clean_v(uint8_t *tile, int key, int lane, int la
 
 // Adds the values that clean_v zeroed to one slot's O (128 columns at `t`, this warp's lanes), from the cache: this
 // lane's row sees keys lo .. hi, of which the slot has those of tiles tile0, tile0 + step, ... Rare, so it is kept out of the kernel's instruction stream.
-__device__ __noinline__ void add_poison(const PagedAttnArgs &a, int64_t table, int kvh, int lo, int hi, int tile0, int step,
+__device__ __noinline__ void add_poison(const PagedAttnArgs &a, int64_t table, int kvh, int lo, int hi, int tk, int tile0, int step,
                                         uint32_t t) {
 #pragma unroll 1
     for (int c = 0; c < kHeadDim; c += 16) {
@@ -196,7 +232,7 @@ __device__ __noinline__ void add_poison(const PagedAttnArgs &a, int64_t table, i
         ptx::tmem_ld_wait();
 #pragma unroll 1
         for (int key = lo; key <= hi; ++key) {
-            if ((key / TK - tile0) % step != 0) continue;  // the other slot's tile
+            if ((key / tk - tile0) % step != 0) continue;  // the other slot's tile
             const int pg = a.page_table[table + key / kPageTokens];
             if (pg < 0 || pg >= a.kv_pages) continue;
             const __nv_bfloat16 *v = a.pool + (size_t)pg * kv_page_elems(a.kv_heads) +
@@ -282,12 +318,12 @@ __device__ __forceinline__ void tmem_st8(uint32_t t, const float (&x)[8]) {
 
 // The sum of the values that clean_v zeroed in dim d of keys lo .. hi in tiles tile0, tile0 + step, ... (infinite or NaN, or
 // 0 if there are none).
-__device__ __noinline__ float poison_sum(const PagedAttnArgs &a, int64_t table, int kvh, int lo, int hi, int tile0, int step,
+__device__ __noinline__ float poison_sum(const PagedAttnArgs &a, int64_t table, int kvh, int lo, int hi, int tk, int tile0, int step,
                                          int d) {
     float sum = 0.f;
 #pragma unroll 1
     for (int key = lo; key <= hi; ++key) {
-        if ((key / TK - tile0) % step != 0) continue;  // the other slot's tile
+        if ((key / tk - tile0) % step != 0) continue;  // the other slot's tile
         const int pg = a.page_table[table + key / kPageTokens];
         if (pg < 0 || pg >= a.kv_pages) continue;
         const float x = __bfloat162float(a.pool[(size_t)pg * kv_page_elems(a.kv_heads) +
@@ -314,7 +350,7 @@ __device__ __forceinline__ void load_scores(uint32_t t, int from, float (&x)[8])
 // An item's tiles in one slot and its epilogue, eight rows at a time in rolled loops (code that the instruction cache
 // holds). Columns of the slot's tensor memory: S^T at 0, O^T at 128, the thread's sums of p at 192 (not beside S^T, which the
 // next item's first scores may overwrite while this item is still read out).
-__device__ __forceinline__ bool few_item(const RoleState &r, const Item &it, uint32_t &steps, uint32_t (&done)[SLOTS]) {
+__device__ __forceinline__ bool few_item(const RoleState &r, const Item &it, uint32_t &steps, uint32_t (&done)[SLOTS]) {  // done: products of the items before, a slot
     Control &c = *r.c;
     const PagedAttnArgs &a = r.p->a;
     const int s = r.s, lane = r.lane, group = r.p->group, nt = it.ke - it.kb, rows = it.ntok * group;
@@ -327,8 +363,8 @@ __device__ __forceinline__ bool few_item(const RoleState &r, const Item &it, uin
     for (int j = s; j < nt; j += 2, ++steps) {
         if (!wait_bar(&c.s_full[s], steps & 1, a.err, kErrWaitSoftmax)) return false;
         ptx::tc_fence_after();
-        const int key0 = (it.kb + j) * TK;
-        const bool first = j == s, dirty = key0 + TK - 1 > it.pos0;  // dirty: some row does not see the whole tile
+        const int key0 = (it.kb + j) * TKF;
+        const bool first = j == s, dirty = key0 + TKF - 1 > it.pos0;  // dirty: some row does not see the whole tile
         // rows are token-major, so the key is seen from this row on
         const int from = dirty ? min(max(key0 + key - it.pos0, 0), 64) * group : 0;
         bool over = first;
@@ -365,7 +401,10 @@ __device__ __forceinline__ bool few_item(const RoleState &r, const Item &it, uin
                 }
             }
             ptx::named_barrier(6 + s, 128);
-            if (!first) {  // this S was issued behind the slot's last product, so O is quiescent
+            if (!first) {
+                // O is quiescent once the slot's product before has been added
+                if (!wait_bar(&c.o_done[s], (steps - 1) & 1, a.err, kErrWaitSoftmax)) return false;
+                ptx::tc_fence_after();
 #pragma unroll 1
                 for (int g = 0; g < rows; g += 8) {
                     float o[8], l[8], alpha[8];
@@ -384,6 +423,8 @@ __device__ __forceinline__ bool few_item(const RoleState &r, const Item &it, uin
                 ptx::tmem_st_wait();
             }
         }
+        // P's place is free once the slot's product before has read it
+        if (steps > 0 && !wait_bar(&c.o_done[s], (steps - 1) & 1, a.err, kErrWaitSoftmax)) return false;
 #pragma unroll 1
         for (int g = 0; g < rows; g += 8) {
             float x[8], l[8], neg[8];
@@ -405,8 +446,11 @@ __device__ __forceinline__ bool few_item(const RoleState &r, const Item &it, uin
                              "h"((uint16_t)(w[e / 2] >> (e & 1 ? 16 : 0))));
             tmem_st8(tL + g, l);
         }
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&c.s_free[s]);
         if (dirty) {
-            const int xv = r.ring + 2 * j + 1;
+            const int xv = r.ring + ring_of_v(j, nt, false);
             if (!wait_bar(&c.kv_full[xv % KV_ST], (xv / KV_ST) & 1, a.err, kErrWaitSoftmax)) return false;
             clean_v(r.kv + (xv % KV_ST) * TILE, key, lane, it.pos0 + it.ntok - 1 - key0, &c.poison[s][r.k & 1], r.k + 1);
         } else {
@@ -419,8 +463,11 @@ __device__ __forceinline__ bool few_item(const RoleState &r, const Item &it, uin
     }
 
     const bool two = nt > 1;  // the second slot has a state
-    bool ok = wait_bar(&c.o_done[0], done[0]++ & 1, a.err, kErrWaitSoftmax);
-    if (ok && two) ok = wait_bar(&c.o_done[1], done[1]++ & 1, a.err, kErrWaitSoftmax);
+    done[0] += (nt + 1) / 2;
+    done[1] += nt / 2;
+    // this slot's last product first: the other's barrier is then at its own last one's phase
+    bool ok = nt <= s || wait_bar(&c.o_done[s], (done[s] - 1) & 1, a.err, kErrWaitSoftmax);
+    if (ok && nt > 1 - s) ok = wait_bar(&c.o_done[1 - s], (done[1 - s] - 1) & 1, a.err, kErrWaitSoftmax);
     if (!ok) return false;
     ptx::tc_fence_after();
     if (c.poison[0][r.k & 1] == r.k + 1 || c.poison[1][r.k & 1] == r.k + 1) {
@@ -431,8 +478,8 @@ __device__ __forceinline__ bool few_item(const RoleState &r, const Item &it, uin
                 asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(o) : "r"(tO + e));
                 ptx::tmem_ld_wait();
                 o = __float_as_uint(__uint_as_float(o) +
-                                    poison_sum(a, it.table, it.kvh, max(it.kb * TK, it.pos0 / TK * TK),
-                                               min(it.pos0 + e / group, it.ke * TK - 1), it.kb + s, 2, key));
+                                    poison_sum(a, it.table, it.kvh, max(it.kb * TKF, it.pos0 / TKF * TKF),
+                                               min(it.pos0 + e / group, it.ke * TKF - 1), TKF, it.kb + s, 2, key));
                 asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(tO + e), "r"(o) : "memory");
             }
         ptx::tmem_st_wait();
@@ -529,6 +576,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // (the shuffle tells the compiler that the warp index, and so the role, is the same in all lanes)
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid / 32, 0), lane = tid % 32;
     const int cta = blockIdx.x, span = SLOTS * p.tt;
+    const sched::Shape shape = {p.group, span};
     if (ptx::smem_u32(smem) & 1023) {  // the swizzled tiles and their descriptors need 1024-byte alignment
         if (tid == 0) {
             atomicCAS(err, 0u, kErrWaitScheduler);
@@ -539,19 +587,19 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if (warp == 2) {
         if (lane == 0) {
-            ptx::mbar_init(&c.q_full[0], 2);  // the two producer warps
-            ptx::mbar_init(&c.q_full[1], 2);
+            ptx::mbar_init(&c.q_full[0], 1);
+            ptx::mbar_init(&c.q_full[1], 1);
             ptx::mbar_init(&c.q_empty[0], 1);
             ptx::mbar_init(&c.q_empty[1], 1);
             ptx::mbar_init(&c.fin, 1);
             ptx::mbar_init(&c.o_free, 8);
             for (int s = 0; s < KV_ST; ++s) {
-                ptx::mbar_init(&c.kv_full[s], 2);
+                ptx::mbar_init(&c.kv_full[s], 1);
                 ptx::mbar_init(&c.kv_empty[s], 1);
             }
             for (int s = 0; s < SLOTS; ++s) {
                 ptx::mbar_init(&c.s_full[s], 1);
-                ptx::mbar_init(&c.p_part[s], 4);
+                ptx::mbar_init(&c.s_free[s], 4);
                 ptx::mbar_init(&c.p_full[s], 4);
                 ptx::mbar_init(&c.o_done[s], 1);
                 c.poison[s][0] = c.poison[s][1] = 0;
@@ -579,7 +627,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
     for (int r = r0; r < r1; ++r) {
         const Request q = load_request(a, r, cta == 0);
-        if (q.n) own += sched::head_units(q.n, q.kv, span) * (uint64_t)a.kv_heads;
+        if (q.n) own += sched::head_units(shape, q.n, q.kv) * (uint64_t)a.kv_heads;
     }
     uint64_t incl = own;
 #pragma unroll
@@ -607,11 +655,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int r = r0; r < r1; ++r) {
             const Request q = load_request(a, r, false);
             if (!q.n) continue;
-            const uint64_t w = sched::head_units(q.n, q.kv, span) * (uint64_t)a.kv_heads;
+            const uint64_t w = sched::head_units(shape, q.n, q.kv) * (uint64_t)a.kv_heads;
             if (u1 - 1 < at + w) {
                 c.start_req = r;
                 c.start_off = u1 - 1 - at;
-                c.start_head = sched::head_units(q.n, q.kv, span);
+                c.start_head = sched::head_units(shape, q.n, q.kv);
                 c.start = q;
                 break;
             }
@@ -632,11 +680,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 uint64_t left = u1 - u0;
                 int h = (int)sched::quotient(c.start_off, c.start_head);
                 const uint64_t off = c.start_off - (uint64_t)h * c.start_head;
-                int i = sched::item_at(q.n, q.kv, span, off);
-                int tiles = sched::item_tiles(q.n, q.kv, span, i);
-                sched::Cost cost = sched::item_cost(q.n, span, i);
+                int i = sched::item_at(shape, q.n, q.kv, off);
+                int tiles = sched::item_tiles(shape, q.n, q.kv, i);
+                sched::Cost cost = sched::item_cost(shape, q.n, i);
                 // the share's end within the item, in units
-                int end = (int)(off - sched::units_before(q.n, q.kv, span, i)) + 1;
+                int end = (int)(off - sched::units_before(shape, q.n, q.kv, i)) + 1;
                 Record rec = {0, 0, 0, 0};
                 int k = 0;
                 for (;;) {
@@ -680,196 +728,269 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                         i = sched::items_of(q.n, span) - 1;
                     }
-                    tiles = sched::item_tiles(q.n, q.kv, span, i);
-                    cost = sched::item_cost(q.n, span, i);
+                    tiles = sched::item_tiles(shape, q.n, q.kv, i);
+                    cost = sched::item_cost(shape, q.n, i);
                     end = cost.own + cost.tile * tiles;
                 }
                 p.records[cta] = rec;
             }
         } else if (warp == 0 || warp == 3) {
-            // ---- TMA producers: warp 0 the first 64 dims of every tile, warp 3 the others ----
-            const int half = warp == 3;
+            // ---- TMA producers: warp 0 q and the tiles of K, warp 3 those of V ----
+            // A stage's barrier counts phases of both; the ring's order is also the order in which the tiles are released,
+            // and a producer's next tile is at most 5 items on, so its wait cannot be a phase behind.
+            const int kv = warp == 3;
             const int oob = a.kv_pages * a.kv_heads * 2;  // past the tensor map: read as zeros, without a memory access
-            int ring = 0;    // ring items issued so far
-            int q_free = 0;  // items known to be through with q
-            bool ok = true, few_before = false;
-            for (int k = 0; ok; ++k) {
-                if (lane == 0) ok = wait_bar(&c.item_full[k % ITEMS], (k / ITEMS) & 1, err, kErrWaitProducer);
-                ok = __shfl_sync(0xffffffffu, ok, 0);
-                if (!ok) break;
-                const Item it = c.items[k % ITEMS];
+            int ring = 0, q_free = 0;  // ring items of the items before this one; items known to be through with q
+            bool few_before = false;
+            for (int k = 0;; ++k) {
+                bool ok = wait_bar(&c.item_full[k % ITEMS], (k / ITEMS) & 1, err, kErrWaitProducer);
+                if (__any_sync(0xffffffffu, !ok)) break;
+                const Item &item = c.items[k % ITEMS];
+                const int tok0 = uniform(item.tok0), ntok = uniform(item.ntok), kvh = uniform(item.kvh);
+                const int kb = uniform(item.kb), nt = uniform(item.ke) - kb, npages = uniform(item.npages);
+                const int32_t *pages = a.page_table + item.table;
                 __syncwarp();
                 if (lane == 0) ptx::mbar_arrive(&c.item_empty[k % ITEMS]);
-                if (it.ntok == 0) break;
-                // z coordinates (K block of page and head) of 4 tiles' pages, one a lane; the next 4 tiles' are fetched
-                // while these are issued
-                auto fetch = [&](int tile) {
-                    const int pg = tile * 8 + lane;
-                    if (pg >= it.npages) return oob;  // keys past the request, which no row sees
-                    const int id = a.page_table[it.table + pg];
-                    if ((uint32_t)id < (uint32_t)a.kv_pages) return (id * a.kv_heads + it.kvh) * 2;
+                if (ntok == 0) break;
+                const bool few = ntok * p.group <= kFewRows, wide = ntok > p.tt;
+                const int tile_pages = few ? TKF / kPageTokens : TK / kPageTokens, window = 32 / tile_pages;
+                // The z coordinates (K or V block of page and head) of a window of tiles, one a lane.
+                auto fetch = [&](int t) {
+                    const int pg = (kb + t) * tile_pages + lane;
+                    if (pg >= npages) return oob;  // keys past the request, which no row sees
+                    const int id = pages[pg];
+                    if ((uint32_t)id < (uint32_t)a.kv_pages) return (id * a.kv_heads + kvh) * 2 + kv;
                     atomicCAS(err, 0u, kErrAttnPage);
                     return oob;
                 };
-                int z = fetch(it.kb), z_next = it.kb + 4 < it.ke ? fetch(it.kb + 4) : oob;
-                const bool few = it.ntok * p.group <= kFewRows;
-                if (lane == 0) {
+                int z = fetch(0);
+                if (!kv) {
                     // Two few-row items in a row use different places for q, so the second one's q is loaded while the
                     // first still runs; otherwise q's place is free once the item before is through. Even and odd items
                     // have a barrier each: one that is waited for late, behind two items, would have lost its phase.
                     for (const int need = few && few_before ? k - 1 : k; ok && q_free < need; ++q_free)
                         ok = wait_bar(&c.q_empty[q_free & 1], (q_free >> 1) & 1, err, kErrWaitProducer);
-                    if (ok) {
-                        const int slots = it.ntok > p.tt ? 2 : 1, rows = (few ? p.few_tok : p.tt) * p.group;
-                        uint64_t *bar = &c.q_full[k & 1];
-                        uint8_t *dst = few ? sQ + (k & 1) * 2 * FEW_SUB + half * FEW_SUB : sQ + half * SUB;
-                        ptx::mbar_arrive_expect_tx(bar, slots * rows * 128);
-                        for (int s = 0; s < slots; ++s)
-                            ptx::tma_load_3d(dst + s * TILE, few ? &tq_few : &tq, bar, 64 * half, it.kvh * p.group,
-                                             it.tok0 + s * p.tt);
-                    }
-                }
-                few_before = few;
-                ok = __shfl_sync(0xffffffffu, ok, 0);
-                for (int t = it.kb; ok && t < it.ke; ++t) {
-                    const int sub = (t - it.kb) & 3;
-                    if (sub == 0 && t != it.kb) {
-                        z = z_next;
-                        z_next = t + 4 < it.ke ? fetch(t + 4) : oob;
-                    }
-                    int zp[8];
-#pragma unroll
-                    for (int u = 0; u < 8; ++u) zp[u] = __shfl_sync(0xffffffffu, z, sub * 8 + u);
+                    if (__any_sync(0xffffffffu, !ok)) break;
+                    few_before = few;
                     if (ptx::elect_one()) {
+                        uint64_t *bar = &c.q_full[k & 1];
+                        if (few) {
+                            uint8_t *dst = sQ + (k & 1) * 2 * FEW_SUB;
+                            ptx::mbar_arrive_expect_tx(bar, p.few_tok * p.group * 256);
+                            ptx::tma_load_3d(dst, &tq_few, bar, 0, kvh * p.group, tok0);
+                            ptx::tma_load_3d(dst + FEW_SUB, &tq_few, bar, 64, kvh * p.group, tok0);
+                        } else {
+                            ptx::mbar_arrive_expect_tx(bar, (wide ? 2 : 1) * p.tt * p.group * 256);
 #pragma unroll 1
-                        for (int kv = 0; ok && kv < 2; ++kv) {
-                            const int x = ring + kv, st = x % KV_ST;
-                            ok = wait_bar(&c.kv_empty[st], ((x / KV_ST) & 1) ^ 1, err, kErrWaitProducer);
-                            if (!ok) break;
-                            ptx::mbar_arrive_expect_tx(&c.kv_full[st], SUB);
-                            uint8_t *dst = sKV + st * TILE + half * SUB;
-#pragma unroll
-                            for (int u = 0; u < 8; ++u)
-                                ptx::tma_load_3d(dst + u * 2048, &tkv, &c.kv_full[st], 64 * half, 0, zp[u] + kv);
+                            for (int s = 0; s < (wide ? 2 : 1); ++s) {
+                                ptx::tma_load_3d(sQ + s * TILE, &tq, bar, 0, kvh * p.group, tok0 + s * p.tt);
+                                ptx::tma_load_3d(sQ + s * TILE + SUB, &tq, bar, 64, kvh * p.group, tok0 + s * p.tt);
+                            }
                         }
                     }
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (ok) ring += 2;
+                    __syncwarp();
                 }
+                const int lead = wide ? 2 : 3;
+#pragma unroll 1
+                for (int t0 = 0; t0 < nt; t0 += window) {
+                    c.z[kv][lane] = z;
+                    __syncwarp();
+                    z = t0 + window < nt ? fetch(t0 + window) : oob;
+                    // One lane issues a window's copies (the choice of it and the return from it cost some 170 cycles).
+                    if (ptx::elect_one()) {
+                        const int t1 = min(nt, t0 + window);
+                        const int *zt = c.z[kv];
+#pragma unroll 1
+                        for (int t = t0; t < t1; ++t, zt += tile_pages) {
+                            const int x = ring + t + (kv ? min(nt, t + lead) : max(0, t - lead + 1)), st = x % KV_ST;
+                            const uint32_t bar = ptx::smem_u32(&c.kv_full[st]), dst = ptx::smem_u32(sKV) + st * TILE;
+                            int zp[8];
+#pragma unroll
+                            for (int u = 0; u < 8; ++u) zp[u] = zt[u];  // (the array behind z is read past a window's end)
+                            ok = wait_bar(&c.kv_empty[st], ((x / KV_ST) & 1) ^ 1, err, kErrWaitProducer);
+                            if (!ok) break;
+                            ptx::mbar_arrive_expect_tx(&c.kv_full[st], tile_pages * 4096);
+#pragma unroll
+                            for (int u = 0; u < 5; ++u) {
+                                tma_3d(dst + u * 2048, &tkv, bar, 0, zp[u]);
+                                tma_3d(dst + SUB + u * 2048, &tkv, bar, 64, zp[u]);
+                            }
+                            if (few) {
+#pragma unroll
+                                for (int u = 5; u < 8; ++u) {
+                                    tma_3d(dst + u * 2048, &tkv, bar, 0, zp[u]);
+                                    tma_3d(dst + SUB + u * 2048, &tkv, bar, 64, zp[u]);
+                                }
+                            }
+                        }
+                        // on the error path, the copies in flight must land before the CTA exits
+                        for (int y = ok ? t1 : 0; y < t1; ++y) {
+                            const int x = ring + y + (kv ? min(nt, y + lead) : max(0, y - lead + 1));
+                            wait_bar(&c.kv_full[x % KV_ST], (x / KV_ST) & 1, err, kErrWaitProducer);
+                        }
+                    }
+                    __syncwarp();
+                    if (__any_sync(0xffffffffu, !ok)) break;
+                }
+                if (__any_sync(0xffffffffu, !ok)) break;
+                ring += 2 * nt;
             }
-            // Copies in flight must land before the CTA exits (this matters on the error path; a fill of which only
-            // one half was issued is waited for until the wait's limit).
-            for (int x = ring > KV_ST ? ring - KV_ST : 0; x < ring; ++x)
-                wait_bar(&c.kv_full[x % KV_ST], (x / KV_ST) & 1, err, kErrWaitProducer);
         } else if (warp == 1) {
             // ---- tensor-core issuer ----
-            // The whole warp runs this, with everything it goes by the same in all lanes, and one lane issues: so the
-            // descriptors are computed once a warp (in uniform registers), 5 instructions an MMA. (Inside one lane's
-            // branch an MMA took 110 cycles to issue, more than the 64 that it runs.)
-            constexpr uint32_t idesc_qk = ptx::idesc_bf16_f32(128, 128, false);
+            constexpr uint32_t idesc_qk = ptx::idesc_bf16_f32(128, TK, false);
             constexpr uint32_t idesc_pv = ptx::idesc_bf16_f32(128, 128, true);
             constexpr uint32_t kHi = 1u << 14 | 2u << 29;  // descriptor bits 32-63: version 1, 128-byte swizzle
             const uint32_t bQ = ptx::smem_u32(sQ) >> 4, bKV = ptx::smem_u32(sKV) >> 4;
-            int ring = 0;                // ring items of the items before this one
-            uint32_t steps[SLOTS] = {}, parts[SLOTS] = {};  // P tiles consumed so far, a slot; those in two parts
-            bool ok = true;
-            auto wait = [&](uint64_t *bar, uint32_t parity) {
-                ok = __all_sync(0xffffffffu, ok && wait_bar(bar, parity, err, kErrWaitIssuer));
-                ptx::tc_fence_after();
-                return ok;
-            };
-            auto wait_ring = [&](int x) { return wait(&c.kv_full[x % KV_ST], (x / KV_ST) & 1); };
             // K-major: rows of 128 bytes, 8-row groups 1024 apart; MN-major (V): 64-dim halves SUB apart, the same groups
             auto kmajor = [](uint32_t at) { return (uint64_t)(kHi | 1024 >> 4) << 32 | (1u << 16 | at); };
             auto mnmajor = [](uint32_t at) { return (uint64_t)(kHi | 1024 >> 4) << 32 | ((uint32_t)(SUB >> 4) << 16 | at); };
-            for (int k = 0; ok; ++k) {
-                if (!wait(&c.item_full[k % ITEMS], (k / ITEMS) & 1)) break;
-                const int ntok = __shfl_sync(0xffffffffu, c.items[k % ITEMS].ntok, 0);
-                const int nt = __shfl_sync(0xffffffffu, c.items[k % ITEMS].ke - c.items[k % ITEMS].kb, 0);
+            int ring = 0;                // ring items of the items before this one
+            uint32_t before0 = 0, before1 = 0;  // products of the items before, a slot
+            for (int k = 0;; ++k) {
+                bool ok = wait_bar(&c.item_full[k % ITEMS], (k / ITEMS) & 1, err, kErrWaitIssuer);
+                if (!__all_sync(0xffffffffu, ok)) break;
+                const int ntok = uniform(c.items[k % ITEMS].ntok);
+                const int nt = uniform(c.items[k % ITEMS].ke - c.items[k % ITEMS].kb);
+                __syncwarp();
                 if (lane == 0) ptx::mbar_arrive(&c.item_empty[k % ITEMS]);
                 if (ntok == 0) break;
                 const bool wide = ntok > p.tt, few = ntok * p.group <= kFewRows;
                 // few: S^T = K Q^T (128 keys x 16 or 32 rows) and O^T = V^T P^T (128 dims x rows)
                 const int nrow = ntok * p.group <= 16 ? 16 : 32;
-                const uint32_t idesc_s = few ? ptx::idesc_bf16_f32(128, nrow) : idesc_qk;
-                const uint32_t idesc_o = ptx::idesc_bf16_f32(128, nrow) | 1u << 15;  // A (V) MN-major
-                if (!wait(&c.q_full[k & 1], (k >> 1) & 1)) break;
-                // Products n = 0 .. count - 1: slot n & 1, key tile n / 2 (wide) or n (narrow, few). Step n issues
-                // O += P V of product n - 2, then S = Q K^T of product n in the same slot. The tensor core runs one
-                // thread's MMAs in order, so S overwrites P only after its product with V has read it.
-                const int count = wide ? 2 * nt : nt;
+                const uint32_t idesc_s = ptx::idesc_bf16_f32(128, nrow), idesc_o = idesc_s | 1u << 15;  // A (V) MN-major
+                // Product n's slot is n & 1. S lies beside P, so the next S of a slot is computed as soon as its softmax
+                // has taken this one, and waits there for it; only P V waits for P.
+                const int count = wide ? 2 * nt : nt, lag = products_lag(wide);
+                // One lane runs the item (choosing it and returning from it cost some 170 cycles); what the MMAs go by was
+                // made uniform above, so their descriptors stay in uniform registers.
+                if (ptx::elect_one()) {
+                    uint32_t st = ring % KV_ST, phase = (ring / KV_ST) & 1;  // the next ring item
+                    auto wait = [&](uint32_t bar, uint32_t parity) {
+                        ok = wait_bar(bar, parity, err, kErrWaitIssuer);
+                        ptx::tc_fence_after();
+                        return ok;
+                    };
+                    // The next tile of the ring: its stage, or -1.
+                    auto next_tile = [&]() {
+                        const int x = (int)st;
+                        const bool got = wait(ptx::smem_u32(&c.kv_full[0]) + 8 * st, phase);
+                        if (++st == KV_ST) {
+                            st = 0;
+                            phase ^= 1;
+                        }
+                        return got ? x : -1;
+                    };
+                    const uint32_t s_free = ptx::smem_u32(&c.s_free[0]), p_full = ptx::smem_u32(&c.p_full[0]);
+                    wait(ptx::smem_u32(&c.q_full[k & 1]), (k >> 1) & 1);
+                    if (wide) {
+                        // Both slots of tile t: S of 0, P V of 1 (two tiles back), S of 1, P V of 0 (the tile before).
+                        const uint32_t par0 = before0 & 1, par1 = before1 & 1;  // parity of the item's first product
+                        int kt = 0, vt = 0;  // stages of the last tiles of K and V
 #pragma unroll 1
-                for (int n = 0; ok && n < count + 2; ++n) {
-                    const int s = n & 1;
-                    const uint32_t tS = tmem + 256 * s;
-                    if (n >= 2 && n - 2 < count) {
-                        const int x = ring + 2 * (wide ? (n - 2) >> 1 : n - 2) + 1, st = x % KV_ST;
-                        if (!wait_ring(x)) break;
-                        // O may be overwritten once the item before has been read out
-                        if (n == 2 && k > 0 && !wait(&c.o_free, (k - 1) & 1)) break;
-                        const uint32_t keep = n - 2 >= 2 ? 1u : 0u;  // the slot's first product overwrites O
-                        const uint32_t v = bKV + st * (TILE >> 4);
-                        if (few) {
-                            const uint32_t pt = bQ + ((TILE + s * 2 * FEW_SUB) >> 4);
-                            if (!wait(&c.p_full[s], steps[s] & 1)) break;
-                            if (ptx::elect_one()) {
+                        for (int t = 0; ok && t < nt + 2; ++t) {
+                            if (t < nt) {
+                                if ((kt = next_tile()) < 0) break;
+                                if ((t > 0 || before0 > 0) && !wait(s_free, (par0 ^ t ^ 1) & 1)) break;
+                                const uint32_t key = bKV + kt * (TILE >> 4);
 #pragma unroll
                                 for (int kk = 0; kk < 8; ++kk)
-                                    ptx::mma_bf16(tS + 128, mnmajor(v + kk * (2048 >> 4)),
-                                                  kmajor(pt + (((kk >> 2) * FEW_SUB + (kk & 3) * 32) >> 4)), idesc_o,
-                                                  kk > 0 ? 1u : keep);
-                            }
-                        } else {
-                            if (!wait(&c.p_part[s], parts[s] & 1)) break;
-                            ++parts[s];
-                            if (ptx::elect_one()) {
-#pragma unroll
-                                for (int kk = 0; kk < 6; ++kk)
-                                    ptx::mma_bf16_ts(tS + 128, tS + kk * 8, mnmajor(v + kk * (2048 >> 4)), idesc_pv,
-                                                     kk > 0 ? 1u : keep);
-                            }
-                            if (!wait(&c.p_full[s], steps[s] & 1)) break;
-                            if (ptx::elect_one()) {
-#pragma unroll
-                                for (int kk = 6; kk < 8; ++kk)
-                                    ptx::mma_bf16_ts(tS + 128, tS + kk * 8, mnmajor(v + kk * (2048 >> 4)), idesc_pv, 1u);
-                            }
-                        }
-                        ++steps[s];
-                        if (ptx::elect_one()) {
-                            if (!wide || s == 1) ptx::mma_commit(&c.kv_empty[st]);
-                            if (n >= count) ptx::mma_commit(&c.o_done[s]);
-                        }
-                    }
-                    if (n < count) {
-                        const int x = ring + 2 * (wide ? n >> 1 : n), st = x % KV_ST;
-                        if (!wait_ring(x)) break;
-                        const uint32_t kt = bKV + st * (TILE >> 4);
-                        const uint32_t q = bQ + (few ? (k & 1) * (2 * FEW_SUB >> 4) : (wide ? s : 0) * (TILE >> 4));
-                        if (few) {
-                            if (ptx::elect_one()) {
-#pragma unroll
-                                for (int kk = 0; kk < 8; ++kk)
-                                    ptx::mma_bf16(tS, kmajor(kt + (((kk >> 2) * SUB + (kk & 3) * 32) >> 4)),
-                                                  kmajor(q + (((kk >> 2) * FEW_SUB + (kk & 3) * 32) >> 4)), idesc_s,
+                                    ptx::mma_bf16(tmem, kmajor(bQ + (((kk >> 2) * SUB + (kk & 3) * 32) >> 4)),
+                                                  kmajor(key + (((kk >> 2) * SUB + (kk & 3) * 32) >> 4)), idesc_qk,
                                                   kk > 0 ? 1u : 0u);
+                                ptx::mma_commit(&c.s_full[0]);
                             }
-                        } else if (ptx::elect_one()) {
+                            if (t >= 2) {
+                                if (!wait(p_full + 8, (par1 ^ t) & 1)) break;
+                                const uint32_t v = bKV + vt * (TILE >> 4), keep = t > 2 ? 1u : 0u;
 #pragma unroll
-                            for (int kk = 0; kk < 8; ++kk)
-                                ptx::mma_bf16(tS, kmajor(q + (((kk >> 2) * SUB + (kk & 3) * 32) >> 4)),
-                                              kmajor(kt + (((kk >> 2) * SUB + (kk & 3) * 32) >> 4)), idesc_qk,
-                                              kk > 0 ? 1u : 0u);
+                                for (int kk = 0; kk < TK / 16; ++kk)
+                                    ptx::mma_bf16_ts(tmem + 384, tmem + 256 + P_COL + kk * 8, mnmajor(v + kk * (2048 >> 4)),
+                                                     idesc_pv, kk > 0 ? 1u : keep);
+                                ptx::mma_commit(&c.o_done[1]);
+                                ptx::mma_commit(&c.kv_empty[vt]);
+                            }
+                            if (t < nt) {
+                                if ((t > 0 || before1 > 0) && !wait(s_free + 8, (par1 ^ t ^ 1) & 1)) break;
+                                const uint32_t key = bKV + kt * (TILE >> 4);
+#pragma unroll
+                                for (int kk = 0; kk < 8; ++kk)
+                                    ptx::mma_bf16(tmem + 256, kmajor(bQ + ((TILE + (kk >> 2) * SUB + (kk & 3) * 32) >> 4)),
+                                                  kmajor(key + (((kk >> 2) * SUB + (kk & 3) * 32) >> 4)), idesc_qk,
+                                                  kk > 0 ? 1u : 0u);
+                                ptx::mma_commit(&c.s_full[1]);
+                                ptx::mma_commit(&c.kv_empty[kt]);
+                                if (t == nt - 1) ptx::mma_commit(&c.q_empty[k & 1]);
+                            }
+                            if (t >= 1 && t <= nt) {
+                                if ((vt = next_tile()) < 0) break;
+                                // O may be overwritten once the item before has been read out
+                                if (t == 1 && k > 0 && !wait(ptx::smem_u32(&c.o_free), (k - 1) & 1)) break;
+                                if (!wait(p_full, (par0 ^ t ^ 1) & 1)) break;
+                                const uint32_t v = bKV + vt * (TILE >> 4), keep = t > 1 ? 1u : 0u;
+#pragma unroll
+                                for (int kk = 0; kk < TK / 16; ++kk)
+                                    ptx::mma_bf16_ts(tmem + 128, tmem + P_COL + kk * 8, mnmajor(v + kk * (2048 >> 4)), idesc_pv,
+                                                     kk > 0 ? 1u : keep);
+                                ptx::mma_commit(&c.o_done[0]);
+                            }
                         }
-                        if (ptx::elect_one()) {
-                            ptx::mma_commit(&c.s_full[s]);
-                            if (!wide || s == 1) ptx::mma_commit(&c.kv_empty[st]);
-                            if (n == count - 1 && !few) ptx::mma_commit(&c.q_empty[k & 1]);
+                    } else {
+                        int vt = 0, kt = 0;
+#pragma unroll 1
+                        for (int m = 0; ok && m < nt + 2; ++m) {
+                            const int s = m & 1;
+                            const uint32_t tS = tmem + 256 * s, prod = (s ? before1 : before0) + (m >> 1);
+                            if (m < nt) {
+                                if ((kt = next_tile()) < 0) break;
+                                if (prod > 0 && !wait(s_free + 8 * s, (prod - 1) & 1)) break;
+                                const uint32_t key = bKV + kt * (TILE >> 4);
+                                if (few) {
+                                    const uint32_t q = bQ + (k & 1) * (2 * FEW_SUB >> 4);
+#pragma unroll
+                                    for (int kk = 0; kk < 8; ++kk)
+                                        ptx::mma_bf16(tS, kmajor(key + (((kk >> 2) * SUB + (kk & 3) * 32) >> 4)),
+                                                      kmajor(q + (((kk >> 2) * FEW_SUB + (kk & 3) * 32) >> 4)), idesc_s,
+                                                      kk > 0 ? 1u : 0u);
+                                } else {
+#pragma unroll
+                                    for (int kk = 0; kk < 8; ++kk)
+                                        ptx::mma_bf16(tS, kmajor(bQ + (((kk >> 2) * SUB + (kk & 3) * 32) >> 4)),
+                                                      kmajor(key + (((kk >> 2) * SUB + (kk & 3) * 32) >> 4)), idesc_qk,
+                                                      kk > 0 ? 1u : 0u);
+                                }
+                                ptx::mma_commit(&c.s_full[s]);
+                                ptx::mma_commit(&c.kv_empty[kt]);
+                                if (m == nt - 1 && !few) ptx::mma_commit(&c.q_empty[k & 1]);
+                            }
+                            if (m >= 2) {
+                                if ((vt = next_tile()) < 0) break;
+                                if (m == 2 && k > 0 && !wait(ptx::smem_u32(&c.o_free), (k - 1) & 1)) break;
+                                if (!wait(p_full + 8 * s, (prod - 1) & 1)) break;
+                                const uint32_t v = bKV + vt * (TILE >> 4), keep = m >= 4 ? 1u : 0u;
+                                if (few) {
+                                    const uint32_t pt = bQ + ((TILE + s * 2 * FEW_SUB) >> 4);
+#pragma unroll
+                                    for (int kk = 0; kk < 8; ++kk)
+                                        ptx::mma_bf16(tS + 128, mnmajor(v + kk * (2048 >> 4)),
+                                                      kmajor(pt + (((kk >> 2) * FEW_SUB + (kk & 3) * 32) >> 4)), idesc_o,
+                                                      kk > 0 ? 1u : keep);
+                                } else {
+#pragma unroll
+                                    for (int kk = 0; kk < TK / 16; ++kk)
+                                        ptx::mma_bf16_ts(tS + 128, tS + P_COL + kk * 8, mnmajor(v + kk * (2048 >> 4)),
+                                                         idesc_pv, kk > 0 ? 1u : keep);
+                                }
+                                ptx::mma_commit(&c.o_done[s]);
+                                ptx::mma_commit(&c.kv_empty[vt]);
+                            }
                         }
+                        if (few) ptx::mma_commit(&c.q_empty[k & 1]);  // P lies beside q
                     }
                 }
-                if (few && ptx::elect_one()) ptx::mma_commit(&c.q_empty[k & 1]);  // P lies beside q
+                if (__any_sync(0xffffffffu, !ok)) break;
                 ring += 2 * nt;
+                before0 += (count + 1) / 2;
+                before1 += count / 2;
             }
             // No MMA may still be writing TMEM when it is freed (this matters on the error path).
             if (ptx::elect_one()) ptx::mma_commit(&c.fin);
@@ -893,8 +1014,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t tS = tmem + 256 * s + lanes;
         const float sc = a.scale_log2;
         int ring = 0;
-        uint32_t steps = 0, done[SLOTS] = {};  // S tiles taken from this slot; items that used each slot
-        bool ok = true;
+        uint32_t steps = 0, done[SLOTS] = {};  // products of this slot so far; products of the items before, a slot
+        bool ok = true, narrow_before = false;
         for (int k = 0; ok; ++k) {
             if (!wait_bar(&c.item_full[k % ITEMS], (k / ITEMS) & 1, err, kErrWaitSoftmax)) break;
             const Item it = c.items[k % ITEMS];
@@ -903,12 +1024,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (it.ntok == 0) break;
             if (it.ntok * p.group <= kFewRows) {
                 const RoleState r = {&c, &p, sKV, sQ + TILE + s * 2 * FEW_SUB, tmem, s, quarter, lane, cta, k, ring};
+                // the sums of p go where a narrow item's O is: both warpgroups have read that out behind this
+                if (narrow_before) ptx::named_barrier(1, 256);
+                narrow_before = false;
                 ok = few_item(r, it, steps, done);
                 ring += 2 * (it.ke - it.kb);
                 if (!ok) break;
                 continue;
             }
             const bool wide = it.ntok > p.tt;
+            narrow_before = !wide;
             const int token = wide ? s * p.tt + tl : tl;  // of the item
             const bool valid = tl < p.tt && token < it.ntok;
             const int warp_token = wide ? s * p.tt + warp_tl : warp_tl;
@@ -925,29 +1050,40 @@ __global__ void __launch_bounds__(kThreads, 1)
                 ptx::tc_fence_after();
                 const int key0 = (it.kb + j) * TK;
                 const bool dirty = key0 + TK - 1 > it.pos0;  // some row of the item does not see the whole tile
-                uint32_t pk[64];
+                float x[TK];
                 if (active) {
-                    float x[128];
                     ptx::tmem_ld32(tS, reinterpret_cast<uint32_t *>(x));
                     ptx::tmem_ld32(tS + 32, reinterpret_cast<uint32_t *>(x) + 32);
-                    ptx::tmem_ld32(tS + 64, reinterpret_cast<uint32_t *>(x) + 64);
-                    ptx::tmem_ld32(tS + 96, reinterpret_cast<uint32_t *>(x) + 96);
+                    ptx::tmem_ld16(tS + 64, *reinterpret_cast<uint32_t(*)[16]>(x + 64));
                     ptx::tmem_ld_wait();
+                }
+                ptx::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(&c.s_free[s]);
+                float tmax = -INFINITY;
+                if (active) {
                     if (key0 + TK - 1 > it.pos0 + warp_token) {
                         const int lim = it.pos0 + token - key0;  // keys 0..lim of the tile are visible
 #pragma unroll
-                        for (int e = 0; e < 128; ++e) x[e] = e <= lim ? x[e] : -INFINITY;
+                        for (int e = 0; e < TK; ++e) x[e] = e <= lim ? x[e] : -INFINITY;
                     }
                     float mx[8];
 #pragma unroll
                     for (int u = 0; u < 8; ++u) mx[u] = fmaxf(x[u], x[u + 8]);
 #pragma unroll
-                    for (int e = 16; e < 128; e += 16) {
+                    for (int e = 16; e < TK; e += 16) {
 #pragma unroll
                         for (int u = 0; u < 8; ++u) mx[u] = max3(mx[u], x[e + u], x[e + 8 + u]);
                     }
-                    const float tmax =
-                        fmaxf(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], max3(mx[5], mx[6], mx[7]))) * sc;
+                    tmax = fmaxf(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], max3(mx[5], mx[6], mx[7]))) * sc;
+                }
+                // The slot's product before has been added to O and has read P: both may be written.
+                if (steps > 0 && !wait_bar(&c.o_done[s], (steps - 1) & 1, err, kErrWaitSoftmax)) {
+                    ok = false;
+                    break;
+                }
+                ptx::tc_fence_after();
+                if (active) {
                     bool rescale = false;
                     float alpha = 1.f;
                     if (first) {
@@ -958,7 +1094,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                         rescale = true;
                     }
                     if (__any_sync(0xffffffffu, rescale)) {
-                        // this S was issued behind the slot's last product, so O is quiescent
                         l *= alpha;
 #pragma unroll 1
                         for (int col = 0; col < 128; col += 32) {
@@ -972,8 +1107,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     const float nm = m_ref == -INFINITY ? 0.f : -m_ref;  // a row that has seen no key yet: p = 0
                     float la = 0.f, lb = 0.f, lc = 0.f, ld = 0.f;
+                    uint32_t pk[TK / 2];
 #pragma unroll
-                    for (int e = 0; e < 64; ++e) {
+                    for (int e = 0; e < TK / 2; ++e) {
                         float u, v;
                         ptx::fma_x2(u, v, x[2 * e], x[2 * e + 1], sc, sc, nm, nm);
                         u = ptx::ex2(u);
@@ -985,26 +1121,20 @@ __global__ void __launch_bounds__(kThreads, 1)
                         pk[e] = pack2(u, v);
                     }
                     l += (la + lb) + (lc + ld);
-                    ptx::tmem_st32(tS, pk);
-                    ptx::tmem_st16(tS + 32, *reinterpret_cast<const uint32_t(*)[16]>(pk + 32));
+                    ptx::tmem_st32(tS + P_COL, pk);
+                    tmem_st8(tS + P_COL + 32, *reinterpret_cast<const float(*)[8]>(pk + 32));
                 }
                 first = false;
                 if (dirty) {
-                    const int xv = ring + 2 * j + 1;
+                    const int xv = ring + ring_of_v(j, nt, wide);
                     if (!wait_bar(&c.kv_full[xv % KV_ST], (xv / KV_ST) & 1, err, kErrWaitSoftmax)) {
                         ok = false;
                         break;
                     }
-                    clean_v(sKV + (xv % KV_ST) * TILE, rl, lane, it.pos0 + it.ntok - 1 - key0, &c.poison[s][k & 1], k + 1);
+                    if (rl < TK)
+                        clean_v(sKV + (xv % KV_ST) * TILE, rl, lane, it.pos0 + it.ntok - 1 - key0, &c.poison[s][k & 1], k + 1);
                 }
                 if (active) ptx::tmem_st_wait();
-                ptx::tc_fence_before();
-                __syncwarp();
-                if (lane == 0) ptx::mbar_arrive(&c.p_part[s]);
-                if (active) {
-                    ptx::tmem_st16(tS + P_SPLIT, *reinterpret_cast<const uint32_t(*)[16]>(pk + P_SPLIT));
-                    ptx::tmem_st_wait();
-                }
                 ptx::tc_fence_before();
                 __syncwarp();
                 if (lane == 0) ptx::mbar_arrive(&c.p_full[s]);
@@ -1014,18 +1144,16 @@ __global__ void __launch_bounds__(kThreads, 1)
 
             // ---- epilogue ----
             const bool used1 = wide || nt > 1;
+            done[0] += wide ? nt : (nt + 1) / 2;
+            done[1] += wide ? nt : nt / 2;
             auto wait_done = [&](int slot) {
-                if (!wait_bar(&c.o_done[slot], done[slot] & 1, err, kErrWaitSoftmax)) ok = false;
-                ++done[slot];
+                if (!wait_bar(&c.o_done[slot], (done[slot] - 1) & 1, err, kErrWaitSoftmax)) ok = false;
                 ptx::tc_fence_after();
                 return ok;
             };
-            if (wide && s == 1) {
-                if (!wait_done(0) || !wait_done(1)) break;
-            } else {
-                if (!wait_done(0)) break;
-                if (!wide && used1 && !wait_done(1)) break;
-            }
+            // this slot's last product first: the other's barrier is then at its own last one's phase
+            if ((s == 0 || used1) && !wait_done(s)) break;
+            if (!wide && (s == 1 || used1) && !wait_done(1 - s)) break;
             float w[SLOTS] = {1.f, 0.f};  // weights of the two slots' states (narrow)
             if (!wide) {
                 // both warpgroups hold the same rows: exchange the states, then each takes half of the dims
@@ -1049,7 +1177,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const int lo = max(it.kb * TK, it.pos0 / TK * TK);
                     const int hi = valid ? min(it.pos0 + token, it.ke * TK - 1) : -1;
                     if (wide || nt > s)
-                        add_poison(a, it.table, it.kvh, lo, hi, it.kb + (wide ? 0 : s), wide ? 1 : 2, tS + 128);
+                        add_poison(a, it.table, it.kvh, lo, hi, TK, it.kb + (wide ? 0 : s), wide ? 1 : 2, tS + 128);
                     if (!wide) {  // the other warpgroup's warp of these lanes reads this slot's O too
                         ptx::tc_fence_before();
                         ptx::named_barrier(2 + quarter, 64);
@@ -1114,7 +1242,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             ptx::tc_fence_before();
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(&c.o_free);
-            if (wide && s == 0 && !wait_done(1)) break;  // keeps in step with the slot's barrier
         }
     }
     ptx::tc_fence_before();

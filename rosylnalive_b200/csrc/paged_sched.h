@@ -2,12 +2,12 @@
 // be checked on the CPU).
 //
 // A request has n new tokens, the last of its kv keys, and `group` query heads a KV head. An item is up to `span`
-// consecutive tokens of one request and KV head, all their query heads, and reads as many tiles of 128 keys as its last
-// token sees. A wide item (more than half a span: both slots' rows) counts 2 units of work a tile and 3 for itself, a
-// narrow one 1 a tile and 2 for itself: about 2,500 cycles each, as measured. All units of a call, ordered by (request,
-// KV head, item, key), are cut into `ctas` ranges of equal length, one a CTA, so every mixture of lengths is balanced; an
-// item that a cut passes through is merged from its CTAs' partial results. (Counting tiles alone left 32 requests of 5
-// tokens over 100 to 6000 keys at 64 us against 43, and 8 chunks of 511 tokens among 56 decodes at 103 against 73.)
+// consecutive tokens of one request and KV head, all their query heads, and reads the keys that its last token sees in
+// tiles: of 128 keys when it has few rows (kFewRows), else of 80. An item counts units of work for its start and end and
+// for each tile, as measured (Cost). All units of a call, ordered by (request, KV head, item, key), are cut into `ctas`
+// ranges of equal length, one a CTA, so every mixture of lengths is balanced; an item that a cut passes through is merged
+// from its CTAs' partial results. (Counting tiles alone left 32 requests of 5 tokens over 100 to 6000 keys at 64 us
+// against 43, and 8 chunks of 511 tokens among 56 decodes at 103 against 87.)
 #pragma once
 
 #include <stdint.h>
@@ -23,8 +23,8 @@
 namespace lrm {
 namespace sched {
 
-constexpr int kTileKeys = 128;
 constexpr int kTileRows = 128;
+constexpr int kFewRows = 32, kFewTileKeys = 128, kTileKeys = 80;
 
 // sum over i in [0, n) of floor((a i + b) / m), by Euclid's steps on (a, m); a, b >= 0, m > 0.
 LRM_HD_FAR uint64_t floor_sum(uint64_t n, uint32_t m, uint32_t a, uint64_t b) {
@@ -46,44 +46,50 @@ LRM_HD_FAR uint64_t floor_sum(uint64_t n, uint32_t m, uint32_t a, uint64_t b) {
 
 LRM_HD int items_of(int n, int span) { return (n + span - 1) / span; }
 
+struct Shape {
+    int group, span;
+};
+LRM_HD int item_tokens(Shape s, int n, int i) { return n - i * s.span < s.span ? n - i * s.span : s.span; }
+LRM_HD int tile_keys(int rows) { return rows <= kFewRows ? kFewTileKeys : kTileKeys; }
+
 // Key tiles of item i.
-LRM_HD int item_tiles(int n, int kv, int span, int i) {
-    const int last = (i + 1) * span < n ? (i + 1) * span : n;  // (i + 1) * span <= n + span: no overflow at 2^24 tokens
-    return (kv - n + last - 1) / kTileKeys + 1;
+LRM_HD int item_tiles(Shape s, int n, int kv, int i) {
+    const int tokens = item_tokens(s, n, i);
+    return (kv - n + i * s.span + tokens - 1) / tile_keys(tokens * s.group) + 1;
 }
 
-// An item's units: `own` for its start and end, then `tile` a tile.
+// An item's units: `own` for its start and end, then `tile` a tile. One is about 830 cycles: a tile of 128 keys comes
+// from HBM in 2,500; one of 80 keys takes 1,700 for two slots' rows.
 struct Cost {
     int own, tile;
 };
-LRM_HD Cost item_cost(int n, int span, int i) {
-    const bool wide = n - i * span > span / 2;
-    return wide ? Cost{3, 2} : Cost{2, 1};
+LRM_HD Cost item_cost(Shape s, int n, int i) {
+    return item_tokens(s, n, i) * s.group <= kFewRows ? Cost{6, 3} : Cost{6, 2};
 }
 // The first tile that lies behind `units` of an item's units (neighbouring shares round to the same tile).
 LRM_HD int tile_at(Cost c, int units) { return units > c.own ? (units - c.own) / c.tile : 0; }
 
-// Units of the items before item i (i <= items - 1, so all of them are wide) of one head.
-LRM_HD uint64_t units_before(int n, int kv, int span, int i) {
+// Units of the items before item i (i <= items - 1, so they are whole spans: more than kFewRows rows) of one head.
+LRM_HD uint64_t units_before(Shape s, int n, int kv, int i) {
     if (i == 0) return 0;
-    const Cost c = item_cost(n, span, 0);
-    return (floor_sum((uint64_t)i, kTileKeys, (uint32_t)span, (uint64_t)(kv - n + span - 1)) + (uint64_t)i) *
+    const Cost c = item_cost(s, n, 0);
+    return (floor_sum((uint64_t)i, kTileKeys, (uint32_t)s.span, (uint64_t)(kv - n + s.span - 1)) + (uint64_t)i) *
                (uint64_t)c.tile + (uint64_t)i * c.own;
 }
 
 // Units of one head.
-LRM_HD uint64_t head_units(int n, int kv, int span) {
-    const int last = items_of(n, span) - 1;
-    const Cost c = item_cost(n, span, last);
-    return units_before(n, kv, span, last) + (uint64_t)(item_tiles(n, kv, span, last) * c.tile + c.own);
+LRM_HD uint64_t head_units(Shape s, int n, int kv) {
+    const int last = items_of(n, s.span) - 1;
+    const Cost c = item_cost(s, n, last);
+    return units_before(s, n, kv, last) + (uint64_t)(item_tiles(s, n, kv, last) * c.tile + c.own);
 }
 
 // The item of a head that holds its unit `off`.
-LRM_HD int item_at(int n, int kv, int span, uint64_t off) {
-    int lo = 0, hi = items_of(n, span);  // units_before(lo) <= off < units_before(hi)
+LRM_HD int item_at(Shape s, int n, int kv, uint64_t off) {
+    int lo = 0, hi = items_of(n, s.span);  // units_before(lo) <= off < units_before(hi)
     while (hi - lo > 1) {
         const int mid = (lo + hi) / 2;
-        if (units_before(n, kv, span, mid) <= off)
+        if (units_before(s, n, kv, mid) <= off)
             lo = mid;
         else
             hi = mid;
@@ -91,7 +97,7 @@ LRM_HD int item_at(int n, int kv, int span, uint64_t off) {
     return lo;
 }
 
-// CTAs that take part: at least `least` units each (2 or more, so that a share within an item holds a tile), so that
+// CTAs that take part: at least `least` units each (3 or more, so that a share within an item holds a tile), so that
 // short work is not cut into pieces that cost more to merge than they save.
 LRM_HD int ctas_of(uint64_t units, int ctas, int least) {
     if (units >= (uint64_t)ctas * (uint64_t)least) return ctas;
