@@ -50,7 +50,7 @@ constexpr int kRegsLaunch = 168;  // 65536 / 384, rounded down to the allocation
 constexpr int kRegsControl = 72, kRegsSoftmax = 216;
 static_assert(128 * kRegsControl + 256 * kRegsSoftmax <= kThreads * kRegsLaunch, "register split exceeds the launch");
 constexpr float kRescaleThreshold = 8.0f;  // log2 units: the reference maximum moves only when a tile exceeds it by more
-constexpr int kLeastUnits = 12;
+constexpr int kLeastUnits = 30;
 constexpr int kFewRows = sched::kFewRows;  // items of up to this many rows run with keys and rows swapped
 constexpr int FEW_SUB = kFewRows * 128;  // half of the dims (q) or keys (P) of up to 32 rows
 constexpr uint32_t kErrWaitProducer = 0x4010, kErrWaitIssuer = 0x4011, kErrWaitSoftmax = 0x4012, kErrWaitScheduler = 0x4013;
@@ -66,7 +66,7 @@ struct Item {
 
 // An item whose last keys lie in later CTAs' ranges, left by the CTA that holds its first: partial slot 1 of this CTA
 // and slots 0 of the next `follow` CTAs make it up. ntok 0: none.
-struct Record {
+struct alignas(16) Record {
     int tok0, ntok, kvh, follow;
 };
 
@@ -115,6 +115,7 @@ struct Params {
     PagedAttnArgs a;
     int group, tt, rows_cap;  // query heads a KV head; tokens a slot; rows of a partial slot
     int few_tok;              // tokens of a few-row item's q box
+    int inv_group;            // ceil(2^16 / group): r * inv_group >> 16 = r / group for r < 128
     float *part_o, *part_ml;
     Record *records;
 };
@@ -479,7 +480,7 @@ __device__ __forceinline__ bool few_item(const RoleState &r, const Item &it, uin
                 ptx::tmem_ld_wait();
                 o = __float_as_uint(__uint_as_float(o) +
                                     poison_sum(a, it.table, it.kvh, max(it.kb * TKF, it.pos0 / TKF * TKF),
-                                               min(it.pos0 + e / group, it.ke * TKF - 1), TKF, it.kb + s, 2, key));
+                                               min(it.pos0 + (e * r.p->inv_group >> 16), it.ke * TKF - 1), TKF, it.kb + s, 2, key));
                 asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(tO + e), "r"(o) : "memory");
             }
         ptx::tmem_st_wait();
@@ -523,7 +524,7 @@ __device__ __forceinline__ bool few_item(const RoleState &r, const Item &it, uin
     float w0 = l0 == 0.f ? 0.f : ptx::ex2(m0 - mt), w1 = l1 == 0.f ? 0.f : ptx::ex2(m1 - mt);
     const float lt = (l0 == 0.f ? 0.f : w0 * l0) + (l1 == 0.f ? 0.f : w1 * l1);
     const size_t part = ((size_t)r.cta * 2 + (it.dest > 0)) * r.p->rows_cap;
-    const int tok = lane / group;
+    const int tok = lane * r.p->inv_group >> 16;
     int64_t at;  // of the row in out, or in the partial results
     if (it.dest < 0) {
         const float inv = 1.f / lt;
@@ -1002,14 +1003,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int s = (warp - 4) >> 2;  // slot
         const int quarter = warp & 3;   // TMEM lanes this warp may access
         const int rl = quarter * 32 + lane;
-        const int tl = rl / p.group, hl = rl - tl * p.group;  // this row's token (of the slot) and query head (of the group)
-        const int warp_tl = (quarter * 32) / p.group;         // the warp's first token
-        int rows4[4];  // token << 8 | query head of the four rows that this lane helps to write
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int r = quarter * 32 + (lane & ~3) + j;
-            rows4[j] = (r / p.group) << 8 | (r % p.group);
-        }
+        const int tl = rl * p.inv_group >> 16, hl = rl - tl * p.group;  // this row's token (of the slot) and query head (of the group)
+        const int warp_tl = quarter * 32 * p.inv_group >> 16;  // the warp's first token
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         const uint32_t tS = tmem + 256 * s + lanes;
         const float sc = a.scale_log2;
@@ -1064,8 +1059,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (active) {
                     if (key0 + TK - 1 > it.pos0 + warp_token) {
                         const int lim = it.pos0 + token - key0;  // keys 0..lim of the tile are visible
+                        const int low = it.pos0 + warp_token - key0;  // keys 0..low are visible to every row of the warp
 #pragma unroll
-                        for (int e = 0; e < TK; ++e) x[e] = e <= lim ? x[e] : -INFINITY;
+                        for (int b = 0; b < TK; b += 16)
+                            if (b + 15 > low) {
+#pragma unroll
+                                for (int e = b; e < b + 16; ++e) x[e] = e <= lim ? x[e] : -INFINITY;
+                            }
                     }
                     float mx[8];
 #pragma unroll
@@ -1170,7 +1170,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             const bool poisoned = c.poison[0][k & 1] == k + 1 || c.poison[1][k & 1] == k + 1;
             if (active) {
-                // o = w[0] O_0 + w[1] O_1 (wide: this slot's O alone), 16 dims at a time
+                // o = w[0] O_0 + w[1] O_1 (wide: this slot's O alone), 32 dims at a time
                 const uint32_t tO = (wide ? tS : tmem + lanes) + 128;
                 const bool two = !wide && used1;
                 if (poisoned) {
@@ -1184,57 +1184,63 @@ __global__ void __launch_bounds__(kThreads, 1)
                         ptx::tc_fence_after();
                     }
                 }
-                const float inv = it.dest < 0 ? 1.f / l : 1.f;
-                const float w0 = w[0] * inv, w1 = w[1] * inv;
-                const size_t part = ((size_t)cta * 2 + (it.dest > 0)) * p.rows_cap;
                 const int c0 = wide ? 0 : 64 * s, c1 = wide ? 128 : 64 * s + 64;
-                if (it.dest >= 0 && valid && c0 == 0)
-                    *reinterpret_cast<float2 *>(p.part_ml + (part + token * p.group + hl) * 2) = make_float2(m_ref, l);
+                const float inv = it.dest < 0 ? 1.f / l : 1.f, w0 = w[0] * inv, w1 = w[1] * inv;
+                if (it.dest < 0) {
+                    // four lanes write 64 contiguous bytes of each of their four rows
+                    __nv_bfloat16 *rows[4];
+                    bool real[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int r = quarter * 32 + (lane & ~3) + j, tj = r * p.inv_group >> 16, tok = wide ? s * p.tt + tj : tj;
+                        real[j] = tj < p.tt && tok < it.ntok;
+                        rows[j] = a.out + (size_t)(it.tok0 + tok) * a.ld_out +
+                                  (size_t)(it.kvh * p.group + r - tj * p.group) * kHeadDim + 8 * (lane & 3);
+                    }
 #pragma unroll 1
-                for (int col = c0; col < c1; col += 32) {
-                    uint4 v[4];
-#pragma unroll
-                    for (int b = 0; b < 2; ++b) {
-                        uint32_t o[16];
-                        ptx::tmem_ld16(tO + col + 16 * b, o);
+                    for (int col = c0; col < c1; col += 32) {
+                        float o[32];
+                        ptx::tmem_ld32(tO + col, reinterpret_cast<uint32_t *>(o));
                         ptx::tmem_ld_wait();
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * w0);
                         if (two) {
-                            uint32_t o1[16];
-                            ptx::tmem_ld16(tO + 256 + col + 16 * b, o1);
+                            float o1[32];
+                            ptx::tmem_ld32(tO + 256 + col, reinterpret_cast<uint32_t *>(o1));
                             ptx::tmem_ld_wait();
 #pragma unroll
-                            for (int e = 0; e < 16; ++e)
-                                o[e] = __float_as_uint(fmaf(__uint_as_float(o1[e]), w1, __uint_as_float(o[e])));
-                        }
-                        if (it.dest < 0) {
+                            for (int e = 0; e < 32; ++e) o[e] = fmaf(o1[e], w1, o[e] * w0);
+                        } else {
 #pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const uint32_t *x = o + 8 * e;
-                                v[2 * b + e] = make_uint4(pack2(__uint_as_float(x[0]), __uint_as_float(x[1])),
-                                                          pack2(__uint_as_float(x[2]), __uint_as_float(x[3])),
-                                                          pack2(__uint_as_float(x[4]), __uint_as_float(x[5])),
-                                                          pack2(__uint_as_float(x[6]), __uint_as_float(x[7])));
-                            }
-                        } else if (valid) {
-                            float4 *d = reinterpret_cast<float4 *>(p.part_o + (part + token * p.group + hl) * kHeadDim + col + 16 * b);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                d[e] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]),
-                                                   __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
+                            for (int e = 0; e < 32; e += 2) ptx::fma_x2(o[e], o[e + 1], o[e], o[e + 1], w0, w0, 0.f, 0.f);
                         }
-                    }
-                    if (it.dest < 0) {
-                        // four lanes write 64 contiguous bytes of each of their four rows
+                        uint4 v[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            v[e] = make_uint4(pack2(o[8 * e], o[8 * e + 1]), pack2(o[8 * e + 2], o[8 * e + 3]),
+                                              pack2(o[8 * e + 4], o[8 * e + 5]), pack2(o[8 * e + 6], o[8 * e + 7]));
                         quad_transpose(v, lane);
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const int tj = rows4[j] >> 8, hj = rows4[j] & 255, tok = wide ? s * p.tt + tj : tj;
-                            if (tj < p.tt && tok < it.ntok)
-                                *reinterpret_cast<uint4 *>(a.out + (size_t)(it.tok0 + tok) * a.ld_out +
-                                                           (size_t)(it.kvh * p.group + hj) * kHeadDim + col +
-                                                           8 * (lane & 3)) = v[j];
+                        for (int j = 0; j < 4; ++j)
+                            if (real[j]) *reinterpret_cast<uint4 *>(rows[j] + col) = v[j];
+                    }
+                } else {
+                    const size_t row = ((size_t)cta * 2 + (it.dest > 0)) * p.rows_cap + token * p.group + hl;
+                    if (valid && c0 == 0) *reinterpret_cast<float2 *>(p.part_ml + row * 2) = make_float2(m_ref, l);
+#pragma unroll 1
+                    for (int col = c0; col < c1; col += 16) {
+                        float o[16];
+                        ptx::tmem_ld16(tO + col, reinterpret_cast<uint32_t(&)[16]>(o));
+                        ptx::tmem_ld_wait();
+                        if (two) {
+                            float o1[16];
+                            ptx::tmem_ld16(tO + 256 + col, reinterpret_cast<uint32_t(&)[16]>(o1));
+                            ptx::tmem_ld_wait();
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) o[e] = fmaf(o1[e], w1, o[e] * w0);
+                        }
+                        if (valid) {
+                            float4 *d = reinterpret_cast<float4 *>(p.part_o + row * kHeadDim + col);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) d[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
                         }
                     }
                 }
@@ -1251,41 +1257,53 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // Merges the partial results of the items that a cut passes through: o = sum 2^(m_i - m) o_i / sum 2^(m_i - m) l_i in the
-// order of their keys. Block (CTA, 8 rows), a warp a row, 4 dims a lane.
-__global__ void __launch_bounds__(256) paged_combine_kernel(Params p) {
+// order of their keys. Block (CTA, part of its rows), a warp a row at a time, 4 dims a lane. Rows of two parts (a cut or
+// two) are nearly all there is; their loads are issued together.
+constexpr int kCombineRows = 32;  // rows of a block of 8 warps
+__global__ void __launch_bounds__(256) paged_combine_kernel(const __grid_constant__ Params p) {
     ptx::griddep_wait();
-    const Record rec = p.records[blockIdx.x];
-    const int row = blockIdx.y * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
-    if (row >= rec.ntok * p.group) return;
-    const int n = rec.follow + 1;
+    const int4 rec = *reinterpret_cast<const int4 *>(p.records + blockIdx.x);  // tok0, ntok, kvh, follow
+    const int lane = threadIdx.x % 32, n = rec.w + 1, rows = rec.y * p.group;
     // partial i: slot 1 of the record's CTA, then slot 0 of each CTA behind it
-    auto at = [&](int i) { return ((size_t)(blockIdx.x + i) * 2 + (i == 0)) * p.rows_cap + row; };
-    float m = -INFINITY;
-    for (int i = lane; i < n; i += 32) {
-        const float2 ml = *reinterpret_cast<const float2 *>(p.part_ml + at(i) * 2);
-        if (ml.y != 0.f) m = fmaxf(m, ml.x);
-    }
+    const size_t first = ((size_t)blockIdx.x * 2 + 1) * p.rows_cap, step = (size_t)2 * p.rows_cap;
+#pragma unroll 1
+    for (int row = blockIdx.y * kCombineRows + threadIdx.x / 32; row < min(rows, (int)(blockIdx.y + 1) * kCombineRows);
+         row += 8) {
+        auto at = [&](int i) { return (i ? first + p.rows_cap + (size_t)(i - 1) * step : first) + row; };
+        float m = -INFINITY, l = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+        for (int i = 0; i < n; i += 4) {
+            float2 ml[4];
+            float4 o[4];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    float l = 0.f;
-#pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-        const float2 ml = *reinterpret_cast<const float2 *>(p.part_ml + at(i) * 2);
-        const float4 o = *reinterpret_cast<const float4 *>(p.part_o + at(i) * kHeadDim + 4 * lane);
-        if (ml.y == 0.f) continue;  // the row saw none of this part's keys
-        const float w = ptx::ex2(ml.x - m);
-        l += w * ml.y;
-        acc.x += w * o.x;
-        acc.y += w * o.y;
-        acc.z += w * o.z;
-        acc.w += w * o.w;
+            for (int u = 0; u < 4; ++u) {
+                ml[u] = make_float2(-INFINITY, 0.f);
+                o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (i + u < n) {
+                    const size_t x = at(i + u);
+                    ml[u] = *reinterpret_cast<const float2 *>(p.part_ml + x * 2);
+                    o[u] = *reinterpret_cast<const float4 *>(p.part_o + x * kHeadDim + 4 * lane);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if (ml[u].y == 0.f) continue;  // the row saw none of this part's keys
+                const float m2 = fmaxf(m, ml[u].x), w = ptx::ex2(ml[u].x - m2), f = l == 0.f ? 0.f : ptx::ex2(m - m2);
+                l = l * f + w * ml[u].y;
+                acc.x = acc.x * f + w * o[u].x;
+                acc.y = acc.y * f + w * o[u].y;
+                acc.z = acc.z * f + w * o[u].z;
+                acc.w = acc.w * f + w * o[u].w;
+                m = m2;
+            }
+        }
+        const float inv = 1.f / l;
+        const int token = row / p.group, h = row - token * p.group;
+        *reinterpret_cast<uint2 *>(p.a.out + (size_t)(rec.x + token) * p.a.ld_out +
+                                   (size_t)(rec.z * p.group + h) * kHeadDim + 4 * lane) =
+            make_uint2(pack2(acc.x * inv, acc.y * inv), pack2(acc.z * inv, acc.w * inv));
     }
-    const float inv = 1.f / l;
-    const int token = row / p.group, h = row - token * p.group;
-    *reinterpret_cast<uint2 *>(p.a.out + (size_t)(rec.tok0 + token) * p.a.ld_out +
-                               (size_t)(rec.kvh * p.group + h) * kHeadDim + 4 * lane) =
-        make_uint2(pack2(acc.x * inv, acc.y * inv), pack2(acc.z * inv, acc.w * inv));
 }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
@@ -1333,6 +1351,7 @@ cudaError_t launch_paged_attention(const PagedAttnArgs &a, int sms, cudaStream_t
     Params p;
     p.a = a;
     p.group = a.q_heads / a.kv_heads;
+    p.inv_group = (65535 + p.group) / p.group;
     p.tt = sched::kTileRows / p.group;
     p.rows_cap = partial_rows(a.tokens, a.q_heads, a.kv_heads);
     p.records = reinterpret_cast<Record *>(a.workspace);
@@ -1352,7 +1371,7 @@ cudaError_t launch_paged_attention(const PagedAttnArgs &a, int sms, cudaStream_t
     if (e != cudaSuccess) return e;
     // The merge launches under the attention kernel's tail; its own wait orders it behind that kernel's writes.
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(sms, (p.rows_cap + 7) / 8);
+    cfg.gridDim = dim3(sms, (p.rows_cap + kCombineRows - 1) / kCombineRows);
     cfg.blockDim = dim3(256);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];

@@ -58,13 +58,14 @@ LRM_HD int item_tiles(Shape s, int n, int kv, int i) {
     return (kv - n + i * s.span + tokens - 1) / tile_keys(tokens * s.group) + 1;
 }
 
-// An item's units: `own` for its start and end, then `tile` a tile. One is about 830 cycles: a tile of 128 keys comes
-// from HBM in 2,500; one of 80 keys takes 1,700 for two slots' rows.
+// An item's units: `own` for its start and end, then `tile` a tile. A unit is about 300 cycles, from a fit over the CTAs of
+// forty mixtures: few rows 4,500 + 1,800 a tile, one slot's rows 6,600 + 1,500, two slots' 9,500 + 2,000.
 struct Cost {
     int own, tile;
 };
 LRM_HD Cost item_cost(Shape s, int n, int i) {
-    return item_tokens(s, n, i) * s.group <= kFewRows ? Cost{6, 3} : Cost{6, 2};
+    const int tokens = item_tokens(s, n, i);
+    return tokens * s.group <= kFewRows ? Cost{15, 6} : (tokens <= s.span / 2 ? Cost{22, 5} : Cost{32, 7});
 }
 // The first tile that lies behind `units` of an item's units (neighbouring shares round to the same tile).
 LRM_HD int tile_at(Cost c, int units) { return units > c.own ? (units - c.own) / c.tile : 0; }
@@ -97,7 +98,7 @@ LRM_HD int item_at(Shape s, int n, int kv, uint64_t off) {
     return lo;
 }
 
-// CTAs that take part: at least `least` units each (3 or more, so that a share within an item holds a tile), so that
+// CTAs that take part: at least `least` units each (7 or more, so that a share within an item holds a tile), so that
 // short work is not cut into pieces that cost more to merge than they save.
 LRM_HD int ctas_of(uint64_t units, int ctas, int least) {
     if (units >= (uint64_t)ctas * (uint64_t)least) return ctas;
@@ -107,13 +108,13 @@ LRM_HD int ctas_of(uint64_t units, int ctas, int least) {
 
 // Where CTA c's range starts. (32-bit arithmetic where it fits: a 64-bit division costs the start of a short call.)
 LRM_HD uint64_t cut(uint64_t units, int ctas, int c) {
-    if (units < (1u << 20) && ctas <= 4096) return (uint32_t)units * (uint32_t)c / (uint32_t)ctas;
+    if (units < (1u << 20) && ctas <= 4095) return (uint32_t)units * (uint32_t)c / (uint32_t)ctas;
     return units * (uint64_t)c / (uint64_t)ctas;
 }
 
 // The CTA whose range holds unit u.
 LRM_HD int cta_of(uint64_t units, int ctas, uint64_t u) {
-    if (units < (1u << 20) && ctas <= 4096) return (int)((((uint32_t)u + 1) * (uint32_t)ctas - 1) / (uint32_t)units);
+    if (units < (1u << 20) && ctas <= 4095) return (int)((((uint32_t)u + 1) * (uint32_t)ctas - 1) / (uint32_t)units);
     return (int)(((u + 1) * (uint64_t)ctas - 1) / units);
 }
 
