@@ -362,13 +362,13 @@ lrm_status lrm_op_qkv_append(void *stream, const lrm_qkv_append_desc *desc);
  * A request whose rows fall outside the tokens, whose slot is outside 0 .. max_seqs - 1, or whose kv_len is below its
  * tokens or above 16 * pages_per_seq is not computed: its rows are left as they were and the error word gets 0x4001. A
  * page id outside the pool is never read: its keys count as zeros and the error word gets 0x4002. `workspace`:
- * lrm_op_paged_attention_workspace bytes, 16-byte aligned, any contents; calls that can run at the same time need one
- * each. scale must be positive and finite; ld_q and ld_out multiples of 8; q, pool and out 16-byte aligned.
+ * workspace_bytes, at least lrm_op_paged_attention_workspace's, 16-byte aligned, any contents; calls that can run at the
+ * same time need one each. scale must be positive and finite; ld_q and ld_out multiples of 8; q, pool and out 16-byte aligned.
  * Limits: requests 1 .. 65535, tokens 1 .. 2^24, max_seqs 1 .. 2^17, pages_per_seq 1 .. 2^20, kv_pages 1 .. 2^26 with
  * kv_pages * kv_heads below 2^30. */
 typedef struct lrm_paged_attn_desc {
     uint64_t q, pool, page_table, slots, cu_seqlens, kv_len, out, workspace;
-    int64_t ld_q, ld_out;
+    int64_t ld_q, ld_out, workspace_bytes;
     int32_t requests, tokens, q_heads, kv_heads, head_dim, max_seqs, pages_per_seq, kv_pages;
     float scale;
 } lrm_paged_attn_desc;

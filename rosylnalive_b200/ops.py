@@ -6,6 +6,7 @@ Arguments are torch CUDA tensors (used only as device memory and streams); every
 from __future__ import annotations
 
 import ctypes
+import struct
 
 from . import native as N
 
@@ -60,9 +61,9 @@ class QkvAppendDesc(ctypes.Structure):
 
 class PagedAttnDesc(ctypes.Structure):
     _fields_ = [("q", U64), ("pool", U64), ("page_table", U64), ("slots", U64), ("cu_seqlens", U64), ("kv_len", U64),
-                ("out", U64), ("workspace", U64), ("ld_q", I64), ("ld_out", I64), ("requests", I32), ("tokens", I32),
-                ("q_heads", I32), ("kv_heads", I32), ("head_dim", I32), ("max_seqs", I32), ("pages_per_seq", I32),
-                ("kv_pages", I32), ("scale", ctypes.c_float)]
+                ("out", U64), ("workspace", U64), ("ld_q", I64), ("ld_out", I64), ("workspace_bytes", I64),
+                ("requests", I32), ("tokens", I32), ("q_heads", I32), ("kv_heads", I32), ("head_dim", I32),
+                ("max_seqs", I32), ("pages_per_seq", I32), ("kv_pages", I32), ("scale", ctypes.c_float)]
 
 
 DEC_SWIGLU, DEC_RESID = 1, 2
@@ -78,11 +79,11 @@ N.extra_signatures({
     "lrm_op_wait_probe": [P, U32, U32],
     "lrm_op_argmax_rows": [P, P, I32, I32, P],
     "lrm_op_decode_gemm": [P, ctypes.POINTER(DecodeGemmDesc)],
-    "lrm_op_page_plan": [P, ctypes.POINTER(PagePlanDesc)],
-    "lrm_op_page_release": [P, ctypes.POINTER(PageReleaseDesc)],
-    "lrm_op_qkv_append": [P, ctypes.POINTER(QkvAppendDesc)],
+    "lrm_op_page_plan": [P, P],  # the descriptors of these four also as packed bytes
+    "lrm_op_page_release": [P, P],
+    "lrm_op_qkv_append": [P, P],
     "lrm_op_paged_attention_workspace": [I32, I32, I32],
-    "lrm_op_paged_attention": [P, ctypes.POINTER(PagedAttnDesc)],
+    "lrm_op_paged_attention": [P, P],
 }, {"lrm_op_decode_attention_workspace": U64, "lrm_op_paged_attention_workspace": U64})
 
 # Scratch built into liblrmcuda.so for lrm_op_decode_attention_static (LRM_DECODE_ATTN_STATIC_SCRATCH_BYTES).
@@ -192,52 +193,63 @@ def decode_attention_static(q, pool, page_table, seq_len, slots, out, pages_per_
 # from the host. These take tensors of any CUDA device (all of a call on one) and launch on `stream`, or on that
 # device's current stream. What only the device knows (slots, lengths, page ids) is checked there: error_word().
 
-def _need(ok, what):
-    if not ok:
-        raise ValueError(what)
+# A call is a few microseconds on the device, so the checks are kept to a few as well: one loop over its tensors, and the
+# descriptor packed in one go (the layouts of PagePlanDesc and its like above).
+
+_PLAN, _RELEASE = struct.Struct("12Q5i"), struct.Struct("8Q4i")
+_APPEND, _ATTN = struct.Struct("9Q2q6if"), struct.Struct("8Q3q8if")
+assert [x.size for x in (_PLAN, _RELEASE, _APPEND, _ATTN)] == [
+    _LAST.offset + _LAST.size for _LAST in (PagePlanDesc.max_tokens, PageReleaseDesc.kv_pages, QkvAppendDesc.eps,
+                                            PagedAttnDesc.scale)]
+_torch = None
 
 
-def _same_device(call, tensors):
-    """The device index that all of a call's tensors are on."""
-    dev = tensors[0].get_device()
+def _t():
+    global _torch
+    if _torch is None:
+        import torch
+
+        _torch = torch
+    return _torch
+
+
+def _int32(call, names, tensors, dev):
+    """Checks that the tensors are contiguous int32 tensors of device `dev`."""
+    i32 = _t().int32
     for t in tensors:
-        if t.get_device() != dev or dev < 0:
-            raise ValueError(f"{call}: all tensors must be on one CUDA device")
-    return dev
-
-
-def _int32(call, **tensors):
-    """The tensors are contiguous int32."""
-    import torch
-
-    for name, t in tensors.items():
-        if t.dtype is not torch.int32 or not t.is_contiguous():
+        if t.dtype is not i32 or t.get_device() != dev or not t.is_contiguous():
+            if t.dtype is i32 and t.is_contiguous():
+                raise ValueError(f"{call}: all tensors must be on one CUDA device")
+            name = names.split()[next(i for i, x in enumerate(tensors) if x is t)]
             raise ValueError(f"{call}: {name} must be a contiguous int32 tensor")
 
 
 def _pool(call, pool):
-    import torch
-
-    if pool.dtype is not torch.bfloat16 or pool.dim() != 5 or pool.shape[2:] != (2, 16, 128) or \
-            not pool.is_contiguous():
+    if pool.dtype is not _t().bfloat16 or pool.dim() != 5 or pool.shape[2:] != (2, 16, 128) or not pool.is_contiguous():
         raise ValueError(f"{call}: pool must be contiguous bfloat16 [pages, kv_heads, 2, 16, 128]")
 
 
-def _rows_of_heads(t):
-    """Whether only the rows of [T, heads, 128] are strided."""
-    return t.stride(2) == 1 and (t.stride(1) == 128 or t.shape[1] == 1)
+def _rows_of_heads(t, shape):
+    """The row stride of [T, heads, 128] when only its rows are strided, else None."""
+    rows, heads, last = t.stride()
+    if last != 1 or (heads != 128 and shape[1] != 1):
+        return None
+    return rows if shape[0] > 1 else shape[1] * 128
 
 
 def _launch(call, fn, desc, dev, stream):
-    import torch
-
-    if dev == torch.cuda.current_device():
-        s = torch.cuda.current_stream(dev) if stream is None else stream
-        N.check(fn(s.cuda_stream, ctypes.byref(desc)), None, call)
+    if dev < 0:
+        raise ValueError(f"{call}: all tensors must be on one CUDA device")
+    torch = _t()
+    if dev == torch._C._cuda_getDevice():
+        s = torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream
+        status = fn(s, desc)
     else:
         with torch.cuda.device(dev):
             s = torch.cuda.current_stream(dev) if stream is None else stream
-            N.check(fn(s.cuda_stream, ctypes.byref(desc)), None, call)
+            status = fn(s.cuda_stream, desc)
+    if status:
+        N.check(status, None, call)
 
 
 def page_plan(slots, new_len, seq_len, page_table, free_list, free_count, cu_seqlens, kv_len, tok_pos, slot_map,
@@ -247,26 +259,26 @@ def page_plan(slots, new_len, seq_len, page_table, free_list, free_count, cu_seq
     each; seq_len [max_seqs], page_table [max_seqs, pages_per_seq], free_list [kv_pages] and free_count [1] are the
     cache's state, updated in place unless seq_len_out / free_count_out are given. All or nothing: a step that breaks a
     rule (error_word 0x5001 .. 0x5004) takes no page and becomes a step of no tokens."""
-    call = "page_plan"
-    seq_len_out = seq_len if seq_len_out is None else seq_len_out
-    free_count_out = free_count if free_count_out is None else free_count_out
-    _int32(call, slots=slots, new_len=new_len, seq_len=seq_len, page_table=page_table, free_list=free_list,
-           free_count=free_count, cu_seqlens=cu_seqlens, kv_len=kv_len, tok_pos=tok_pos, slot_map=slot_map,
-           seq_len_out=seq_len_out, free_count_out=free_count_out)
-    n, seqs, tokens = slots.numel(), seq_len.numel(), tok_pos.numel()
-    _need(page_table.dim() == 2 and page_table.shape[0] == seqs and seq_len_out.numel() == seqs,
-          "page_plan: page_table must be [max_seqs, pages_per_seq] and seq_len, seq_len_out [max_seqs]")
-    _need(new_len.numel() == n and kv_len.numel() == n and cu_seqlens.numel() == n + 1 and slot_map.numel() == tokens
-          and free_count.numel() == 1 and free_count_out.numel() == 1,
-          "page_plan: new_len and kv_len are [requests], cu_seqlens [requests + 1], tok_pos and slot_map one size, "
-          "free_count and free_count_out one element")
-    dev = _same_device(call, (slots, new_len, seq_len, page_table, free_list, free_count, cu_seqlens, kv_len, tok_pos,
-                              slot_map, seq_len_out, free_count_out))
-    d = PagePlanDesc(slots.data_ptr(), new_len.data_ptr(), seq_len.data_ptr(), page_table.data_ptr(),
-                     free_list.data_ptr(), free_count.data_ptr(), cu_seqlens.data_ptr(), kv_len.data_ptr(),
-                     tok_pos.data_ptr(), slot_map.data_ptr(), seq_len_out.data_ptr(), free_count_out.data_ptr(), n,
-                     seqs, page_table.shape[1], free_list.numel(), tokens)
-    _launch(call, N.lib().lrm_op_page_plan, d, dev, stream)
+    if seq_len_out is None:
+        seq_len_out = seq_len
+    if free_count_out is None:
+        free_count_out = free_count
+    dev = slots.get_device()
+    _int32("page_plan", "slots new_len seq_len page_table free_list free_count cu_seqlens kv_len tok_pos slot_map "
+           "seq_len_out free_count_out",
+           (slots, new_len, seq_len, page_table, free_list, free_count, cu_seqlens, kv_len, tok_pos, slot_map,
+            seq_len_out, free_count_out), dev)
+    n, seqs, tokens, table = slots.numel(), seq_len.numel(), tok_pos.numel(), page_table.shape
+    if len(table) != 2 or table[0] != seqs or seq_len_out.numel() != seqs:
+        raise ValueError("page_plan: page_table must be [max_seqs, pages_per_seq] and seq_len, seq_len_out [max_seqs]")
+    if (new_len.numel() != n or kv_len.numel() != n or cu_seqlens.numel() != n + 1 or slot_map.numel() != tokens
+            or free_count.numel() != 1 or free_count_out.numel() != 1):
+        raise ValueError("page_plan: new_len and kv_len are [requests], cu_seqlens [requests + 1], tok_pos and slot_map "
+                         "one size, free_count and free_count_out one element")
+    _launch("page_plan", N.lib().lrm_op_page_plan, _PLAN.pack(
+        slots.data_ptr(), new_len.data_ptr(), seq_len.data_ptr(), page_table.data_ptr(), free_list.data_ptr(),
+        free_count.data_ptr(), cu_seqlens.data_ptr(), kv_len.data_ptr(), tok_pos.data_ptr(), slot_map.data_ptr(),
+        seq_len_out.data_ptr(), free_count_out.data_ptr(), n, seqs, table[1], free_list.numel(), tokens), dev, stream)
 
 
 def page_release(slots, keep_len, seq_len, page_table, free_list, free_count, seq_len_out=None, free_count_out=None,
@@ -274,22 +286,22 @@ def page_release(slots, keep_len, seq_len, page_table, free_list, free_count, se
     """Cuts slots [requests] (-1: padding) back to their first keep_len tokens (0 frees a slot) and puts the pages
     behind them back on top of the free list. State and outputs as in page_plan. All or nothing: a call that breaks a
     rule (error_word 0x5011, 0x5012, 0x5014) changes nothing."""
-    call = "page_release"
-    seq_len_out = seq_len if seq_len_out is None else seq_len_out
-    free_count_out = free_count if free_count_out is None else free_count_out
-    _int32(call, slots=slots, keep_len=keep_len, seq_len=seq_len, page_table=page_table, free_list=free_list,
-           free_count=free_count, seq_len_out=seq_len_out, free_count_out=free_count_out)
-    n, seqs = slots.numel(), seq_len.numel()
-    _need(page_table.dim() == 2 and page_table.shape[0] == seqs and seq_len_out.numel() == seqs,
-          "page_release: page_table must be [max_seqs, pages_per_seq] and seq_len, seq_len_out [max_seqs]")
-    _need(keep_len.numel() == n and free_count.numel() == 1 and free_count_out.numel() == 1,
-          "page_release: keep_len is [requests], free_count and free_count_out one element")
-    dev = _same_device(call, (slots, keep_len, seq_len, page_table, free_list, free_count, seq_len_out,
-                              free_count_out))
-    d = PageReleaseDesc(slots.data_ptr(), keep_len.data_ptr(), seq_len.data_ptr(), page_table.data_ptr(),
-                        free_list.data_ptr(), free_count.data_ptr(), seq_len_out.data_ptr(),
-                        free_count_out.data_ptr(), n, seqs, page_table.shape[1], free_list.numel())
-    _launch(call, N.lib().lrm_op_page_release, d, dev, stream)
+    if seq_len_out is None:
+        seq_len_out = seq_len
+    if free_count_out is None:
+        free_count_out = free_count
+    dev = slots.get_device()
+    _int32("page_release", "slots keep_len seq_len page_table free_list free_count seq_len_out free_count_out",
+           (slots, keep_len, seq_len, page_table, free_list, free_count, seq_len_out, free_count_out), dev)
+    n, seqs, table = slots.numel(), seq_len.numel(), page_table.shape
+    if len(table) != 2 or table[0] != seqs or seq_len_out.numel() != seqs:
+        raise ValueError("page_release: page_table must be [max_seqs, pages_per_seq] and seq_len, seq_len_out [max_seqs]")
+    if keep_len.numel() != n or free_count.numel() != 1 or free_count_out.numel() != 1:
+        raise ValueError("page_release: keep_len is [requests], free_count and free_count_out one element")
+    _launch("page_release", N.lib().lrm_op_page_release, _RELEASE.pack(
+        slots.data_ptr(), keep_len.data_ptr(), seq_len.data_ptr(), page_table.data_ptr(), free_list.data_ptr(),
+        free_count.data_ptr(), seq_len_out.data_ptr(), free_count_out.data_ptr(), n, seqs, table[1],
+        free_list.numel()), dev, stream)
 
 
 def qkv_append(qkv, q_norm, k_norm, eps, cos, sin, tok_pos, slot_map, q_out, pool, stream=None):
@@ -298,53 +310,56 @@ def qkv_append(qkv, q_norm, k_norm, eps, cos, sin, tok_pos, slot_map, q_out, poo
     to pool [pages, kv_heads, 2, 16, 128] at slot_map [T] (int32 page * 16 + offset; -1 skips the row). q_norm, k_norm:
     bfloat16 [128], or both None for no norm. cos, sin: float32 [rows, 64] read at tok_pos [T], or all three None for
     no rotation."""
-    import torch
-
-    call = "qkv_append"
-    _pool(call, pool)
-    bf16 = torch.bfloat16
-    _need(qkv.dtype is bf16 and q_out.dtype is bf16 and qkv.dim() == 2 and q_out.dim() == 3 and q_out.shape[2] == 128
-          and q_out.shape[0] == qkv.shape[0],
-          "qkv_append: qkv must be bfloat16 [T, columns] and q_out bfloat16 [T, q_heads, 128]")
-    tokens, q_heads, kv_heads = qkv.shape[0], q_out.shape[1], pool.shape[1]
-    _need(qkv.shape[1] == (q_heads + 2 * kv_heads) * 128, "qkv_append: qkv has (q_heads + 2 kv_heads) * 128 columns")
-    _need(qkv.stride(1) == 1 and _rows_of_heads(q_out),
-          "qkv_append: only the rows of qkv and q_out may be strided")
-    _int32(call, slot_map=slot_map)
-    _need(slot_map.numel() == tokens, "qkv_append: slot_map is [T]")
-    tensors = [qkv, slot_map, q_out, pool]
+    torch = _t()
+    bf16, dev = torch.bfloat16, qkv.get_device()
+    _pool("qkv_append", pool)
+    shape, q_shape, pool_shape = qkv.shape, q_out.shape, pool.shape
+    if (qkv.dtype is not bf16 or q_out.dtype is not bf16 or len(shape) != 2 or len(q_shape) != 3 or q_shape[2] != 128
+            or q_shape[0] != shape[0]):
+        raise ValueError("qkv_append: qkv must be bfloat16 [T, columns] and q_out bfloat16 [T, q_heads, 128]")
+    tokens, q_heads, kv_heads = shape[0], q_shape[1], pool_shape[1]
+    if shape[1] != (q_heads + 2 * kv_heads) * 128:
+        raise ValueError("qkv_append: qkv has (q_heads + 2 kv_heads) * 128 columns")
+    ld_q, (ld_qkv, inner) = _rows_of_heads(q_out, q_shape), qkv.stride()
+    if inner != 1 or ld_q is None:
+        raise ValueError("qkv_append: only the rows of qkv and q_out may be strided")
+    _int32("qkv_append", "slot_map", (slot_map,), dev)
+    if slot_map.numel() != tokens:
+        raise ValueError("qkv_append: slot_map is [T]")
+    gains = table = (0, 0)
+    at = rope_rows = 0
     if q_norm is not None or k_norm is not None:
-        _need(q_norm is not None and k_norm is not None, "qkv_append: give both gains or none")
+        if q_norm is None or k_norm is None:
+            raise ValueError("qkv_append: give both gains or none")
         for g in (q_norm, k_norm):
-            _need(g.dtype is bf16 and g.numel() == 128 and g.is_contiguous(),
-                  "qkv_append: q_norm and k_norm are contiguous bfloat16 [128]")
-        tensors += (q_norm, k_norm)
-    rope_rows = 0
+            if g.dtype is not bf16 or g.numel() != 128 or not g.is_contiguous():
+                raise ValueError("qkv_append: q_norm and k_norm are contiguous bfloat16 [128]")
+            if g.get_device() != dev:
+                raise ValueError("qkv_append: all tensors must be on one CUDA device")
+        gains = q_norm.data_ptr(), k_norm.data_ptr()
     if cos is not None or sin is not None:
-        _need(cos is not None and sin is not None and tok_pos is not None,
-              "qkv_append: give cos, sin and tok_pos, or none of them")
-        _int32(call, tok_pos=tok_pos)
+        if cos is None or sin is None or tok_pos is None:
+            raise ValueError("qkv_append: give cos, sin and tok_pos, or none of them")
+        _int32("qkv_append", "tok_pos", (tok_pos,), dev)
+        rope = cos.shape
         for c in (cos, sin):
-            _need(c.dtype is torch.float32 and c.dim() == 2 and c.shape[1] == 64 and c.is_contiguous(),
-                  "qkv_append: cos and sin are contiguous float32 [rows, 64]")
-        _need(cos.shape == sin.shape and tok_pos.numel() == tokens,
-              "qkv_append: cos and sin have one shape and tok_pos is [T]")
-        rope_rows = cos.shape[0]
-        tensors += (cos, sin, tok_pos)
-    dev = _same_device(call, tensors)
-
-    def ptr(t):
-        return 0 if t is None else t.data_ptr()
-
-    d = QkvAppendDesc(qkv.data_ptr(), ptr(q_norm), ptr(k_norm), ptr(cos), ptr(sin), ptr(tok_pos) if rope_rows else 0,
-                      slot_map.data_ptr(), q_out.data_ptr(), pool.data_ptr(),
-                      qkv.stride(0) if tokens > 1 else qkv.shape[1], q_out.stride(0) if tokens > 1 else q_heads * 128,
-                      tokens, q_heads, kv_heads, 128, rope_rows, pool.shape[0], eps)
-    _launch(call, N.lib().lrm_op_qkv_append, d, dev, stream)
+            if c.dtype is not torch.float32 or c.dim() != 2 or c.shape[1] != 64 or not c.is_contiguous():
+                raise ValueError("qkv_append: cos and sin are contiguous float32 [rows, 64]")
+            if c.get_device() != dev:
+                raise ValueError("qkv_append: all tensors must be on one CUDA device")
+        if rope != sin.shape or tok_pos.numel() != tokens:
+            raise ValueError("qkv_append: cos and sin have one shape and tok_pos is [T]")
+        table, at, rope_rows = (cos.data_ptr(), sin.data_ptr()), tok_pos.data_ptr(), rope[0]
+    if q_out.get_device() != dev or pool.get_device() != dev:
+        raise ValueError("qkv_append: all tensors must be on one CUDA device")
+    _launch("qkv_append", N.lib().lrm_op_qkv_append, _APPEND.pack(
+        qkv.data_ptr(), *gains, *table, at, slot_map.data_ptr(), q_out.data_ptr(), pool.data_ptr(),
+        ld_qkv if tokens > 1 else shape[1], ld_q, tokens, q_heads, kv_heads, 128, rope_rows, pool_shape[0], eps), dev,
+        stream)
 
 
 def paged_attention_workspace(tokens, q_heads, kv_heads) -> int:
-    """Bytes of workspace for paged_attention calls of up to `tokens` rows on the current device."""
+    """Bytes of workspace for paged_attention calls of up to `tokens` rows, on the current device."""
     return int(N.lib().lrm_op_paged_attention_workspace(tokens, q_heads, kv_heads))
 
 
@@ -353,26 +368,24 @@ def paged_attention(q, pool, page_table, slots, cu_seqlens, kv_len, out, workspa
     [T, q_heads, 128] (bfloat16, rows may be strided, as may out's) are the last tokens of the kv_len[i] keys of slot
     slots[i], read through page_table [max_seqs, pages_per_seq] from pool [pages, kv_heads, 2, 16, 128]. Rows of no
     request are left as they were. workspace: paged_attention_workspace(T, ...) bytes, any contents."""
-    import torch
-
-    call = "paged_attention"
-    _pool(call, pool)
-    bf16 = torch.bfloat16
-    _need(q.dtype is bf16 and out.dtype is bf16 and q.dim() == 3 and q.shape[2] == 128 and out.shape == q.shape,
-          "paged_attention: q and out must be bfloat16 [T, q_heads, 128]")
-    _need(_rows_of_heads(q) and _rows_of_heads(out),
-          "paged_attention: only the rows of q and out may be strided")
-    _int32(call, page_table=page_table, slots=slots, cu_seqlens=cu_seqlens, kv_len=kv_len)
-    tokens, q_heads, kv_heads, n = q.shape[0], q.shape[1], pool.shape[1], slots.numel()
-    _need(page_table.dim() == 2 and kv_len.numel() == n and cu_seqlens.numel() == n + 1,
-          "paged_attention: page_table is [max_seqs, pages_per_seq], kv_len [requests], cu_seqlens [requests + 1]")
-    _need(workspace.is_contiguous(), "paged_attention: the workspace must be contiguous")
-    dev = _same_device(call, (q, pool, page_table, slots, cu_seqlens, kv_len, out, workspace))
-    lib = N.lib()
-    _need(workspace.numel() * workspace.element_size() >= lib.lrm_op_paged_attention_workspace(tokens, q_heads, kv_heads),
-          "paged_attention: the workspace is smaller than paged_attention_workspace says")
-    d = PagedAttnDesc(q.data_ptr(), pool.data_ptr(), page_table.data_ptr(), slots.data_ptr(), cu_seqlens.data_ptr(),
-                      kv_len.data_ptr(), out.data_ptr(), workspace.data_ptr(),
-                      q.stride(0) if tokens > 1 else q_heads * 128, out.stride(0) if tokens > 1 else q_heads * 128, n,
-                      tokens, q_heads, kv_heads, 128, page_table.shape[0], page_table.shape[1], pool.shape[0], scale)
-    _launch(call, lib.lrm_op_paged_attention, d, dev, stream)
+    bf16, dev = _t().bfloat16, q.get_device()
+    _pool("paged_attention", pool)
+    shape, pool_shape, table = q.shape, pool.shape, page_table.shape
+    if q.dtype is not bf16 or out.dtype is not bf16 or len(shape) != 3 or shape[2] != 128 or out.shape != shape:
+        raise ValueError("paged_attention: q and out must be bfloat16 [T, q_heads, 128]")
+    ld_q, ld_out = _rows_of_heads(q, shape), _rows_of_heads(out, shape)
+    if ld_q is None or ld_out is None:
+        raise ValueError("paged_attention: only the rows of q and out may be strided")
+    _int32("paged_attention", "page_table slots cu_seqlens kv_len", (page_table, slots, cu_seqlens, kv_len), dev)
+    (tokens, q_heads, _), kv_heads, n = shape, pool_shape[1], slots.numel()
+    if len(table) != 2 or kv_len.numel() != n or cu_seqlens.numel() != n + 1:
+        raise ValueError("paged_attention: page_table is [max_seqs, pages_per_seq], kv_len [requests], cu_seqlens "
+                         "[requests + 1]")
+    if out.get_device() != dev or pool.get_device() != dev or workspace.get_device() != dev:
+        raise ValueError("paged_attention: all tensors must be on one CUDA device")
+    if not workspace.is_contiguous():
+        raise ValueError("paged_attention: the workspace must be contiguous")
+    _launch("paged_attention", N.lib().lrm_op_paged_attention, _ATTN.pack(
+        q.data_ptr(), pool.data_ptr(), page_table.data_ptr(), slots.data_ptr(), cu_seqlens.data_ptr(),
+        kv_len.data_ptr(), out.data_ptr(), workspace.data_ptr(), ld_q, ld_out, workspace.nbytes, n, tokens, q_heads,
+        kv_heads, 128, table[0], table[1], pool_shape[0], scale), dev, stream)

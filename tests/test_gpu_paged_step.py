@@ -141,6 +141,43 @@ def test_plan_and_release_follow_the_lists(requests, max_seqs, cap):
         sv.same_state()
 
 
+def test_plan_and_release_of_more_requests_than_one_pass_of_the_cluster():
+    max_seqs, requests, P = 20000, 9001, 3
+    sv = Server(max_seqs, P, max_seqs * P, seed=5)
+    r = np.random.default_rng(5)
+    for step in range(2):
+        slots = r.permutation(max_seqs)[:requests]
+        slots = np.where(r.uniform(size=requests) < 0.1, -1, slots)
+        new = np.array([0 if s == -1 else min(int(r.integers(0, 25)), 48 - sv.len[s]) for s in slots])
+        check_plan(sv, slots.tolist(), new.tolist(), int(new.sum()) + 3)
+        slots = r.permutation(max_seqs)[:requests]
+        keep = [int(r.integers(0, sv.len[s] + 1)) for s in slots]
+        gpu_release(sv, slots.tolist(), keep)
+        sv.release(slots.tolist(), keep)
+        sv.same_state()
+
+
+@pytest.mark.parametrize("shift", [0, 1, 2, 3])
+def test_a_large_plan_writes_rows_at_any_alignment(shift):
+    # Above 5120 rows the outputs are written 16 bytes at a time where they can be.
+    requests, max_seqs, P = 300, 300, 12
+    sv = Server(max_seqs, P, max_seqs * P, seed=shift)
+    slots = np.random.default_rng(9).permutation(max_seqs).tolist()
+    new = np.random.default_rng(8).integers(0, 60, requests).tolist()
+    max_tokens = 12000
+    big = [torch.full((max_tokens + 4,), -77, dtype=torch.int32, device="cuda") for _ in range(2)]
+    pos, smap = [b[shift: shift + max_tokens] for b in big]
+    cu, kv = step_buffers(requests, 1)[:2]
+    ops.page_plan(i32(slots), i32(new), sv.seq_len, sv.table, sv.free_list, sv.count, cu, kv, pos, smap)
+    want = sv.plan(slots, new)
+    pad = max_tokens - len(want[2])
+    assert cu.tolist() == want[0] and kv.tolist() == want[1]
+    assert pos.tolist() == want[2] + [0] * pad and smap.tolist() == want[3] + [-1] * pad
+    for b in big:
+        assert b[:shift].tolist() == [-77] * shift and b[shift + max_tokens:].tolist() == [-77] * (4 - shift)
+    sv.same_state()
+
+
 def test_plan_takes_the_very_last_page_and_fills_a_row():
     sv = Server(2, 3, 4, seed=3)
     check_plan(sv, [1, 0], [48, 16], 64)

@@ -32,7 +32,7 @@ def append(**kw):
 
 def attn(**kw):
     d = dict(q=A, pool=A, page_table=A, slots=A, cu_seqlens=A, kv_len=A, out=A, workspace=A, ld_q=16 * 128,
-             ld_out=16 * 128, requests=3, tokens=5, q_heads=16, kv_heads=8, head_dim=128, max_seqs=4, pages_per_seq=5,
+             ld_out=16 * 128, workspace_bytes=1 << 40, requests=3, tokens=5, q_heads=16, kv_heads=8, head_dim=128, max_seqs=4, pages_per_seq=5,
              kv_pages=6, scale=0.1)
     return "lrm_op_paged_attention", O.PagedAttnDesc(**{**d, **kw})
 
@@ -57,7 +57,7 @@ REFUSED = [
       for v in (0, -1, BIG)],
     attn(q_heads=15), attn(q_heads=129, kv_heads=1, ld_q=129 * 128, ld_out=129 * 128), attn(head_dim=64),
     attn(kv_pages=1 << 26, kv_heads=16), attn(ld_q=16 * 128 - 8), attn(ld_q=16 * 128 + 4), attn(ld_out=0),
-    attn(ld_out=1 << 40), attn(scale=0.0), attn(scale=-1.0), attn(scale=INF), attn(scale=NAN), attn(scale=3e38),
+    attn(ld_out=1 << 40), attn(workspace_bytes=0), attn(workspace_bytes=-1), attn(workspace_bytes=1000), attn(scale=0.0), attn(scale=-1.0), attn(scale=INF), attn(scale=NAN), attn(scale=3e38),
 ]
 
 
@@ -123,3 +123,9 @@ def test_the_wrappers_check_types_shapes_and_devices():
     refused(O.paged_attention, ok_attn, 1, b(3, 2, 2, 16, 64), "pool")
     refused(O.paged_attention, ok_attn, 4, i(4), "cu_seqlens")
     refused(O.paged_attention, ok_attn, 6, b(4, 4, 128), "out")
+
+
+def test_the_packed_descriptors_are_the_structures():
+    for packed, desc in ((O._PLAN, plan()[1]), (O._RELEASE, release()[1]), (O._APPEND, append()[1]), (O._ATTN, attn()[1])):
+        values = [getattr(desc, name) for name, _ in desc._fields_]
+        assert packed.pack(*values) == bytes(desc)[:packed.size]
