@@ -50,7 +50,7 @@ constexpr int kRegsLaunch = 168;  // 65536 / 384, rounded down to the allocation
 constexpr int kRegsControl = 72, kRegsSoftmax = 216;
 static_assert(128 * kRegsControl + 256 * kRegsSoftmax <= kThreads * kRegsLaunch, "register split exceeds the launch");
 constexpr float kRescaleThreshold = 8.0f;  // log2 units: the reference maximum moves only when a tile exceeds it by more
-constexpr int kLeastUnits = 30;
+constexpr int kLeastUnits = 12;  // of a CTA (900 keys, 8 KV heads: 11.7 us, 14.1 with 30; more CTAs than that do not help)
 constexpr int kFewRows = sched::kFewRows;  // items of up to this many rows run with keys and rows swapped
 constexpr int FEW_SUB = kFewRows * 128;  // half of the dims (q) or keys (P) of up to 32 rows
 constexpr uint32_t kErrWaitProducer = 0x4010, kErrWaitIssuer = 0x4011, kErrWaitSoftmax = 0x4012, kErrWaitScheduler = 0x4013;
@@ -107,12 +107,14 @@ struct Control {
         } few;
     };
 };
+static_assert(kLeastUnits > sched::kWide.tile, "a share within an item holds a tile");
 static_assert(offsetof(Control, few) % 16 == 0, "few.max is read as float4");
 constexpr int SMEM_BYTES = (SLOTS + KV_ST) * TILE + (int)sizeof(Control);
 static_assert(SMEM_BYTES <= 227 * 1024, "shared memory of one CTA");
 
 struct Params {
     PagedAttnArgs a;
+    sched::Shape shape;
     int group, tt, rows_cap;  // query heads a KV head; tokens a slot; rows of a partial slot
     int few_tok;              // tokens of a few-row item's q box
     int inv_group;            // ceil(2^16 / group): r * inv_group >> 16 = r / group for r < 128
@@ -173,18 +175,21 @@ __device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap *map, uin
 
 __device__ __forceinline__ bool finite_bf16(uint32_t h) { return (h & 0x7F80u) != 0x7F80u; }
 
-__device__ __forceinline__ Request load_request(const PagedAttnArgs &a, int r, bool report) {
-    Request q;
-    q.start = a.cu_seqlens[r];
-    const int end = a.cu_seqlens[r + 1];
-    q.kv = a.kv_len[r];
-    q.slot = a.slots[r];
-    const int64_t n = (int64_t)end - q.start;
-    const bool ok = q.start >= 0 && n > 0 && end <= a.tokens && q.slot >= 0 && q.slot < a.max_seqs && q.kv >= n &&
-                    q.kv <= (int64_t)a.pages_per_seq * kPageTokens;
+struct RawRequest {
+    int start, end, kv, slot;
+};
+__device__ __forceinline__ RawRequest fetch_request(const PagedAttnArgs &a, int r) {
+    return RawRequest{a.cu_seqlens[r], a.cu_seqlens[r + 1], a.kv_len[r], a.slots[r]};
+}
+__device__ __forceinline__ Request check_request(const PagedAttnArgs &a, const RawRequest &w, bool report) {
+    const int64_t n = (int64_t)w.end - w.start;
+    const bool ok = w.start >= 0 && n > 0 && w.end <= a.tokens && w.slot >= 0 && w.slot < a.max_seqs && w.kv >= n &&
+                    w.kv <= (int64_t)a.pages_per_seq * kPageTokens;
     if (report && !ok && n != 0) atomicCAS(a.err, 0u, kErrAttnRequest);
-    q.n = ok ? (int)n : 0;
-    return q;
+    return Request{w.start, ok ? (int)n : 0, w.kv, w.slot};
+}
+__device__ __forceinline__ Request load_request(const PagedAttnArgs &a, int r, bool report) {
+    return check_request(a, fetch_request(a, r), report);
 }
 
 // Tests v in this warp's quarter of a tile (32 keys, one a lane) and zeroes what is not finite. Keys up to
@@ -577,7 +582,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     // (the shuffle tells the compiler that the warp index, and so the role, is the same in all lanes)
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid / 32, 0), lane = tid % 32;
     const int cta = blockIdx.x, span = SLOTS * p.tt;
-    const sched::Shape shape = {p.group, span};
+    const sched::Shape &shape = p.shape;
+    // This thread's requests, `per` of them. The first one's lengths are on their way while the CTA sets itself up.
+    const int per = a.requests <= kThreads ? 1 : (a.requests + kThreads - 1) / kThreads;
+    const int r0 = min(a.requests, tid * per), r1 = min(a.requests, r0 + per);
+    RawRequest raw = {0, 0, 0, 0};
+    if (r0 < r1) raw = fetch_request(a, r0);
     if (ptx::smem_u32(smem) & 1023) {  // the swizzled tiles and their descriptors need 1024-byte alignment
         if (tid == 0) {
             atomicCAS(err, 0u, kErrWaitScheduler);
@@ -622,11 +632,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     // ---- this CTA's range ----
     // Units of each thread's requests, their exclusive sums over the threads, and the request of the range's last unit.
-    const int per = (a.requests + kThreads - 1) / kThreads;
-    const int r0 = min(a.requests, tid * per), r1 = min(a.requests, r0 + per);
-    uint64_t own = 0;
+    Request mine = check_request(a, raw, cta == 0);
+    uint64_t head = mine.n ? sched::head_units(shape, mine.n, mine.kv) : 0;
+    uint64_t own = head * (uint64_t)a.kv_heads;
 #pragma unroll 1
-    for (int r = r0; r < r1; ++r) {
+    for (int r = r0 + 1; r < r1; ++r) {
         const Request q = load_request(a, r, cta == 0);
         if (q.n) own += sched::head_units(shape, q.n, q.kv) * (uint64_t)a.kv_heads;
     }
@@ -647,25 +657,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         units += c.warp_sum[w];
     }
     const uint32_t tmem = __shfl_sync(0xffffffffu, c.tmem, 0);
-    const int ctas = sched::ctas_of(units, (int)gridDim.x, kLeastUnits);
-    const bool idle = cta >= ctas;
-    const uint64_t u0 = idle ? 0 : sched::cut(units, ctas, cta), u1 = idle ? 0 : sched::cut(units, ctas, cta + 1);
+    const sched::Cut cut = sched::make_cut(units, (int)gridDim.x, kLeastUnits);
+    const bool idle = cta >= cut.ctas;
+    const uint64_t u0 = sched::begin(cut, cta), u1 = sched::begin(cut, cta + 1);
     if (!idle && before <= u1 - 1 && u1 - 1 < before + own) {
-        uint64_t at = before;
+        int r = r0;
+        uint64_t at = before, w = head * (uint64_t)a.kv_heads;  // units before request r, and of it
 #pragma unroll 1
-        for (int r = r0; r < r1; ++r) {
-            const Request q = load_request(a, r, false);
-            if (!q.n) continue;
-            const uint64_t w = sched::head_units(shape, q.n, q.kv) * (uint64_t)a.kv_heads;
-            if (u1 - 1 < at + w) {
-                c.start_req = r;
-                c.start_off = u1 - 1 - at;
-                c.start_head = sched::head_units(shape, q.n, q.kv);
-                c.start = q;
-                break;
-            }
+        while (u1 - 1 >= at + w) {
             at += w;
+            mine = load_request(a, ++r, false);
+            head = mine.n ? sched::head_units(shape, mine.n, mine.kv) : 0;
+            w = head * (uint64_t)a.kv_heads;
         }
+        c.start_req = r;
+        c.start_off = u1 - 1 - at;
+        c.start_head = head;
+        c.start = mine;
     }
     __syncthreads();
 
@@ -681,9 +689,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 uint64_t left = u1 - u0;
                 int h = (int)sched::quotient(c.start_off, c.start_head);
                 const uint64_t off = c.start_off - (uint64_t)h * c.start_head;
-                int i = sched::item_at(shape, q.n, q.kv, off);
-                int tiles = sched::item_tiles(shape, q.n, q.kv, i);
-                sched::Cost cost = sched::item_cost(shape, q.n, i);
+                int items = sched::items_of(shape, q.n);
+                int i = sched::item_at(shape, q.n, q.kv, off, items);
+                sched::Item cost = sched::item_of(shape, q.n, q.kv, i, items);
                 // the share's end within the item, in units
                 int end = (int)(off - sched::units_before(shape, q.n, q.kv, i)) + 1;
                 Record rec = {0, 0, 0, 0};
@@ -695,13 +703,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                         begin = (uint64_t)end > left ? end - (int)left : 0;
                         it.kb = sched::tile_at(cost, begin);
                         it.ke = sched::tile_at(cost, end);
+                        it.table = (int64_t)q.slot * a.pages_per_seq;
+                        if (it.ke > it.kb)  // the producers' first load of page ids would miss otherwise
+                            asm volatile("prefetch.global.L2 [%0];" ::"l"(a.page_table + it.table +
+                                                                          it.kb * (cost.tile == sched::kFew.tile ? TKF : TK) / kPageTokens));
                         it.tok0 = q.start + i * span;
                         it.ntok = min(span, q.n - i * span);
                         it.kvh = h;
                         it.pos0 = q.kv - q.n + i * span;
                         it.npages = (q.kv + kPageTokens - 1) / kPageTokens;
-                        it.table = (int64_t)q.slot * a.pages_per_seq;
-                        it.dest = it.kb == 0 && it.ke == tiles ? -1 : (it.kb == 0 ? 1 : 0);
+                        it.dest = it.kb == 0 && it.ke == cost.tiles ? -1 : (it.kb == 0 ? 1 : 0);
                     }
                     if (it.ke > it.kb || left == 0) {  // a share of the item's own cost alone has no tiles
                         if (!wait_bar(&c.item_empty[k % ITEMS], ((k / ITEMS) & 1) ^ 1, err, kErrWaitScheduler)) break;
@@ -710,8 +721,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         ++k;
                         if (it.dest == 1)  // the range's last item, begun here: the rest of it lies behind the range
                             rec = Record{it.tok0, it.ntok, h,
-                                         sched::cta_of(units, ctas, u1 - 1 + (uint64_t)(cost.own + cost.tile * tiles - end)) -
-                                             cta};
+                                         sched::cta_of(cut, u1 - 1 + (uint64_t)(cost.units - end)) - cta};
                     }
                     if (left == 0) break;
                     left -= (uint64_t)(end - begin);
@@ -726,12 +736,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                             do q = load_request(a, --r, false);
                             while (!q.n);
                             h = a.kv_heads - 1;
+                            items = sched::items_of(shape, q.n);
                         }
-                        i = sched::items_of(q.n, span) - 1;
+                        i = items - 1;
                     }
-                    tiles = sched::item_tiles(shape, q.n, q.kv, i);
-                    cost = sched::item_cost(shape, q.n, i);
-                    end = cost.own + cost.tile * tiles;
+                    cost = sched::item_of(shape, q.n, q.kv, i, items);
+                    end = cost.units;
                 }
                 p.records[cta] = rec;
             }
@@ -756,15 +766,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const bool few = ntok * p.group <= kFewRows, wide = ntok > p.tt;
                 const int tile_pages = few ? TKF / kPageTokens : TK / kPageTokens, window = 32 / tile_pages;
                 // The z coordinates (K or V block of page and head) of a window of tiles, one a lane.
+                // Its page ids are loaded ahead and first used when they are needed (for the first ones, once q is on its way).
                 auto fetch = [&](int t) {
                     const int pg = (kb + t) * tile_pages + lane;
-                    if (pg >= npages) return oob;  // keys past the request, which no row sees
-                    const int id = pages[pg];
+                    return pg < npages ? pages[pg] : 0;
+                };
+                auto place = [&](int t, int id) {
+                    if ((kb + t) * tile_pages + lane >= npages) return oob;  // keys past the request, which no row sees
                     if ((uint32_t)id < (uint32_t)a.kv_pages) return (id * a.kv_heads + kvh) * 2 + kv;
                     atomicCAS(err, 0u, kErrAttnPage);
                     return oob;
                 };
-                int z = fetch(0);
+                int id = fetch(0);
                 if (!kv) {
                     // Two few-row items in a row use different places for q, so the second one's q is loaded while the
                     // first still runs; otherwise q's place is free once the item before is through. Even and odd items
@@ -794,9 +807,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int lead = wide ? 2 : 3;
 #pragma unroll 1
                 for (int t0 = 0; t0 < nt; t0 += window) {
-                    c.z[kv][lane] = z;
+                    c.z[kv][lane] = place(t0, id);
                     __syncwarp();
-                    z = t0 + window < nt ? fetch(t0 + window) : oob;
+                    if (t0 + window < nt) id = fetch(t0 + window);
                     // One lane issues a window's copies (the choice of it and the return from it cost some 170 cycles).
                     if (ptx::elect_one()) {
                         const int t1 = min(nt, t0 + window);
@@ -1131,7 +1144,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                         ok = false;
                         break;
                     }
-                    if (rl < TK)
+                    // (wide: the other slot's product of this tile is issued behind this one's)
+                    if (rl < TK && !(wide && s == 1))
                         clean_v(sKV + (xv % KV_ST) * TILE, rl, lane, it.pos0 + it.ntok - 1 - key0, &c.poison[s][k & 1], k + 1);
                 }
                 if (active) ptx::tmem_st_wait();
@@ -1257,52 +1271,67 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // Merges the partial results of the items that a cut passes through: o = sum 2^(m_i - m) o_i / sum 2^(m_i - m) l_i in the
-// order of their keys. Block (CTA, part of its rows), a warp a row at a time, 4 dims a lane. Rows of two parts (a cut or
-// two) are nearly all there is; their loads are issued together.
-constexpr int kCombineRows = 32;  // rows of a block of 8 warps
-__global__ void __launch_bounds__(256) paged_combine_kernel(const __grid_constant__ Params p) {
+// order of their keys. Block (CTA, 32 of its rows), a warp four rows at a time, 4 dims a lane. It is bound by latency, and
+// two parts (a cut or two) are nearly all there is, so the loads of two parts of the four rows are issued together.
+constexpr int kCombineWarps = 8, kCombineAtOnce = 4, kCombineRows = kCombineWarps * kCombineAtOnce;
+__global__ void __launch_bounds__(32 * kCombineWarps) paged_combine_kernel(const __grid_constant__ Params p) {
     ptx::griddep_wait();
     const int4 rec = *reinterpret_cast<const int4 *>(p.records + blockIdx.x);  // tok0, ntok, kvh, follow
     const int lane = threadIdx.x % 32, n = rec.w + 1, rows = rec.y * p.group;
+    const int row0 = blockIdx.y * kCombineRows + threadIdx.x / 32;
+    if (row0 >= rows) return;
     // partial i: slot 1 of the record's CTA, then slot 0 of each CTA behind it
     const size_t first = ((size_t)blockIdx.x * 2 + 1) * p.rows_cap, step = (size_t)2 * p.rows_cap;
-#pragma unroll 1
-    for (int row = blockIdx.y * kCombineRows + threadIdx.x / 32; row < min(rows, (int)(blockIdx.y + 1) * kCombineRows);
-         row += 8) {
-        auto at = [&](int i) { return (i ? first + p.rows_cap + (size_t)(i - 1) * step : first) + row; };
-        float m = -INFINITY, l = 0.f;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 1
-        for (int i = 0; i < n; i += 4) {
-            float2 ml[4];
-            float4 o[4];
+    float m[kCombineAtOnce], l[kCombineAtOnce];
+    float4 acc[kCombineAtOnce];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                ml[u] = make_float2(-INFINITY, 0.f);
-                o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (i + u < n) {
-                    const size_t x = at(i + u);
-                    ml[u] = *reinterpret_cast<const float2 *>(p.part_ml + x * 2);
-                    o[u] = *reinterpret_cast<const float4 *>(p.part_o + x * kHeadDim + 4 * lane);
+    for (int r = 0; r < kCombineAtOnce; ++r) {
+        m[r] = -INFINITY;
+        l[r] = 0.f;
+        acc[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll 1
+    for (int i = 0; i < n; i += 2) {
+        float2 ml[2][kCombineAtOnce];
+        float4 o[2][kCombineAtOnce];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const size_t part = (i + u ? first + p.rows_cap + (size_t)(i + u - 1) * step : first) + row0;
+#pragma unroll
+            for (int r = 0; r < kCombineAtOnce; ++r) {
+                ml[u][r] = make_float2(-INFINITY, 0.f);
+                o[u][r] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (i + u < n && row0 + r * kCombineWarps < rows) {
+                    const size_t x = part + r * kCombineWarps;
+                    ml[u][r] = *reinterpret_cast<const float2 *>(p.part_ml + x * 2);
+                    o[u][r] = *reinterpret_cast<const float4 *>(p.part_o + x * kHeadDim + 4 * lane);
                 }
             }
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                if (ml[u].y == 0.f) continue;  // the row saw none of this part's keys
-                const float m2 = fmaxf(m, ml[u].x), w = ptx::ex2(ml[u].x - m2), f = l == 0.f ? 0.f : ptx::ex2(m - m2);
-                l = l * f + w * ml[u].y;
-                acc.x = acc.x * f + w * o[u].x;
-                acc.y = acc.y * f + w * o[u].y;
-                acc.z = acc.z * f + w * o[u].z;
-                acc.w = acc.w * f + w * o[u].w;
-                m = m2;
-            }
         }
-        const float inv = 1.f / l;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r = 0; r < kCombineAtOnce; ++r) {
+                if (ml[u][r].y == 0.f) continue;  // the row saw none of this part's keys
+                const float m2 = fmaxf(m[r], ml[u][r].x), w = ptx::ex2(ml[u][r].x - m2);
+                const float f = l[r] == 0.f ? 0.f : ptx::ex2(m[r] - m2);
+                l[r] = l[r] * f + w * ml[u][r].y;
+                acc[r].x = acc[r].x * f + w * o[u][r].x;
+                acc[r].y = acc[r].y * f + w * o[u][r].y;
+                acc[r].z = acc[r].z * f + w * o[u][r].z;
+                acc[r].w = acc[r].w * f + w * o[u][r].w;
+                m[r] = m2;
+            }
+    }
+#pragma unroll
+    for (int r = 0; r < kCombineAtOnce; ++r) {
+        const int row = row0 + r * kCombineWarps;
+        if (row >= rows) break;
+        const float inv = 1.f / l[r];
         const int token = row / p.group, h = row - token * p.group;
         *reinterpret_cast<uint2 *>(p.a.out + (size_t)(rec.x + token) * p.a.ld_out +
                                    (size_t)(rec.z * p.group + h) * kHeadDim + 4 * lane) =
-            make_uint2(pack2(acc.x * inv, acc.y * inv), pack2(acc.z * inv, acc.w * inv));
+            make_uint2(pack2(acc[r].x * inv, acc[r].y * inv), pack2(acc[r].z * inv, acc[r].w * inv));
     }
 }
 
@@ -1336,7 +1365,7 @@ bool make_tmap(CUtensorMap *map, const void *ptr, uint64_t y, uint64_t z, uint64
 
 // Rows of a partial slot: those of an item, which a call of `tokens` rows bounds too.
 int partial_rows(int tokens, int q_heads, int kv_heads) {
-    const int group = q_heads / kv_heads, span = 2 * (sched::kTileRows / group);
+    const int group = q_heads / kv_heads, span = sched::make_shape(group).span;
     return (tokens < span ? tokens : span) * group;
 }
 
@@ -1351,6 +1380,7 @@ cudaError_t launch_paged_attention(const PagedAttnArgs &a, int sms, cudaStream_t
     Params p;
     p.a = a;
     p.group = a.q_heads / a.kv_heads;
+    p.shape = sched::make_shape(p.group);
     p.inv_group = (65535 + p.group) / p.group;
     p.tt = sched::kTileRows / p.group;
     p.rows_cap = partial_rows(a.tokens, a.q_heads, a.kv_heads);
@@ -1372,7 +1402,7 @@ cudaError_t launch_paged_attention(const PagedAttnArgs &a, int sms, cudaStream_t
     // The merge launches under the attention kernel's tail; its own wait orders it behind that kernel's writes.
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(sms, (p.rows_cap + kCombineRows - 1) / kCombineRows);
-    cfg.blockDim = dim3(256);
+    cfg.blockDim = dim3(32 * kCombineWarps);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -8,16 +8,19 @@
 // ranges of equal length, one a CTA, so every mixture of lengths is balanced; an item that a cut passes through is merged
 // from its CTAs' partial results. (Counting tiles alone left 32 requests of 5 tokens over 100 to 6000 keys at 64 us
 // against 43, and 8 chunks of 511 tokens among 56 decodes at 103 against 87.)
+//
+// Every CTA computes its range before it can load anything, so this is kept to a few multiplications: an item of a whole
+// span counts tile * keys / 80 rather than the tile's cost times its rounded-up tiles, which makes the units of the items
+// before one a closed form; divisions are by constants, or by the span with its inverse. (With the exact count, its sum by
+// Euclid's steps and divisions, it took 10 us of the 66 of those mixed chunks.)
 #pragma once
 
 #include <stdint.h>
 
 #ifdef __CUDACC__
 #define LRM_HD __host__ __device__ __forceinline__
-#define LRM_HD_FAR static __host__ __device__ __noinline__  // one copy: instruction space is scarce in the kernel
 #else
 #define LRM_HD inline
-#define LRM_HD_FAR inline
 #endif
 
 namespace lrm {
@@ -26,68 +29,67 @@ namespace sched {
 constexpr int kTileRows = 128;
 constexpr int kFewRows = 32, kFewTileKeys = 128, kTileKeys = 80;
 
-// sum over i in [0, n) of floor((a i + b) / m), by Euclid's steps on (a, m); a, b >= 0, m > 0.
-LRM_HD_FAR uint64_t floor_sum(uint64_t n, uint32_t m, uint32_t a, uint64_t b) {
-    uint64_t sum = 0;
-    for (;;) {
-        if (n == 0) return sum;
-        sum += (n * (n - 1) / 2) * (a / m) + n * (b / m);
-        a %= m;
-        b %= m;
-        const uint64_t y = (uint64_t)a * n + b;
-        if (y < m) return sum;
-        n = y / m;
-        b = y % m;
-        const uint32_t t = m;
-        m = a;
-        a = t;
-    }
-}
-
-LRM_HD int items_of(int n, int span) { return (n + span - 1) / span; }
-
+// inv_span = ceil(2^38 / span): x * inv_span >> 38 is x / span for x < 2^30 (span <= 256).
 struct Shape {
     int group, span;
+    uint64_t inv_span;
 };
-LRM_HD int item_tokens(Shape s, int n, int i) { return n - i * s.span < s.span ? n - i * s.span : s.span; }
-LRM_HD int tile_keys(int rows) { return rows <= kFewRows ? kFewTileKeys : kTileKeys; }
-
-// Key tiles of item i.
-LRM_HD int item_tiles(Shape s, int n, int kv, int i) {
-    const int tokens = item_tokens(s, n, i);
-    return (kv - n + i * s.span + tokens - 1) / tile_keys(tokens * s.group) + 1;
+LRM_HD Shape make_shape(int group) {
+    const int span = 2 * (kTileRows / group);
+    return Shape{group, span, ((uint64_t(1) << 38) + (uint64_t)span - 1) / (uint64_t)span};
 }
+LRM_HD int items_of(const Shape &s, int n) { return (int)(((uint64_t)(uint32_t)(n + s.span - 1) * s.inv_span) >> 38); }
 
-// An item's units: `own` for its start and end, then `tile` a tile. A unit is about 300 cycles, from a fit over the CTAs of
-// forty mixtures: few rows 4,500 + 1,800 a tile, one slot's rows 6,600 + 1,500, two slots' 9,500 + 2,000.
+// An item's units: `own` for its start and end, then `tile` a tile. A unit is about 300 cycles. Alone, items of few rows
+// take 4,000 cycles + 1,400 a tile, of one slot's rows 6,700 + 1,400, of two slots' 13,300 + 1,950; beside items of few
+// rows, whose loads fill the memory's queues, those of two slots wait for their tiles: 8,800 + 2,800. The weights lie in
+// between (8 chunks of 511 tokens among 56 single ones: 65.7 us, 68.8 with 32 + 7 units, 70.1 with 46 + 11).
 struct Cost {
     int own, tile;
 };
-LRM_HD Cost item_cost(Shape s, int n, int i) {
-    const int tokens = item_tokens(s, n, i);
-    return tokens * s.group <= kFewRows ? Cost{15, 6} : (tokens <= s.span / 2 ? Cost{22, 5} : Cost{32, 7});
-}
-// The first tile that lies behind `units` of an item's units (neighbouring shares round to the same tile).
-LRM_HD int tile_at(Cost c, int units) { return units > c.own ? (units - c.own) / c.tile : 0; }
+constexpr Cost kFew = {13, 5}, kNarrow = {22, 6}, kWide = {40, 10};
 
-// Units of the items before item i (i <= items - 1, so they are whole spans: more than kFewRows rows) of one head.
-LRM_HD uint64_t units_before(Shape s, int n, int kv, int i) {
+// Units of the items before item i of a head: all of them are whole spans, and so of two slots' rows.
+LRM_HD uint64_t units_before(const Shape &s, int n, int kv, int i) {
     if (i == 0) return 0;
-    const Cost c = item_cost(s, n, 0);
-    return (floor_sum((uint64_t)i, kTileKeys, (uint32_t)s.span, (uint64_t)(kv - n + s.span - 1)) + (uint64_t)i) *
-               (uint64_t)c.tile + (uint64_t)i * c.own;
+    const uint64_t keys = (uint64_t)i * (uint64_t)(uint32_t)(kv - n + s.span) + (uint64_t)i * (uint64_t)(i - 1) / 2 * s.span;
+    return keys * kWide.tile / kTileKeys + (uint64_t)i * kWide.own;
+}
+
+struct Item {
+    int tiles, units, own, tile;
+};
+// Item i of `items`.
+LRM_HD Item item_of(const Shape &s, int n, int kv, int i, int items) {
+    if (i < items - 1)
+        return Item{(int)((uint32_t)(kv - n + (i + 1) * s.span + kTileKeys - 1) / kTileKeys),
+                    (int)(units_before(s, n, kv, i + 1) - units_before(s, n, kv, i)), kWide.own, kWide.tile};
+    const int tokens = n - i * s.span;
+    const bool few = tokens * s.group <= kFewRows, narrow = 2 * tokens <= s.span;
+    const Cost c = few ? kFew : (narrow ? kNarrow : kWide);
+    const int tiles = few ? (int)((uint32_t)(kv + kFewTileKeys - 1) / kFewTileKeys)
+                          : (int)((uint32_t)(kv + kTileKeys - 1) / kTileKeys);
+    return Item{tiles, c.own + c.tile * tiles, c.own, c.tile};
+}
+
+// The first tile that lies behind `units` of an item's units (neighbouring shares round to the same tile). A whole span's
+// units are at most own + tile * tiles, so a unit within it is within its tiles, and `tile` + 1 units on hold one at least.
+LRM_HD int tile_at(const Item &t, int units) {
+    if (units >= t.units) return t.tiles;
+    if (units <= t.own) return 0;
+    const uint32_t x = (uint32_t)(units - t.own);
+    return (int)(t.tile == kWide.tile ? x / kWide.tile : (t.tile == kFew.tile ? x / kFew.tile : x / kNarrow.tile));
 }
 
 // Units of one head.
-LRM_HD uint64_t head_units(Shape s, int n, int kv) {
-    const int last = items_of(n, s.span) - 1;
-    const Cost c = item_cost(s, n, last);
-    return units_before(s, n, kv, last) + (uint64_t)(item_tiles(s, n, kv, last) * c.tile + c.own);
+LRM_HD uint64_t head_units(const Shape &s, int n, int kv) {
+    const int last = items_of(s, n) - 1;
+    return units_before(s, n, kv, last) + (uint64_t)item_of(s, n, kv, last, last + 1).units;
 }
 
 // The item of a head that holds its unit `off`.
-LRM_HD int item_at(Shape s, int n, int kv, uint64_t off) {
-    int lo = 0, hi = items_of(n, s.span);  // units_before(lo) <= off < units_before(hi)
+LRM_HD int item_at(const Shape &s, int n, int kv, uint64_t off, int items) {
+    int lo = 0, hi = items;  // units_before(lo) <= off < units_before(hi)
     while (hi - lo > 1) {
         const int mid = (lo + hi) / 2;
         if (units_before(s, n, kv, mid) <= off)
@@ -98,28 +100,34 @@ LRM_HD int item_at(Shape s, int n, int kv, uint64_t off) {
     return lo;
 }
 
-// CTAs that take part: at least `least` units each (7 or more, so that a share within an item holds a tile), so that
-// short work is not cut into pieces that cost more to merge than they save.
-LRM_HD int ctas_of(uint64_t units, int ctas, int least) {
-    if (units >= (uint64_t)ctas * (uint64_t)least) return ctas;
-    const int want = (int)((uint32_t)units / (uint32_t)least);
-    return want > 0 ? want : (units > 0 ? 1 : 0);
-}
-
-// Where CTA c's range starts. (32-bit arithmetic where it fits: a 64-bit division costs the start of a short call.)
-LRM_HD uint64_t cut(uint64_t units, int ctas, int c) {
-    if (units < (1u << 20) && ctas <= 4095) return (uint32_t)units * (uint32_t)c / (uint32_t)ctas;
-    return units * (uint64_t)c / (uint64_t)ctas;
-}
-
-// The CTA whose range holds unit u.
-LRM_HD int cta_of(uint64_t units, int ctas, uint64_t u) {
-    if (units < (1u << 20) && ctas <= 4095) return (int)((((uint32_t)u + 1) * (uint32_t)ctas - 1) / (uint32_t)units);
-    return (int)(((u + 1) * (uint64_t)ctas - 1) / units);
-}
-
 LRM_HD uint64_t quotient(uint64_t a, uint64_t b) {
     return (a | b) >> 32 ? a / b : (uint64_t)((uint32_t)a / (uint32_t)b);
+}
+
+// The cut of all units: CTA c's range is [begin(c), begin(c + 1)). CTAs that take part have at least `least` units each
+// (more than kWide.tile, so that a share within an item holds a tile): short work is not cut into pieces that cost more
+// to merge than they save.
+struct Cut {
+    int ctas;
+    uint32_t more;   // the first ranges that are one unit longer
+    uint64_t share;
+};
+LRM_HD Cut make_cut(uint64_t units, int ctas, int least) {
+    if (units < (uint64_t)ctas * (uint64_t)least) {
+        const int want = (int)((uint32_t)units / (uint32_t)least);
+        ctas = want > 0 ? want : (units > 0 ? 1 : 0);
+        if (!ctas) return Cut{0, 0, 0};
+    }
+    const uint64_t share = quotient(units, (uint64_t)ctas);
+    return Cut{ctas, (uint32_t)(units - share * (uint64_t)ctas), share};
+}
+LRM_HD uint64_t begin(const Cut &k, int c) {
+    return k.share * (uint64_t)c + ((uint32_t)c < k.more ? (uint32_t)c : k.more);
+}
+// The CTA whose range holds unit u.
+LRM_HD int cta_of(const Cut &k, uint64_t u) {
+    const uint64_t longer = (k.share + 1) * k.more;
+    return u < longer ? (int)quotient(u, k.share + 1) : (int)(k.more + quotient(u - longer, k.share));
 }
 
 }  // namespace sched
