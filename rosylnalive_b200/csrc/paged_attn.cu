@@ -1200,33 +1200,40 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 const int c0 = wide ? 0 : 64 * s, c1 = wide ? 128 : 64 * s + 64;
                 const float inv = it.dest < 0 ? 1.f / l : 1.f, w0 = w[0] * inv, w1 = w[1] * inv;
-                if (it.dest < 0) {
-                    // four lanes write 64 contiguous bytes of each of their four rows
-                    __nv_bfloat16 *rows[4];
-                    bool real[4];
+                // Four lanes write 64 contiguous bytes of each of their four rows (a lane's own row alone would be 16 bytes a
+                // store: half sectors, which took 11,000 cycles of a partial item against 4,000).
+                const size_t part = ((size_t)cta * 2 + (it.dest > 0)) * p.rows_cap;
+                if (it.dest >= 0 && valid && c0 == 0)
+                    *reinterpret_cast<float2 *>(p.part_ml + (part + token * p.group + hl) * 2) = make_float2(m_ref, l);
+                uint8_t *rows[4];
+                bool real[4];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int r = quarter * 32 + (lane & ~3) + j, tj = r * p.inv_group >> 16, tok = wide ? s * p.tt + tj : tj;
-                        real[j] = tj < p.tt && tok < it.ntok;
-                        rows[j] = a.out + (size_t)(it.tok0 + tok) * a.ld_out +
-                                  (size_t)(it.kvh * p.group + r - tj * p.group) * kHeadDim + 8 * (lane & 3);
-                    }
+                for (int j = 0; j < 4; ++j) {
+                    const int r = quarter * 32 + (lane & ~3) + j, tj = r * p.inv_group >> 16, tok = wide ? s * p.tt + tj : tj;
+                    const int hj = r - tj * p.group;
+                    real[j] = tj < p.tt && tok < it.ntok;
+                    rows[j] = it.dest < 0 ? reinterpret_cast<uint8_t *>(a.out + (size_t)(it.tok0 + tok) * a.ld_out +
+                                                                        (size_t)(it.kvh * p.group + hj) * kHeadDim)
+                                          : reinterpret_cast<uint8_t *>(p.part_o + (part + tok * p.group + hj) * kHeadDim);
+                    rows[j] += 16 * (lane & 3);
+                }
 #pragma unroll 1
-                    for (int col = c0; col < c1; col += 32) {
-                        float o[32];
-                        ptx::tmem_ld32(tO + col, reinterpret_cast<uint32_t *>(o));
+                for (int col = c0; col < c1; col += 32) {
+                    float o[32];
+                    ptx::tmem_ld32(tO + col, reinterpret_cast<uint32_t *>(o));
+                    ptx::tmem_ld_wait();
+                    if (two) {
+                        float o1[32];
+                        ptx::tmem_ld32(tO + 256 + col, reinterpret_cast<uint32_t *>(o1));
                         ptx::tmem_ld_wait();
-                        if (two) {
-                            float o1[32];
-                            ptx::tmem_ld32(tO + 256 + col, reinterpret_cast<uint32_t *>(o1));
-                            ptx::tmem_ld_wait();
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) o[e] = fmaf(o1[e], w1, o[e] * w0);
-                        } else {
+                        for (int e = 0; e < 32; ++e) o[e] = fmaf(o1[e], w1, o[e] * w0);
+                    } else {
 #pragma unroll
-                            for (int e = 0; e < 32; e += 2) ptx::fma_x2(o[e], o[e + 1], o[e], o[e + 1], w0, w0, 0.f, 0.f);
-                        }
-                        uint4 v[4];
+                        for (int e = 0; e < 32; e += 2) ptx::fma_x2(o[e], o[e + 1], o[e], o[e + 1], w0, w0, 0.f, 0.f);
+                    }
+                    uint4 v[4];
+                    if (it.dest < 0) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
                             v[e] = make_uint4(pack2(o[8 * e], o[8 * e + 1]), pack2(o[8 * e + 2], o[8 * e + 3]),
@@ -1234,27 +1241,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                         quad_transpose(v, lane);
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
-                            if (real[j]) *reinterpret_cast<uint4 *>(rows[j] + col) = v[j];
-                    }
-                } else {
-                    const size_t row = ((size_t)cta * 2 + (it.dest > 0)) * p.rows_cap + token * p.group + hl;
-                    if (valid && c0 == 0) *reinterpret_cast<float2 *>(p.part_ml + row * 2) = make_float2(m_ref, l);
-#pragma unroll 1
-                    for (int col = c0; col < c1; col += 16) {
-                        float o[16];
-                        ptx::tmem_ld16(tO + col, reinterpret_cast<uint32_t(&)[16]>(o));
-                        ptx::tmem_ld_wait();
-                        if (two) {
-                            float o1[16];
-                            ptx::tmem_ld16(tO + 256 + col, reinterpret_cast<uint32_t(&)[16]>(o1));
-                            ptx::tmem_ld_wait();
+                            if (real[j]) *reinterpret_cast<uint4 *>(rows[j] + col * 2) = v[j];
+                    } else {
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) o[e] = fmaf(o1[e], w1, o[e] * w0);
-                        }
-                        if (valid) {
-                            float4 *d = reinterpret_cast<float4 *>(p.part_o + row * kHeadDim + col);
+                        for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) d[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                            for (int e = 0; e < 4; ++e) v[e] = *reinterpret_cast<const uint4 *>(o + 16 * h + 4 * e);
+                            quad_transpose(v, lane);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                if (real[j]) *reinterpret_cast<uint4 *>(rows[j] + col * 4 + 64 * h) = v[j];
                         }
                     }
                 }
