@@ -40,7 +40,7 @@
 namespace lrm {
 namespace {
 
-constexpr int TK = sched::kTileKeys, TKF = sched::kFewTileKeys, KV_ST = 5, SLOTS = 2, ITEMS = 4;
+constexpr int TK = sched::kTileKeys, TKF = sched::kFewTileKeys, KV_ST = 5, SLOTS = 2, ITEMS = 4, DIRTY = 8;
 constexpr int P_COL = 80;  // P's columns in tensor memory, behind S's (two bf16 a column): 80 + 40 of the slot's first 128
 constexpr int SUB = 128 * 64 * 2;  // one [128 rows][64] bf16 swizzled sub-tile
 constexpr int TILE = 2 * SUB;      // [128 rows][128]
@@ -61,6 +61,7 @@ struct Item {
     int kvh, pos0;      // KV head; position of its first token
     int kb, ke;
     int npages, dest;   // pages of the request; dest -1: the whole item, else the partial slot 0 or 1
+    int dirty, pad;     // its tiles from this one on are not seen whole by some row
     int64_t table;      // the request's first page-table entry
 };
 
@@ -74,7 +75,6 @@ struct alignas(16) Record {
 // S = Q K^T and then O += P V of product m - lag. Wide: products 2t and 2t + 1 are tile t's two slots, and lag is 3; else
 // product t is tile t, in slot t & 1, and lag is 2. So K_t comes before V_{t - lead + 1}, lead being 2 or 3.
 __device__ __forceinline__ int products_lag(bool wide) { return wide ? 3 : 2; }
-__device__ __forceinline__ int ring_of_v(int t, int nt, bool wide) { return min(nt, t + (wide ? 2 : 3)) + t; }
 
 // A value that is the same in all lanes, so that the compiler knows it is.
 __device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
@@ -88,6 +88,7 @@ struct Control {
     uint64_t kv_full[KV_ST], kv_empty[KV_ST];
     uint64_t s_full[SLOTS], s_free[SLOTS], p_full[SLOTS], o_done[SLOTS];  // a phase each product of the slot
     uint64_t item_full[ITEMS], item_empty[ITEMS];
+    uint64_t v_clean[DIRTY];  // dirty tile n's v is clean: barrier n % DIRTY
     int z[2][32], z_pad[8];  // the producers': z coordinates of a window of pages
     Item items[ITEMS];
     uint64_t warp_sum[kThreads / 32];
@@ -95,7 +96,7 @@ struct Control {
     Request start;
     int start_req;
     uint32_t tmem;
-    int poison[SLOTS][2];  // [slot][item parity]: the item (counted from 1) in which v of a visible key was zeroed
+    int poison[2];  // by item parity: the item (counted from 1) in which v of a visible key was zeroed
     union {
         float ml[SLOTS][128][2];  // narrow: the slots' states
         struct {                  // few
@@ -117,7 +118,7 @@ struct Params {
     sched::Shape shape;
     int group, tt, rows_cap;  // query heads a KV head; tokens a slot; rows of a partial slot
     int few_tok;              // tokens of a few-row item's q box
-    int inv_group;            // ceil(2^16 / group): r * inv_group >> 16 = r / group for r < 128
+    int inv_group;            // ceil(2^16 / group): r * inv_group >> 16 = r / group for r < 256
     float *part_o, *part_ml;
     Record *records;
 };
@@ -192,36 +193,37 @@ __device__ __forceinline__ Request load_request(const PagedAttnArgs &a, int r, b
     return check_request(a, fetch_request(a, r), report);
 }
 
-// Tests v in this warp's quarter of a tile (32 keys, one a lane) and zeroes what is not finite. Keys up to
-// `last_seen` (relative to the tile) are seen by some row: if one of them is hit, `poison` is set.
-__device__ __forceinline__ void clean_v(uint8_t *tile, int key, int lane, int last_seen, volatile int *poison, int id) {
-    const uint32_t row = ptx::smem_u32(tile) + key * 128;
-    __nv_bfloat162 acc[4];
+// Tests v of keys [from, to) of a tile, one a lane of a warp, and zeroes what is not finite. Keys up to `last_seen` are seen
+// by some row: if one of them is hit, `poison` is set.
+__device__ __forceinline__ void clean_v(uint8_t *tile, int from, int to, int lane, int last_seen, volatile int *poison,
+                                        int id) {
     const __nv_bfloat162 zero = __floats2bfloat162_rn(0.f, 0.f);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc[e] = zero;
-#pragma unroll 4
-    for (int i = 0; i < 16; ++i) {  // 16-byte chunks in an order that differs by lane: no bank conflicts
-        const uint4 v = ptx::ld_shared_v4(row + (i >> 3) * SUB + (((i + lane) & 7) << 4));
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e)  // 0 * v + acc: NaN once v is infinite or NaN
-            acc[e] = __hfma2(*reinterpret_cast<const __nv_bfloat162 *>(&w[e]), zero, acc[e]);
-    }
-    const float2 f = __bfloat1622float2(__hadd2(__hadd2(acc[0], acc[1]), __hadd2(acc[2], acc[3])));
-    if (f.x != f.x || f.y != f.y) {
-        if (key <= last_seen) {
-            *poison = id;
-            __threadfence_block();  // seen before the zeros below are (the other warpgroup may find only those)
-        }
 #pragma unroll 1
-        for (int i = 0; i < 64; ++i) {
-            const uint32_t at = row + (i >> 5) * SUB + (i & 31) * 4;
-            uint32_t w;
-            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(at) : "memory");
-            if (!finite_bf16(w)) w &= 0xFFFF0000u;
-            if (!finite_bf16(w >> 16)) w &= 0x0000FFFFu;
-            asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(w) : "memory");
+    for (int key = from + lane; key < to; key += 32) {
+        const uint32_t row = ptx::smem_u32(tile) + key * 128;
+        __nv_bfloat162 acc[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] = zero;
+#pragma unroll 4
+        for (int i = 0; i < 16; ++i) {  // 16-byte chunks in an order that differs by lane: no bank conflicts
+            const uint4 v = ptx::ld_shared_v4(row + (i >> 3) * SUB + (((i + lane) & 7) << 4));
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)  // 0 * v + acc: NaN once v is infinite or NaN
+                acc[e] = __hfma2(*reinterpret_cast<const __nv_bfloat162 *>(&w[e]), zero, acc[e]);
+        }
+        const float2 f = __bfloat1622float2(__hadd2(__hadd2(acc[0], acc[1]), __hadd2(acc[2], acc[3])));
+        if (f.x != f.x || f.y != f.y) {
+            if (key <= last_seen) *poison = id;
+#pragma unroll 1
+            for (int i = 0; i < 64; ++i) {
+                const uint32_t at = row + (i >> 5) * SUB + (i & 31) * 4;
+                uint32_t w;
+                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(at) : "memory");
+                if (!finite_bf16(w)) w &= 0xFFFF0000u;
+                if (!finite_bf16(w >> 16)) w &= 0x0000FFFFu;
+                asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(w) : "memory");
+            }
         }
     }
     ptx::fence_proxy_async();  // the tensor core reads the tile through the async proxy
@@ -289,9 +291,9 @@ __device__ __forceinline__ void quad_transpose(uint4 (&v)[4], int lane) {
 struct RoleState {
     Control *c;
     const Params *p;
-    uint8_t *kv, *pt;  // K/V ring; this slot's P
+    uint8_t *pt;  // this slot's P
     uint32_t tmem;
-    int s, quarter, lane, cta, k, ring;
+    int s, quarter, lane, cta, k;
 };
 
 __device__ __forceinline__ bool barrier_or(int id, int count, bool x) {
@@ -455,13 +457,7 @@ __device__ __forceinline__ bool few_item(const RoleState &r, const Item &it, uin
         ptx::tc_fence_before();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(&c.s_free[s]);
-        if (dirty) {
-            const int xv = r.ring + ring_of_v(j, nt, false);
-            if (!wait_bar(&c.kv_full[xv % KV_ST], (xv / KV_ST) & 1, a.err, kErrWaitSoftmax)) return false;
-            clean_v(r.kv + (xv % KV_ST) * TILE, key, lane, it.pos0 + it.ntok - 1 - key0, &c.poison[s][r.k & 1], r.k + 1);
-        } else {
-            ptx::fence_proxy_async();  // P is read through the async proxy
-        }
+        ptx::fence_proxy_async();  // P is read through the async proxy
         ptx::tmem_st_wait();
         ptx::tc_fence_before();
         __syncwarp();
@@ -476,7 +472,7 @@ __device__ __forceinline__ bool few_item(const RoleState &r, const Item &it, uin
     if (ok && nt > 1 - s) ok = wait_bar(&c.o_done[1 - s], (done[1 - s] - 1) & 1, a.err, kErrWaitSoftmax);
     if (!ok) return false;
     ptx::tc_fence_after();
-    if (c.poison[0][r.k & 1] == r.k + 1 || c.poison[1][r.k & 1] == r.k + 1) {
+    if (c.poison[r.k & 1] == r.k + 1) {
         if (nt > s)
 #pragma unroll 1
             for (int e = 0; e < rows; ++e) {
@@ -484,7 +480,7 @@ __device__ __forceinline__ bool few_item(const RoleState &r, const Item &it, uin
                 asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(o) : "r"(tO + e));
                 ptx::tmem_ld_wait();
                 o = __float_as_uint(__uint_as_float(o) +
-                                    poison_sum(a, it.table, it.kvh, max(it.kb * TKF, it.pos0 / TKF * TKF),
+                                    poison_sum(a, it.table, it.kvh, max(it.kb * TKF, it.pos0 + 1),
                                                min(it.pos0 + (e * r.p->inv_group >> 16), it.ke * TKF - 1), TKF, it.kb + s, 2, key));
                 asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(tO + e), "r"(o) : "memory");
             }
@@ -613,8 +609,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 ptx::mbar_init(&c.s_free[s], 4);
                 ptx::mbar_init(&c.p_full[s], 4);
                 ptx::mbar_init(&c.o_done[s], 1);
-                c.poison[s][0] = c.poison[s][1] = 0;
             }
+            c.poison[0] = c.poison[1] = 0;
+            for (int s = 0; s < DIRTY; ++s) ptx::mbar_init(&c.v_clean[s], 1);
             for (int s = 0; s < ITEMS; ++s) {
                 ptx::mbar_init(&c.item_full[s], 1);
                 ptx::mbar_init(&c.item_empty[s], 11);  // two producers, the issuer, eight softmax warps
@@ -712,6 +709,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                         it.kvh = h;
                         it.pos0 = q.kv - q.n + i * span;
                         it.npages = (q.kv + kPageTokens - 1) / kPageTokens;
+                        const int tk = cost.tile == sched::kFew.tile ? TKF : TK;
+                        it.dirty = max(0, (int)((uint32_t)(it.pos0 + 1) / (uint32_t)tk) - it.kb);
                         it.dest = it.kb == 0 && it.ke == cost.tiles ? -1 : (it.kb == 0 ? 1 : 0);
                     }
                     if (it.ke > it.kb || left == 0) {  // a share of the item's own cost alone has no tiles
@@ -752,6 +751,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int kv = warp == 3;
             const int oob = a.kv_pages * a.kv_heads * 2;  // past the tensor map: read as zeros, without a memory access
             int ring = 0, q_free = 0;  // ring items of the items before this one; items known to be through with q
+            int cleaned = 0;           // dirty tiles so far
             bool few_before = false;
             for (int k = 0;; ++k) {
                 bool ok = wait_bar(&c.item_full[k % ITEMS], (k / ITEMS) & 1, err, kErrWaitProducer);
@@ -760,6 +760,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int tok0 = uniform(item.tok0), ntok = uniform(item.ntok), kvh = uniform(item.kvh);
                 const int kb = uniform(item.kb), nt = uniform(item.ke) - kb, npages = uniform(item.npages);
                 const int32_t *pages = a.page_table + item.table;
+                const int pos0 = item.pos0, item_dirty = item.dirty;
                 __syncwarp();
                 if (lane == 0) ptx::mbar_arrive(&c.item_empty[k % ITEMS]);
                 if (ntok == 0) break;
@@ -804,48 +805,68 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     __syncwarp();
                 }
-                const int lead = wide ? 2 : 3;
+                const int lead = wide ? 2 : 3, dirty = kv ? uniform(item_dirty) : nt;
+                // Dirty tile j's keys that the first token does not see. (Those past the request's pages are zeros.)
+                auto clean = [&](int j) {
+                    const int x = ring + j + min(nt, j + lead), key0 = (kb + j) * tile_pages * kPageTokens;
+                    if (!wait_bar(&c.kv_full[x % KV_ST], (x / KV_ST) & 1, err, kErrWaitProducer)) ok = false;
+                    clean_v(sKV + (x % KV_ST) * TILE, max(0, pos0 + 1 - key0),
+                            min(tile_pages * kPageTokens, npages * kPageTokens - key0), lane, pos0 + ntok - 1 - key0,
+                            &c.poison[k & 1], k + 1);
+                    __syncwarp();
+                    if (lane == 0) ptx::mbar_arrive(&c.v_clean[cleaned % DIRTY]);
+                    ++cleaned;
+                };
 #pragma unroll 1
                 for (int t0 = 0; t0 < nt; t0 += window) {
                     c.z[kv][lane] = place(t0, id);
                     __syncwarp();
                     if (t0 + window < nt) id = fetch(t0 + window);
-                    // One lane issues a window's copies (the choice of it and the return from it cost some 170 cycles).
-                    if (ptx::elect_one()) {
-                        const int t1 = min(nt, t0 + window);
-                        const int *zt = c.z[kv];
+                    const int t_end = min(nt, t0 + window);
+                    // Dirty tiles one by one, each followed by the cleaning of the one before: that one's copy is landing, and
+                    // no copy waits for a stage that only a product of it, or of the tile before it, would free.
 #pragma unroll 1
-                        for (int t = t0; t < t1; ++t, zt += tile_pages) {
-                            const int x = ring + t + (kv ? min(nt, t + lead) : max(0, t - lead + 1)), st = x % KV_ST;
-                            const uint32_t bar = ptx::smem_u32(&c.kv_full[st]), dst = ptx::smem_u32(sKV) + st * TILE;
-                            int zp[8];
+                    for (int ta = t0, t1; ta < t_end; ta = t1) {
+                        t1 = ta < dirty ? min(t_end, dirty) : ta + 1;
+                        // One lane issues the copies (the choice of it and the return from it cost some 170 cycles).
+                        if (ptx::elect_one()) {
+                            const int *zt = c.z[kv] + (ta - t0) * tile_pages;
+#pragma unroll 1
+                            for (int t = ta; t < t1; ++t, zt += tile_pages) {
+                                const int x = ring + t + (kv ? min(nt, t + lead) : max(0, t - lead + 1)), st = x % KV_ST;
+                                const uint32_t bar = ptx::smem_u32(&c.kv_full[st]), dst = ptx::smem_u32(sKV) + st * TILE;
+                                int zp[8];
 #pragma unroll
-                            for (int u = 0; u < 8; ++u) zp[u] = zt[u];  // (the array behind z is read past a window's end)
-                            ok = wait_bar(&c.kv_empty[st], ((x / KV_ST) & 1) ^ 1, err, kErrWaitProducer);
-                            if (!ok) break;
-                            ptx::mbar_arrive_expect_tx(&c.kv_full[st], tile_pages * 4096);
+                                for (int u = 0; u < 8; ++u) zp[u] = zt[u];  // (the array behind z is read past a window's end)
+                                ok = wait_bar(&c.kv_empty[st], ((x / KV_ST) & 1) ^ 1, err, kErrWaitProducer);
+                                if (!ok) break;
+                                ptx::mbar_arrive_expect_tx(&c.kv_full[st], tile_pages * 4096);
 #pragma unroll
-                            for (int u = 0; u < 5; ++u) {
-                                tma_3d(dst + u * 2048, &tkv, bar, 0, zp[u]);
-                                tma_3d(dst + SUB + u * 2048, &tkv, bar, 64, zp[u]);
-                            }
-                            if (few) {
-#pragma unroll
-                                for (int u = 5; u < 8; ++u) {
+                                for (int u = 0; u < 5; ++u) {
                                     tma_3d(dst + u * 2048, &tkv, bar, 0, zp[u]);
                                     tma_3d(dst + SUB + u * 2048, &tkv, bar, 64, zp[u]);
                                 }
+                                if (few) {
+#pragma unroll
+                                    for (int u = 5; u < 8; ++u) {
+                                        tma_3d(dst + u * 2048, &tkv, bar, 0, zp[u]);
+                                        tma_3d(dst + SUB + u * 2048, &tkv, bar, 64, zp[u]);
+                                    }
+                                }
+                            }
+                            // on the error path, the copies in flight must land before the CTA exits
+                            for (int y = ok ? t1 : 0; y < t1; ++y) {
+                                const int x = ring + y + (kv ? min(nt, y + lead) : max(0, y - lead + 1));
+                                wait_bar(&c.kv_full[x % KV_ST], (x / KV_ST) & 1, err, kErrWaitProducer);
                             }
                         }
-                        // on the error path, the copies in flight must land before the CTA exits
-                        for (int y = ok ? t1 : 0; y < t1; ++y) {
-                            const int x = ring + y + (kv ? min(nt, y + lead) : max(0, y - lead + 1));
-                            wait_bar(&c.kv_full[x % KV_ST], (x / KV_ST) & 1, err, kErrWaitProducer);
-                        }
+                        __syncwarp();
+                        if (__any_sync(0xffffffffu, !ok)) break;
+                        if (ta > dirty) clean(ta - 1);
                     }
-                    __syncwarp();
                     if (__any_sync(0xffffffffu, !ok)) break;
                 }
+                if (dirty < nt && __all_sync(0xffffffffu, ok)) clean(nt - 1);
                 if (__any_sync(0xffffffffu, !ok)) break;
                 ring += 2 * nt;
             }
@@ -860,11 +881,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             auto mnmajor = [](uint32_t at) { return (uint64_t)(kHi | 1024 >> 4) << 32 | ((uint32_t)(SUB >> 4) << 16 | at); };
             int ring = 0;                // ring items of the items before this one
             uint32_t before0 = 0, before1 = 0;  // products of the items before, a slot
+            uint32_t cleaned = 0;               // dirty tiles of the items before
             for (int k = 0;; ++k) {
                 bool ok = wait_bar(&c.item_full[k % ITEMS], (k / ITEMS) & 1, err, kErrWaitIssuer);
                 if (!__all_sync(0xffffffffu, ok)) break;
                 const int ntok = uniform(c.items[k % ITEMS].ntok);
                 const int nt = uniform(c.items[k % ITEMS].ke - c.items[k % ITEMS].kb);
+                const int dirty = uniform(c.items[k % ITEMS].dirty);
                 __syncwarp();
                 if (lane == 0) ptx::mbar_arrive(&c.item_empty[k % ITEMS]);
                 if (ntok == 0) break;
@@ -893,6 +916,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                             phase ^= 1;
                         }
                         return got ? x : -1;
+                    };
+                    auto wait_clean = [&](int t) {
+                        const uint32_t n = cleaned + (uint32_t)(t - dirty);
+                        return wait(ptx::smem_u32(&c.v_clean[n % DIRTY]), (n / DIRTY) & 1);
                     };
                     const uint32_t s_free = ptx::smem_u32(&c.s_free[0]), p_full = ptx::smem_u32(&c.p_full[0]);
                     wait(ptx::smem_u32(&c.q_full[k & 1]), (k >> 1) & 1);
@@ -940,6 +967,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 // O may be overwritten once the item before has been read out
                                 if (t == 1 && k > 0 && !wait(ptx::smem_u32(&c.o_free), (k - 1) & 1)) break;
                                 if (!wait(p_full, (par0 ^ t ^ 1) & 1)) break;
+                                if (t > dirty && !wait_clean(t - 1)) break;
                                 const uint32_t v = bKV + vt * (TILE >> 4), keep = t > 1 ? 1u : 0u;
 #pragma unroll
                                 for (int kk = 0; kk < TK / 16; ++kk)
@@ -980,6 +1008,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 if ((vt = next_tile()) < 0) break;
                                 if (m == 2 && k > 0 && !wait(ptx::smem_u32(&c.o_free), (k - 1) & 1)) break;
                                 if (!wait(p_full + 8 * s, (prod - 1) & 1)) break;
+                                if (m - 2 >= dirty && !wait_clean(m - 2)) break;
                                 const uint32_t v = bKV + vt * (TILE >> 4), keep = m >= 4 ? 1u : 0u;
                                 if (few) {
                                     const uint32_t pt = bQ + ((TILE + s * 2 * FEW_SUB) >> 4);
@@ -1005,6 +1034,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 ring += 2 * nt;
                 before0 += (count + 1) / 2;
                 before1 += count / 2;
+                cleaned += (uint32_t)max(0, nt - dirty);
             }
             // No MMA may still be writing TMEM when it is freed (this matters on the error path).
             if (ptx::elect_one()) ptx::mma_commit(&c.fin);
@@ -1021,7 +1051,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         const uint32_t tS = tmem + 256 * s + lanes;
         const float sc = a.scale_log2;
-        int ring = 0;
         uint32_t steps = 0, done[SLOTS] = {};  // products of this slot so far; products of the items before, a slot
         bool ok = true, narrow_before = false;
         for (int k = 0; ok; ++k) {
@@ -1031,12 +1060,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (lane == 0) ptx::mbar_arrive(&c.item_empty[k % ITEMS]);
             if (it.ntok == 0) break;
             if (it.ntok * p.group <= kFewRows) {
-                const RoleState r = {&c, &p, sKV, sQ + TILE + s * 2 * FEW_SUB, tmem, s, quarter, lane, cta, k, ring};
+                const RoleState r = {&c, &p, sQ + TILE + s * 2 * FEW_SUB, tmem, s, quarter, lane, cta, k};
                 // the sums of p go where a narrow item's O is: both warpgroups have read that out behind this
                 if (narrow_before) ptx::named_barrier(1, 256);
                 narrow_before = false;
                 ok = few_item(r, it, steps, done);
-                ring += 2 * (it.ke - it.kb);
                 if (!ok) break;
                 continue;
             }
@@ -1057,7 +1085,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 ptx::tc_fence_after();
                 const int key0 = (it.kb + j) * TK;
-                const bool dirty = key0 + TK - 1 > it.pos0;  // some row of the item does not see the whole tile
                 float x[TK];
                 if (active) {
                     ptx::tmem_ld32(tS, reinterpret_cast<uint32_t *>(x));
@@ -1138,23 +1165,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tmem_st8(tS + P_COL + 32, *reinterpret_cast<const float(*)[8]>(pk + 32));
                 }
                 first = false;
-                if (dirty) {
-                    const int xv = ring + ring_of_v(j, nt, wide);
-                    if (!wait_bar(&c.kv_full[xv % KV_ST], (xv / KV_ST) & 1, err, kErrWaitSoftmax)) {
-                        ok = false;
-                        break;
-                    }
-                    // (wide: the other slot's product of this tile is issued behind this one's)
-                    if (rl < TK && !(wide && s == 1))
-                        clean_v(sKV + (xv % KV_ST) * TILE, rl, lane, it.pos0 + it.ntok - 1 - key0, &c.poison[s][k & 1], k + 1);
-                }
                 if (active) ptx::tmem_st_wait();
                 ptx::tc_fence_before();
                 __syncwarp();
                 if (lane == 0) ptx::mbar_arrive(&c.p_full[s]);
             }
             if (!ok) break;
-            ring += 2 * nt;
 
             // ---- epilogue ----
             const bool used1 = wide || nt > 1;
@@ -1182,13 +1198,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                 l = (l0 == 0.f ? 0.f : w[0] * l0) + (l1 == 0.f ? 0.f : w[1] * l1);
                 ptx::named_barrier(1, 256);  // read by both before either may write there again
             }
-            const bool poisoned = c.poison[0][k & 1] == k + 1 || c.poison[1][k & 1] == k + 1;
+            const bool poisoned = c.poison[k & 1] == k + 1;
             if (active) {
                 // o = w[0] O_0 + w[1] O_1 (wide: this slot's O alone), 32 dims at a time
                 const uint32_t tO = (wide ? tS : tmem + lanes) + 128;
                 const bool two = !wide && used1;
                 if (poisoned) {
-                    const int lo = max(it.kb * TK, it.pos0 / TK * TK);
+                    const int lo = max(it.kb * TK, it.pos0 + 1);
                     const int hi = valid ? min(it.pos0 + token, it.ke * TK - 1) : -1;
                     if (wide || nt > s)
                         add_poison(a, it.table, it.kvh, lo, hi, TK, it.kb + (wide ? 0 : s), wide ? 1 : 2, tS + 128);
@@ -1267,17 +1283,22 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // Merges the partial results of the items that a cut passes through: o = sum 2^(m_i - m) o_i / sum 2^(m_i - m) l_i in the
-// order of their keys. Block (CTA, 32 of its rows), a warp four rows at a time, 4 dims a lane. It is bound by latency, and
-// two parts (a cut or two) are nearly all there is, so the loads of two parts of the four rows are issued together.
-constexpr int kCombineWarps = 8, kCombineAtOnce = 4, kCombineRows = kCombineWarps * kCombineAtOnce;
-__global__ void __launch_bounds__(32 * kCombineWarps) paged_combine_kernel(const __grid_constant__ Params p) {
+// order of their keys. It is bound by latency, its instructions' fetch included. Block (CTA, part of its record's rows), a
+// warp two rows at a time, 4 dims a lane; two parts (a cut or two) are nearly all there is, so the loads of two parts of
+// both rows are issued together. A block has 16 rows, which leaves four blocks an SM. (8 chunks of 511 tokens among 56 decodes
+// and 26 requests with chunks of up to 250: 61.2 and 19.2 us with the attention; with a block for 32 rows, two an SM, 62.9
+// and 20.6; with four blocks a record that loop over its rows, one wave, 63.8 and 23.9; with all records' rows dealt to the
+// warps of one wave by a search 63.4 and 20.0, but one row over 900 keys takes 13.1 for 11.5.)
+constexpr int kCombineWarps = 8, kCombineAtOnce = 2, kCombineRows = kCombineWarps * kCombineAtOnce;
+__global__ void __launch_bounds__(32 * kCombineWarps, 4)
+    paged_combine_kernel(const __grid_constant__ Params p) {
     ptx::griddep_wait();
     const int4 rec = *reinterpret_cast<const int4 *>(p.records + blockIdx.x);  // tok0, ntok, kvh, follow
     const int lane = threadIdx.x % 32, n = rec.w + 1, rows = rec.y * p.group;
-    const int row0 = blockIdx.y * kCombineRows + threadIdx.x / 32;
-    if (row0 >= rows) return;
     // partial i: slot 1 of the record's CTA, then slot 0 of each CTA behind it
     const size_t first = ((size_t)blockIdx.x * 2 + 1) * p.rows_cap, step = (size_t)2 * p.rows_cap;
+    const int row0 = blockIdx.y * kCombineRows + threadIdx.x / 32;
+    if (row0 >= rows) return;
     float m[kCombineAtOnce], l[kCombineAtOnce];
     float4 acc[kCombineAtOnce];
 #pragma unroll
@@ -1324,7 +1345,7 @@ __global__ void __launch_bounds__(32 * kCombineWarps) paged_combine_kernel(const
         const int row = row0 + r * kCombineWarps;
         if (row >= rows) break;
         const float inv = 1.f / l[r];
-        const int token = row / p.group, h = row - token * p.group;
+        const int token = row * p.inv_group >> 16, h = row - token * p.group;
         *reinterpret_cast<uint2 *>(p.a.out + (size_t)(rec.x + token) * p.a.ld_out +
                                    (size_t)(rec.z * p.group + h) * kHeadDim + 4 * lane) =
             make_uint2(pack2(acc[r].x * inv, acc[r].y * inv), pack2(acc[r].z * inv, acc[r].w * inv));
