@@ -41,13 +41,13 @@ LRM_HD Shape make_shape(int group) {
 LRM_HD int items_of(const Shape &s, int n) { return (int)(((uint64_t)(uint32_t)(n + s.span - 1) * s.inv_span) >> 38); }
 
 // An item's units: `own` for its start and end, then `tile` a tile. A unit is about 300 cycles. Alone, items of few rows
-// take 4,000 cycles + 1,400 a tile, of one slot's rows 6,700 + 1,400, of two slots' 13,300 + 1,950; beside items of few
-// rows, whose loads fill the memory's queues, those of two slots wait for their tiles: 8,800 + 2,800. The weights lie in
-// between (8 chunks of 511 tokens among 56 single ones: 65.7 us, 68.8 with 32 + 7 units, 70.1 with 46 + 11).
+// take 4,000 cycles + 1,400 a tile, of one slot's rows 6,700 + 1,400, of two slots' 9,000 + 1,950; where the memory's queues
+// are full, as in most mixtures, tiles take longer and part of `own` hides behind them. The weights are from mixtures (8
+// chunks of 511 tokens among 56 single ones: 56 us, 61 with 13 + 5 for few rows and 40 + 10 for two slots').
 struct Cost {
     int own, tile;
 };
-constexpr Cost kFew = {13, 5}, kNarrow = {22, 6}, kWide = {40, 10};
+constexpr Cost kFew = {13, 6}, kNarrow = {22, 7}, kWide = {30, 10};
 
 // Units of the items before item i of a head: all of them are whole spans, and so of two slots' rows.
 LRM_HD uint64_t units_before(const Shape &s, int n, int kv, int i) {
