@@ -83,6 +83,18 @@ __device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, 
 struct Request {
     int start, n, kv, slot;
 };
+
+// A walk over a CTA's range from its last item to its first: item i of `items` of request r's KV head h, and the share's end
+// in it, in units; units of the range that are left.
+struct Walk {
+    Request q;
+    sched::Item cost;
+    int r, h, i, items, end;
+    int pushed;  // items handed out so far
+    uint64_t left;
+    Record rec;
+};
+
 struct Control {
     uint64_t q_full[2], q_empty[2], fin, o_free;  // q: even and odd items
     uint64_t kv_full[KV_ST], kv_empty[KV_ST];
@@ -92,9 +104,8 @@ struct Control {
     int z[2][32], z_pad[8];  // the producers': z coordinates of a window of pages
     Item items[ITEMS];
     uint64_t warp_sum[kThreads / 32];
-    uint64_t start_off, start_head;  // the range's last unit within its request, and that request's units a head
-    Request start;
-    int start_req;
+    uint64_t started;
+    Walk walk;  // of the scheduler, behind the range's last item
     uint32_t tmem;
     int poison[2];  // by item parity: the item (counted from 1) in which v of a visible key was zeroed
     union {
@@ -564,6 +575,29 @@ __device__ __forceinline__ bool few_item(const RoleState &r, const Item &it, uin
     return true;
 }
 
+// The share of the walk's item that lies in the range, taken off its units.
+__device__ __forceinline__ Item take_share(const Params &p, const sched::Cut &cut, uint64_t u1, int cta, Walk &w) {
+    Item it;
+    const int begin = (uint64_t)w.end > w.left ? w.end - (int)w.left : 0, span = SLOTS * p.tt;
+    const int tk = w.cost.tile == sched::kFew.tile ? TKF : TK;
+    it.kb = sched::tile_at(w.cost, begin);
+    it.ke = sched::tile_at(w.cost, w.end);
+    it.table = (int64_t)w.q.slot * p.a.pages_per_seq;
+    if (it.ke > it.kb)  // the producers' first load of page ids would miss otherwise
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(p.a.page_table + it.table + it.kb * (tk / kPageTokens)));
+    it.tok0 = w.q.start + w.i * span;
+    it.ntok = min(span, w.q.n - w.i * span);
+    it.kvh = w.h;
+    it.pos0 = w.q.kv - w.q.n + w.i * span;
+    it.npages = (w.q.kv + kPageTokens - 1) / kPageTokens;
+    it.dirty = max(0, (tk == TK ? (it.pos0 + 1) / TK : (it.pos0 + 1) / TKF) - it.kb);
+    it.dest = it.kb == 0 && it.ke == w.cost.tiles ? -1 : (it.kb == 0 ? 1 : 0);
+    if (it.dest == 1 && it.ke > it.kb)  // the range's last item, begun here: the rest of it lies behind the range
+        w.rec = Record{it.tok0, it.ntok, w.h, sched::cta_of(cut, u1 - 1 + (uint64_t)(w.cost.units - w.end)) - cta};
+    w.left -= (uint64_t)(w.end - begin);
+    return it;
+}
+
 __global__ void __launch_bounds__(kThreads, 1)
     paged_attn_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tq_few,
                       const __grid_constant__ CUtensorMap tkv, const __grid_constant__ Params p) {
@@ -577,7 +611,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t *err = a.err;
     // (the shuffle tells the compiler that the warp index, and so the role, is the same in all lanes)
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid / 32, 0), lane = tid % 32;
-    const int cta = blockIdx.x, span = SLOTS * p.tt;
+    const int cta = blockIdx.x;
     const sched::Shape &shape = p.shape;
     // This thread's requests, `per` of them. The first one's lengths are on their way while the CTA sets itself up.
     const int per = a.requests <= kThreads ? 1 : (a.requests + kThreads - 1) / kThreads;
@@ -599,6 +633,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             ptx::mbar_init(&c.q_empty[0], 1);
             ptx::mbar_init(&c.q_empty[1], 1);
             ptx::mbar_init(&c.fin, 1);
+            ptx::mbar_init(&c.started, 1);
             ptx::mbar_init(&c.o_free, 8);
             for (int s = 0; s < KV_ST; ++s) {
                 ptx::mbar_init(&c.kv_full[s], 1);
@@ -658,21 +693,36 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool idle = cta >= cut.ctas;
     const uint64_t u0 = sched::begin(cut, cta), u1 = sched::begin(cut, cta + 1);
     if (!idle && before <= u1 - 1 && u1 - 1 < before + own) {
-        int r = r0;
-        uint64_t at = before, w = head * (uint64_t)a.kv_heads;  // units before request r, and of it
+        // The thread whose requests hold the range's last unit hands out that item, so that the rest can begin.
+        Walk w;
+        w.r = r0;
+        uint64_t at = before, sum = head * (uint64_t)a.kv_heads;  // units before request r, and of it
 #pragma unroll 1
-        while (u1 - 1 >= at + w) {
-            at += w;
-            mine = load_request(a, ++r, false);
+        while (u1 - 1 >= at + sum) {
+            at += sum;
+            mine = load_request(a, ++w.r, false);
             head = mine.n ? sched::head_units(shape, mine.n, mine.kv) : 0;
-            w = head * (uint64_t)a.kv_heads;
+            sum = head * (uint64_t)a.kv_heads;
         }
-        c.start_req = r;
-        c.start_off = u1 - 1 - at;
-        c.start_head = head;
-        c.start = mine;
+        w.q = mine;
+        w.h = (int)sched::quotient(u1 - 1 - at, head);
+        const uint64_t off = u1 - 1 - at - (uint64_t)w.h * head;
+        w.items = sched::items_of(shape, mine.n);
+        w.i = sched::item_at(shape, mine.n, mine.kv, off, w.items);
+        w.cost = sched::item_of(shape, mine.n, mine.kv, w.i, w.items);
+        w.end = (int)(off - sched::units_before(shape, mine.n, mine.kv, w.i)) + 1;
+        w.left = u1 - u0;
+        w.rec = Record{0, 0, 0, 0};
+        const Item it = take_share(p, cut, u1, cta, w);
+        w.pushed = it.ke > it.kb;  // a share of the item's own cost alone has no tiles
+        if (w.pushed) {
+            c.items[0] = it;
+            ptx::mbar_arrive(&c.item_full[0]);
+        }
+        c.walk = w;
+        ptx::mbar_arrive(&c.started);
     }
-    __syncthreads();
+    __syncwarp();
 
     if (idle) {
         if (tid == 0) p.records[cta] = Record{0, 0, 0, 0};
@@ -681,68 +731,38 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (warp == 2) {
             // ---- scheduler ----
             if (lane == 0) {
-                int r = c.start_req;
-                Request q = c.start;
-                uint64_t left = u1 - u0;
-                int h = (int)sched::quotient(c.start_off, c.start_head);
-                const uint64_t off = c.start_off - (uint64_t)h * c.start_head;
-                int items = sched::items_of(shape, q.n);
-                int i = sched::item_at(shape, q.n, q.kv, off, items);
-                sched::Item cost = sched::item_of(shape, q.n, q.kv, i, items);
-                // the share's end within the item, in units
-                int end = (int)(off - sched::units_before(shape, q.n, q.kv, i)) + 1;
-                Record rec = {0, 0, 0, 0};
-                int k = 0;
-                for (;;) {
+                bool ok = wait_bar(&c.started, 0, err, kErrWaitScheduler);
+                Walk w = c.walk;
+                while (ok) {
                     Item it = {};
-                    int begin = 0;
-                    if (left > 0) {
-                        begin = (uint64_t)end > left ? end - (int)left : 0;
-                        it.kb = sched::tile_at(cost, begin);
-                        it.ke = sched::tile_at(cost, end);
-                        it.table = (int64_t)q.slot * a.pages_per_seq;
-                        if (it.ke > it.kb)  // the producers' first load of page ids would miss otherwise
-                            asm volatile("prefetch.global.L2 [%0];" ::"l"(a.page_table + it.table +
-                                                                          it.kb * (cost.tile == sched::kFew.tile ? TKF : TK) / kPageTokens));
-                        it.tok0 = q.start + i * span;
-                        it.ntok = min(span, q.n - i * span);
-                        it.kvh = h;
-                        it.pos0 = q.kv - q.n + i * span;
-                        it.npages = (q.kv + kPageTokens - 1) / kPageTokens;
-                        const int tk = cost.tile == sched::kFew.tile ? TKF : TK;
-                        it.dirty = max(0, (int)((uint32_t)(it.pos0 + 1) / (uint32_t)tk) - it.kb);
-                        it.dest = it.kb == 0 && it.ke == cost.tiles ? -1 : (it.kb == 0 ? 1 : 0);
-                    }
-                    if (it.ke > it.kb || left == 0) {  // a share of the item's own cost alone has no tiles
-                        if (!wait_bar(&c.item_empty[k % ITEMS], ((k / ITEMS) & 1) ^ 1, err, kErrWaitScheduler)) break;
-                        c.items[k % ITEMS] = it;
-                        ptx::mbar_arrive(&c.item_full[k % ITEMS]);
-                        ++k;
-                        if (it.dest == 1)  // the range's last item, begun here: the rest of it lies behind the range
-                            rec = Record{it.tok0, it.ntok, h,
-                                         sched::cta_of(cut, u1 - 1 + (uint64_t)(cost.units - end)) - cta};
-                    }
-                    if (left == 0) break;
-                    left -= (uint64_t)(end - begin);
-                    if (left == 0) continue;
-                    // the item before: of this head, else of the head before, else of the request before
-                    if (i > 0) {
-                        --i;
-                    } else {
-                        if (h > 0) {
-                            --h;
+                    if (w.left > 0) {
+                        // the item before: of this head, else of the head before, else of the request before
+                        if (w.i > 0) {
+                            --w.i;
                         } else {
-                            do q = load_request(a, --r, false);
-                            while (!q.n);
-                            h = a.kv_heads - 1;
-                            items = sched::items_of(shape, q.n);
+                            if (w.h > 0) {
+                                --w.h;
+                            } else {
+                                do w.q = load_request(a, --w.r, false);
+                                while (!w.q.n);
+                                w.h = a.kv_heads - 1;
+                                w.items = sched::items_of(shape, w.q.n);
+                            }
+                            w.i = w.items - 1;
                         }
-                        i = items - 1;
+                        w.cost = sched::item_of(shape, w.q.n, w.q.kv, w.i, w.items);
+                        w.end = w.cost.units;
+                        it = take_share(p, cut, u1, cta, w);
+                        if (it.ke == it.kb) continue;
                     }
-                    cost = sched::item_of(shape, q.n, q.kv, i, items);
-                    end = cost.units;
+                    const int k = w.pushed++;
+                    ok = wait_bar(&c.item_empty[k % ITEMS], ((k / ITEMS) & 1) ^ 1, err, kErrWaitScheduler);
+                    if (!ok) break;
+                    c.items[k % ITEMS] = it;
+                    ptx::mbar_arrive(&c.item_full[k % ITEMS]);
+                    if (it.ntok == 0) break;  // the end
                 }
-                p.records[cta] = rec;
+                p.records[cta] = ok ? w.rec : Record{0, 0, 0, 0};
             }
         } else if (warp == 0 || warp == 3) {
             // ---- TMA producers: warp 0 q and the tiles of K, warp 3 those of V ----
