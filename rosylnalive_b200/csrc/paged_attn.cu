@@ -7,24 +7,40 @@
 // The work is cut evenly over one persistent CTA an SM (paged_sched.h): single tokens, verify chunks and prefill chunks
 // of any lengths fill the GPU alike. An item is up to 2 * floor(128 / group) tokens of one request and KV head. Its rows
 // are (token, query head) pairs, token-major, so the query heads that share a KV head share its tiles whatever the group
-// size, and one TMA box brings their q. 128 rows make a "slot" (S and O, 128 x 128 fp32 each, in tensor memory):
-//   wide    (more than 128 rows): each 128-key tile of K and V is used by both slots' rows;
-//   narrow  (up to 128 rows): one set of rows; the even key tiles go to slot 0 and the odd ones to slot 1, so one
-//           slot's products run under the other's softmax; the two states merge at the end.
+// size, and one TMA box brings their q. 128 rows make a "slot" with S, P and O in half of tensor memory:
+//   wide    (more than 128 rows): each tile of K and V is used by both slots' rows;
+//   narrow  (33 to 128 rows): one set of rows; the even key tiles go to slot 0 and the odd ones to slot 1, so one
+//           slot's products run under the other's softmax; the two states merge at the end;
+//   few     (up to 32 rows): as narrow, with keys and rows swapped (below).
+// Tiles of wide and narrow items have 80 keys: S (80 columns) and P (40, two bf16 a column) then lie side by side in the
+// 128 that O leaves of a slot, so the next S is computed while the softmax still works on this one. With 128 keys, P over
+// S, every S waited for the P V before it: 1,000 rows over 121,000 keys took 1.68 million cycles, with 80 keys 1.25.
 // Warps of a CTA:
 //   0, 3    TMA producers: q of an item and K's tiles, and V's tiles, in the order of their use through a ring of five
 //           32 KiB stages (5 or 8 pages of 16 tokens, one box a page and 64 dims), running ahead into the next item;
+//           warp 3 also cleans V;
 //   1       tensor-core issuer (one thread);
 //   2       scheduler: walks the CTA's range and hands the items to the others through a ring of four;
-//   4..11   softmax, one warpgroup a slot, thread = row.
+//   4..11   softmax, one warpgroup a slot, thread = row (few: thread = key).
 // Keys that a row does not see: their scores are replaced before the maximum, and their v, which the product multiplies
-// by 0, must not be infinite or NaN. So in tiles where some row's mask bites (the last tokens' own tiles) the softmax
-// warps test v in shared memory and zero what is not finite; if a key of the request itself was hit, the epilogue adds
-// its original values to the rows that see it.
+// by 0, must not be infinite or NaN. So in tiles where some row's mask bites (the last tokens' own tiles, "dirty") warp 3
+// tests v of the keys that not all rows see, and zeroes what is not finite; if a key of the request itself was hit, the
+// epilogue adds its original values to the rows that see it.
 // Items that a cut passes through leave (m, sum p, unnormalised o) in the workspace, at most two a CTA, and
 // paged_combine_kernel merges them. Within a range the last item is walked first: CTAs that share a head's keys then
 // all start at key 0 of an item and stream the same tiles at about the same time, from L2.
 // Every wait is bounded and reports to the error word.
+//
+// What bounds it and what it measured (device time, both kernels; 8 KV heads, two query heads each unless said):
+//   HBM       64 single tokens over 4096 to 4352 keys: 171 us, 6.48 TB/s, 0.99 of a copy's rate.
+//   HBM and the start: 32 x 5 tokens over 100 to 6000 keys, 32 query heads: 39.7 us, 4.3 TB/s. 3.5 us pass before the first
+//             load (the lengths' and page table's loads, the cut, and code that no CTA has fetched yet), 4 after the last.
+//   softmax and power: 1,000 tokens over 121,000 keys: 1.25 million cycles, tensor pipe active in 67 percent of them, the
+//             exponentials' unit in 67; 820 us at the 1.53 GHz that 1000 W allow, 1 PFLOP/s over seconds.
+//   the same and what an item costs beside its tiles (9,000 cycles of 36,000): 16 x 2048 tokens without a past 311 us.
+//   latency   one token over 900 keys: 10.7 us.
+// Tried and slower: two issuing warps (their MMAs interleave badly); four softmax warpgroups (spills); a part of the
+// exponentials as polynomials on the FMA pipes (the warps' issue is as full as that unit).
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -71,10 +87,10 @@ struct alignas(16) Record {
     int tok0, ntok, kvh, follow;
 };
 
-// The ring order of an item's tiles is the order in which the issuer first uses them. Step m of an item issues product m's
-// S = Q K^T and then O += P V of product m - lag. Wide: products 2t and 2t + 1 are tile t's two slots, and lag is 3; else
-// product t is tile t, in slot t & 1, and lag is 2. So K_t comes before V_{t - lead + 1}, lead being 2 or 3.
-__device__ __forceinline__ int products_lag(bool wide) { return wide ? 3 : 2; }
+// The ring order of an item's tiles is the order in which the issuer first uses them. In step t it issues S = Q K^T of tile t
+// (wide: for both slots) and O += P V of an earlier one. Wide: S of slot 0, P V of slot 1 and tile t - 2, S of slot 1, P V of
+// slot 0 and tile t - 1; else tile t is slot t & 1's, and P V is of tile t - 2. So K_t comes before V_{t - lead + 1}, lead
+// being 2 (wide) or 3, and V_t is ring item t + min(nt, t + lead) of an item of nt tiles.
 
 // A value that is the same in all lanes, so that the compiler knows it is.
 __device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
@@ -241,9 +257,10 @@ __device__ __forceinline__ void clean_v(uint8_t *tile, int from, int to, int lan
 }
 
 // Adds the values that clean_v zeroed to one slot's O (128 columns at `t`, this warp's lanes), from the cache: this
-// lane's row sees keys lo .. hi, of which the slot has those of tiles tile0, tile0 + step, ... Rare, so it is kept out of the kernel's instruction stream.
-__device__ __noinline__ void add_poison(const PagedAttnArgs &a, int64_t table, int kvh, int lo, int hi, int tk, int tile0, int step,
-                                        uint32_t t) {
+// lane's row sees keys lo .. hi, of which the slot has those of tiles tile0, tile0 + step, ... Rare, so it is kept out of the
+// kernel's instruction stream.
+__device__ __noinline__ void add_poison(const PagedAttnArgs &a, int64_t table, int kvh, int lo, int hi, int tk, int tile0,
+                                        int step, uint32_t t) {
 #pragma unroll 1
     for (int c = 0; c < kHeadDim; c += 16) {
         uint32_t o[16];
@@ -297,8 +314,8 @@ __device__ __forceinline__ void quad_transpose(uint4 (&v)[4], int lane) {
 // row, and a thread holds one key's scores. The running maximum of a row is the same in all threads of a slot's
 // warpgroup and moves only when some score exceeds it by 2^8, which one barrier with an OR finds out; only then (and at
 // an item's first tile) are the tile's maxima reduced over threads. P goes to shared memory as the B operand of
-// O^T = V^T P^T; sums of p stay per thread until the end. A tile costs some 500 cycles beside its MMAs' 512, which hides
-// under the 2,600 that its K and V take from HBM.
+// O^T = V^T P^T; sums of p stay per thread until the end. A tile costs 1,400 cycles, which hide under the 2,800 that its K
+// and V take as one SM's share of HBM. (As narrow items, 32 x 5 drafted tokens took 64 us against 43.)
 struct RoleState {
     Control *c;
     const Params *p;
@@ -337,8 +354,8 @@ __device__ __forceinline__ void tmem_st8(uint32_t t, const float (&x)[8]) {
 
 // The sum of the values that clean_v zeroed in dim d of keys lo .. hi in tiles tile0, tile0 + step, ... (infinite or NaN, or
 // 0 if there are none).
-__device__ __noinline__ float poison_sum(const PagedAttnArgs &a, int64_t table, int kvh, int lo, int hi, int tk, int tile0, int step,
-                                         int d) {
+__device__ __noinline__ float poison_sum(const PagedAttnArgs &a, int64_t table, int kvh, int lo, int hi, int tk, int tile0,
+                                         int step, int d) {
     float sum = 0.f;
 #pragma unroll 1
     for (int key = lo; key <= hi; ++key) {
@@ -369,7 +386,8 @@ __device__ __forceinline__ void load_scores(uint32_t t, int from, float (&x)[8])
 // An item's tiles in one slot and its epilogue, eight rows at a time in rolled loops (code that the instruction cache
 // holds). Columns of the slot's tensor memory: S^T at 0, O^T at 128, the thread's sums of p at 192 (not beside S^T, which the
 // next item's first scores may overwrite while this item is still read out).
-__device__ __forceinline__ bool few_item(const RoleState &r, const Item &it, uint32_t &steps, uint32_t (&done)[SLOTS]) {  // done: products of the items before, a slot
+// done: products of the items before, a slot
+__device__ __forceinline__ bool few_item(const RoleState &r, const Item &it, uint32_t &steps, uint32_t (&done)[SLOTS]) {
     Control &c = *r.c;
     const PagedAttnArgs &a = r.p->a;
     const int s = r.s, lane = r.lane, group = r.p->group, nt = it.ke - it.kb, rows = it.ntok * group;
@@ -490,9 +508,9 @@ __device__ __forceinline__ bool few_item(const RoleState &r, const Item &it, uin
                 uint32_t o;
                 asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(o) : "r"(tO + e));
                 ptx::tmem_ld_wait();
-                o = __float_as_uint(__uint_as_float(o) +
-                                    poison_sum(a, it.table, it.kvh, max(it.kb * TKF, it.pos0 + 1),
-                                               min(it.pos0 + (e * r.p->inv_group >> 16), it.ke * TKF - 1), TKF, it.kb + s, 2, key));
+                const int last = min(it.pos0 + (e * r.p->inv_group >> 16), it.ke * TKF - 1);
+                o = __float_as_uint(__uint_as_float(o) + poison_sum(a, it.table, it.kvh, max(it.kb * TKF, it.pos0 + 1), last,
+                                                                    TKF, it.kb + s, 2, key));
                 asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(tO + e), "r"(o) : "memory");
             }
         ptx::tmem_st_wait();
@@ -917,7 +935,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const uint32_t idesc_s = ptx::idesc_bf16_f32(128, nrow), idesc_o = idesc_s | 1u << 15;  // A (V) MN-major
                 // Product n's slot is n & 1. S lies beside P, so the next S of a slot is computed as soon as its softmax
                 // has taken this one, and waits there for it; only P V waits for P.
-                const int count = wide ? 2 * nt : nt, lag = products_lag(wide);
+                const int count = wide ? 2 * nt : nt;
                 // One lane runs the item (choosing it and returning from it cost some 170 cycles); what the MMAs go by was
                 // made uniform above, so their descriptors stay in uniform registers.
                 if (ptx::elect_one()) {
@@ -1066,7 +1084,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int s = (warp - 4) >> 2;  // slot
         const int quarter = warp & 3;   // TMEM lanes this warp may access
         const int rl = quarter * 32 + lane;
-        const int tl = rl * p.inv_group >> 16, hl = rl - tl * p.group;  // this row's token (of the slot) and query head (of the group)
+        // this row's token (of the slot) and query head (of the group)
+        const int tl = rl * p.inv_group >> 16, hl = rl - tl * p.group;
         const int warp_tl = quarter * 32 * p.inv_group >> 16;  // the warp's first token
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         const uint32_t tS = tmem + 256 * s + lanes;
