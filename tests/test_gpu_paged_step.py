@@ -529,10 +529,25 @@ def test_values_that_are_not_finite_reach_only_the_rows_that_see_them(value, wha
         a = int(c.cu_host[i])
         sees = n if i not in first else max(0, first[i] - (kv - n))  # rows before the first such key
         assert torch.equal(got[a:a + sees], clean[a:a + sees]), i
-        if what == "k" and i in first and value != float("-inf") and value == value:
-            pass  # an infinite score: the sign of q decides between NaN and a key that weighs nothing
         if i in first and value != value:
             assert torch.isnan(got[a + sees:a + n].float()).any()
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("heads", [(16, 8), (6, 2), (40, 8)])
+def test_values_that_are_not_finite_in_many_short_requests(value, heads):
+    # Short requests follow one another closely in a CTA, so that the values of one are looked at while the results of the
+    # one before are still read out; all of them hold a value that only their later rows see.
+    r = np.random.default_rng(1)
+    new = r.choice([2, 3, 5, 17, 40, 70], 160).tolist()
+    c = Cache([(n, n + int(p)) for n, p in zip(new, r.choice([0, 1, 20, 90], 160))], *heads, seed=31)
+    own, slots = c.table.cpu().numpy(), c.slots.tolist()
+    for i, (n, kv) in enumerate(c.reqs):
+        key = kv - 1 - (n - 1) // 2
+        c.pool[int(own[slots[i], key // PAGE]), :, 1, key % PAGE, i % 16::16] = value
+        c.v[i][key, :, i % 16::16] = value
+    before = c.out.clone()
+    c.check(c.run(), before)
 
 
 def test_keys_of_minus_infinity_weigh_nothing():
