@@ -1448,11 +1448,15 @@ cudaError_t launch_paged_attention(const PagedAttnArgs &a, int sms, cudaStream_t
     p.few_tok = kFewRows / p.group > 0 ? kFewRows / p.group : 1;
     CUtensorMap tq, tq_few, tkv;
     const uint64_t qrow = (uint64_t)a.ld_q * 2;
-    if (!make_tmap(&tq, a.q, a.q_heads, a.tokens, kHeadDim * 2, qrow, p.group, p.tt) ||
-        !make_tmap(&tq_few, a.q, a.q_heads, a.tokens, kHeadDim * 2, qrow, p.group, p.few_tok) ||
+    // a map is made for the boxes that the call can use (each takes the host 0.4 us, a call of one token 11 in all)
+    const bool few = p.group <= kFewRows, more = (int64_t)a.tokens * p.group > kFewRows;
+    if ((more && !make_tmap(&tq, a.q, a.q_heads, a.tokens, kHeadDim * 2, qrow, p.group, p.tt)) ||
+        (few && !make_tmap(&tq_few, a.q, a.q_heads, a.tokens, kHeadDim * 2, qrow, p.group, p.few_tok)) ||
         !make_tmap(&tkv, a.pool, kPageTokens, (uint64_t)a.kv_pages * a.kv_heads * 2, kHeadDim * 2,
                    kPageTokens * kHeadDim * 2, kPageTokens, 1))
         return cudaErrorInvalidValue;
+    if (!more) tq = tq_few;
+    if (!few) tq_few = tq;
     static SmemOptIn opt;
     if (cudaError_t e = opt.set((const void *)paged_attn_kernel, SMEM_BYTES)) return e;
     cudaError_t e = launch_kernel(paged_attn_kernel, dim3(sms), dim3(kThreads), SMEM_BYTES, st, tq, tq_few, tkv, p);
