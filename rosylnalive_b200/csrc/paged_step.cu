@@ -29,14 +29,14 @@ namespace {
 // give back (release: ceil(len / 16) - ceil(keep / 16)). With exclusive sums N and C over the requests, token t of
 // request i is row N_i + t of the step and page j of request i is entry count - 1 - (C_i + j) of the free list (plan)
 // or count + C_i + j (release). So everything follows from one scan over the requests, and the rest is a binary search
-// and a few loads and stores, by one thread for four pages that are given back or for the tokens of a quad (rows 4k ..
+// and a few loads and stores, by one thread for two or four pages that are given back or for the tokens of a quad (rows 4k ..
 // 4k+3 of the step), whose stores are then 16 bytes: of a large step the number of stores is what counts (65536 tokens on
 // one CTA: 20 us, 44 with single words). A small one is bound by latency, the fetch of instructions included: loops
 // stay rolled where their loads do not have to overlap, and a single CTA takes its tokens one by one.
 //
 // One cluster does it all, each CTA a contiguous part of the requests (1024 a pass, their prefixes in shared memory):
 //   1. load and check the part, and sum it up; a bit a slot, kept by CTA slot % ranks, finds a slot listed twice;
-//   2. all sums are read over distributed shared memory: each CTA's first token and page, and whether the step is sound;
+//   2. each CTA writes its sums to all others' shared memory: its first token and page, and whether the step is sound;
 //   3. the page ids that change hands are checked; the CTAs agree on that too, before anything is written;
 //   4. write the part's outputs, tokens, pages and lengths.
 // A slot is listed once, so no CTA reads a length that another writes, and the new lengths may take the old ones' place;
@@ -233,16 +233,24 @@ __global__ void __launch_bounds__(kPlanThreads, 1) page_step_kernel(const __grid
     auto entry = [&](int r, uint32_t j) {  // of the page table, for page j of the call, which is request r's
         return (int64_t)s.slot[r] * a.pages_per_seq + s.held[r] + (int)(j - s.c0[r]);
     };
-    constexpr int kIds = kRelease ? 4 : 1;  // of a thread, in a row
+    // of a thread, in a row (releases: of 1500 requests 11.5 us, with 8 13.8; of 40 on one CTA 3.4, with 4 3.6, with 1 4.1)
+    constexpr int kIds = kRelease ? (kCluster ? 4 : 2) : 1;
     auto ids_of = [&](uint32_t j, uint32_t end, int(&id)[kIds]) {
         if (j >= end) return;
         if (kRelease) {
             int r = find_request(s.c0, j);
+            // the next request's first page, and where page j of the table would be in this one
+            uint32_t next = r + 1 < kPlanThreads ? s.c0[r + 1] : end;
+            int64_t at = entry(r, j);
 #pragma unroll
             for (int k = 0; k < kIds; ++k) {
                 if (j + k >= end) break;
-                while (r + 1 < kPlanThreads && s.c0[r + 1] <= j + k) ++r;
-                id[k] = a.page_table[entry(r, j + k)];
+                while (j + k >= next) {
+                    ++r;
+                    next = r + 1 < kPlanThreads ? s.c0[r + 1] : end;
+                    at = entry(r, j);
+                }
+                id[k] = a.page_table[at + k];
             }
         } else {
             id[0] = a.free_list[count - 1 - (int)j];
@@ -596,7 +604,7 @@ bool in(int64_t v, int64_t lo, int64_t hi) { return v >= lo && v <= hi; }
 cudaError_t launch_page_step(const PageStepArgs &a, cudaStream_t st) {
     // Up to a size one CTA is faster, above it a cluster of 8 (times in us, one CTA against the cluster). Plans of 64
     // requests and tokens 2.9, 5.9; of 1024 4.5, 6.5; of 512 requests and 4096 tokens 5.3, 6.4, and 6144 tokens 6.5, 6.2.
-    // Releases of 64 requests 3.3, 6.0; of 768 6.2, 6.4; of 1024 7.4, 6.6.
+    // Releases of 64 requests 3.0, 5.9; of 768 6.2, 6.5; of 1024 8.0, 6.6.
     const bool big = a.keep_len ? a.requests > 768 : a.requests > kPlanThreads || a.max_tokens > 5 * 1024;
     const unsigned ctas = big ? kPlanCtas : 1;
     cudaLaunchConfig_t cfg = {};
