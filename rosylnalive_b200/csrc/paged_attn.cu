@@ -406,7 +406,7 @@ __device__ __forceinline__ bool few_item(const RoleState &r, const Item &it, uin
         const bool first = j == s, dirty = key0 + TKF - 1 > it.pos0;  // dirty: some row does not see the whole tile
         // rows are token-major, so the key is seen from this row on
         const int from = dirty ? min(max(key0 + key - it.pos0, 0), 64) * group : 0;
-        bool over = first;
+        bool over = false;
         if (!first) {
 #pragma unroll 1
             for (int g = 0; g < rows; g += 8) {
@@ -417,7 +417,7 @@ __device__ __forceinline__ bool few_item(const RoleState &r, const Item &it, uin
                 for (int e = 0; e < 8; ++e) over |= g + e < rows && x[e] * sc > m[e] + kRescaleThreshold;
             }
         }
-        if (barrier_or(6 + s, 128, over)) {
+        if (first || barrier_or(6 + s, 128, over)) {
 #pragma unroll 1
             for (int g = 0; g < rows; g += 8) {
                 float x[8];
@@ -498,7 +498,30 @@ __device__ __forceinline__ bool few_item(const RoleState &r, const Item &it, uin
     const bool two = nt > 1;  // the second slot has a state
     done[0] += (nt + 1) / 2;
     done[1] += nt / 2;
-    // this slot's last product first: the other's barrier is then at its own last one's phase
+    // This warp's sums of each row's p, while the last product runs: eight rows over 32 lanes, each step halving the rows
+    // that a lane holds.
+    if (nt > s) {
+#pragma unroll 1
+        for (int g = 0; g < rows; g += 8) {
+            float l[8];
+            tmem_ld8(tL + g, l);
+            ptx::tmem_ld_wait();
+#pragma unroll
+            for (int o = 4; o > 0; o /= 2) {
+                const bool up = lane & o;
+#pragma unroll
+                for (int e = 0; e < o; ++e) {
+                    const float give = up ? l[e] : l[e + o], keep = up ? l[e + o] : l[e];
+                    l[e] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+                }
+            }
+            l[0] += __shfl_xor_sync(0xffffffffu, l[0], 8);
+            l[0] += __shfl_xor_sync(0xffffffffu, l[0], 16);
+            if (lane < 8) c.few.l[s][r.quarter][g + lane] = l[0];
+        }
+    }
+    // This slot's last product first: the other's barrier is then at its own last one's phase. (Both warpgroups are through
+    // with their tiles behind these waits, so neither waits in vain at the barriers below.)
     bool ok = nt <= s || wait_bar(&c.o_done[s], (done[s] - 1) & 1, a.err, kErrWaitSoftmax);
     if (ok && nt > 1 - s) ok = wait_bar(&c.o_done[1 - s], (done[1 - s] - 1) & 1, a.err, kErrWaitSoftmax);
     if (!ok) return false;
@@ -519,27 +542,6 @@ __device__ __forceinline__ bool few_item(const RoleState &r, const Item &it, uin
         ptx::tc_fence_before();
         ptx::named_barrier(1, 256);
         ptx::tc_fence_after();
-    }
-    // This warp's sums of each row's p: eight rows over 32 lanes, each step halving the rows that a lane holds.
-    if (nt > s) {
-#pragma unroll 1
-        for (int g = 0; g < rows; g += 8) {
-            float l[8];
-            tmem_ld8(tL + g, l);
-            ptx::tmem_ld_wait();
-#pragma unroll
-            for (int o = 4; o > 0; o /= 2) {
-                const bool up = lane & o;
-#pragma unroll
-                for (int e = 0; e < o; ++e) {
-                    const float give = up ? l[e] : l[e + o], keep = up ? l[e + o] : l[e];
-                    l[e] = keep + __shfl_xor_sync(0xffffffffu, give, o);
-                }
-            }
-            l[0] += __shfl_xor_sync(0xffffffffu, l[0], 8);
-            l[0] += __shfl_xor_sync(0xffffffffu, l[0], 16);
-            if (lane < 8) c.few.l[s][r.quarter][g + lane] = l[0];
-        }
     }
     ptx::named_barrier(1, 256);
     // Lane e: row e's place in the output and its weights of the two slots' O.
