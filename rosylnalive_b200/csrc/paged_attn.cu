@@ -33,7 +33,7 @@
 //
 // What bounds it and what it measured (device time, both kernels; 8 KV heads, two query heads each unless said):
 //   HBM       64 single tokens over 4096 to 4352 keys: 171 us, 6.48 TB/s, 0.99 of a copy's rate.
-//   HBM and the start: 32 x 5 tokens over 100 to 6000 keys, 32 query heads: 39.7 us, 4.3 TB/s. 3.5 us pass before the first
+//   HBM and the start: 32 x 5 tokens over 100 to 6000 keys, 32 query heads: 39.2 us, 4.35 TB/s. 3.5 us pass before the first
 //             load (the lengths' and page table's loads, the cut, and code that no CTA has fetched yet), 4 after the last.
 //   softmax and power: 1,000 tokens over 121,000 keys: 1.25 million cycles, tensor pipe active in 67 percent of them, the
 //             exponentials' unit in 67; 820 us at the 1.53 GHz that 1000 W allow, 1 PFLOP/s over seconds.
