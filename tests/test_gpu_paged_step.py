@@ -496,6 +496,15 @@ def test_attention(mix, heads):
     c.check(c.run(), before)
 
 
+def test_attention_of_more_requests_than_a_block_has_threads():
+    # 900 requests: a thread counts several of them, some without tokens.
+    r = np.random.default_rng(3)
+    new = r.choice([0, 1, 1, 1, 2, 30], 900)
+    c = Cache([(int(n), int(n + p)) for n, p in zip(new, r.integers(0, 120, 900))], 6, 2, seed=13, spare=2)
+    before = c.out.clone()
+    c.check(c.run(), before)
+
+
 @pytest.mark.parametrize("heads", [(64, 1), (100, 1), (128, 1), (33, 1), (256, 2)])
 def test_attention_of_wide_groups(heads):
     c = Cache([(1, 200), (3, 130), (0, 0), (9, 9)], *heads, seed=2)
