@@ -358,7 +358,10 @@ lrm_status lrm_op_qkv_append(void *stream, const lrm_qkv_append_desc *desc);
  * k and v included). out bf16 [tokens][ld_out]. Any q_heads that kv_heads divides, up to 128 query heads a KV head;
  * any mixture of chunk lengths, one token included; requests without tokens are skipped whatever their slot. Keys that a
  * row does not see do not reach it, whatever they hold (NaN and infinities too). Rows outside every request, before
- * cu_seqlens[0] or behind cu_seqlens[requests], are left as they were. Softmax statistics and accumulators are fp32.
+ * cu_seqlens[0] or behind cu_seqlens[requests], are left as they were. Softmax statistics and accumulators are fp32. A
+ * request's tokens are taken in pieces of 2 * floor(128 / group), group = q_heads / kv_heads. In a piece of at most 32 rows
+ * (tokens * group), so for single tokens and short drafts, the weights that multiply v keep 16 bits (off by 2^-15 at most);
+ * in larger ones they are rounded to bf16, as in lrm_op_prefill_attention (off by 2^-8 at most).
  * A request whose rows fall outside the tokens, whose slot is outside 0 .. max_seqs - 1, or whose kv_len is below its
  * tokens or above 16 * pages_per_seq is not computed: its rows are left as they were and the error word gets 0x4001. A
  * page id outside the pool is never read: its keys count as zeros and the error word gets 0x4002. `workspace`:

@@ -2,7 +2,9 @@
 // 5th-generation tensor cores (tcgen05, TMEM, TMA).
 //
 //   o = sum_j p_j v_j / sum_j p_j,   p_j = 2^(scale log2(e) q.k_j - m),   m a running reference maximum:
-// one pass over the keys, with the statistics and the accumulator in fp32 and p rounded to bf16 for the product with v.
+// one pass over the keys, with the statistics and the accumulator in fp32. For the product with v, p is two bf16 values (16
+// bits) in items of up to 32 rows. In larger ones it is rounded to bf16, as in the prefill attention: a second product would
+// add 320 cycles to a tile's 740 of MMAs a slot, and a second P does not fit beside S and O in tensor memory.
 //
 // The work is cut evenly over one persistent CTA an SM (paged_sched.h): single tokens, verify chunks and prefill chunks
 // of any lengths fill the GPU alike. An item is up to 2 * floor(128 / group) tokens of one request and KV head. Its rows
@@ -68,7 +70,8 @@ static_assert(128 * kRegsControl + 256 * kRegsSoftmax <= kThreads * kRegsLaunch,
 constexpr float kRescaleThreshold = 8.0f;  // log2 units: the reference maximum moves only when a tile exceeds it by more
 constexpr int kLeastUnits = 12;  // of a CTA (900 keys, 8 KV heads: 11.7 us, 14.1 with 30; more CTAs than that do not help)
 constexpr int kFewRows = sched::kFewRows;  // items of up to this many rows run with keys and rows swapped
-constexpr int FEW_SUB = kFewRows * 128;  // half of the dims (q) or keys (P) of up to 32 rows
+constexpr int FEW_SUB = kFewRows * 128;  // half of the dims of up to 32 rows of q
+constexpr int FEW_P_SUB = 2 * FEW_SUB, FEW_P = 2 * FEW_P_SUB;  // half of the keys (all) of P, two lines a row, in a slot
 constexpr uint32_t kErrWaitProducer = 0x4010, kErrWaitIssuer = 0x4011, kErrWaitSoftmax = 0x4012, kErrWaitScheduler = 0x4013;
 
 // One item's share of a CTA's range: key tiles [kb, ke) of it.
@@ -141,6 +144,7 @@ static_assert(kLeastUnits > sched::kWide.tile, "a share within an item holds a t
 static_assert(offsetof(Control, few) % 16 == 0, "few.max is read as float4");
 constexpr int SMEM_BYTES = (SLOTS + KV_ST) * TILE + (int)sizeof(Control);
 static_assert(SMEM_BYTES <= 227 * 1024, "shared memory of one CTA");
+static_assert(SLOTS * FEW_P <= TILE && 2 * 2 * FEW_SUB <= TILE, "q of two few-row items in one tile, their P in the other");
 
 struct Params {
     PagedAttnArgs a;
@@ -317,7 +321,13 @@ __device__ __forceinline__ void quad_transpose(uint4 (&v)[4], int lane) {
 // warpgroup and moves only when some score exceeds it by 2^8, which one barrier with an OR finds out; only then (and at
 // an item's first tile) are the tile's maxima reduced over threads. P goes to shared memory as the B operand of
 // O^T = V^T P^T; sums of p stay per thread until the end. A tile costs 1,400 cycles, which hide under the 2,800 that its K
-// and V take as one SM's share of HBM. (As narrow items, 32 x 5 drafted tokens took 64 us against 43.)
+// and V take as one SM's share of HBM.
+// Each row of P has two rows of bf16 here, its first 16 bits and the rest: together off by 2^-15 of p at most, so that a
+// single token is as precise as with lrm_op_decode_attention, whose p is fp32. Groups of eight rows alternate (eight rows,
+// the eight rests, ...), so O^T's columns do too, and up to eight rows still make one MMA of 16 columns. (p rounded to bf16
+// alone: 64 single tokens over 4096 keys off by 2.3e-3 in norm instead of 1.66e-3, which is the output's own rounding; 32 x 5
+// drafted tokens 40.4 us instead of 41.2, 8 x 511 among 56 decodes 55.1 instead of 58.3, single tokens alike. The rests in
+// eight MMAs of their own: 42.7, and 64 x 4096 173.9 instead of 172.5.)
 struct RoleState {
     Control *c;
     const Params *p;
@@ -377,6 +387,13 @@ __device__ __forceinline__ void load8(const float *shared, float (&x)[8]) {
     x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
 }
 
+// What is left of p beside its first 16 bits (the difference is exact); above 0 where p is, so that it times an infinite v is
+// that infinity and no NaN.
+__device__ __forceinline__ float rest(float p) {
+    const float hi = __uint_as_float(__float_as_uint(p) & 0xFFFF0000u);
+    return fmaxf(p - hi, fminf(p, 0x1p-126f));
+}
+
 // Eight rows' scores of this thread's key; rows that do not see it (those before `from`) as -inf.
 __device__ __forceinline__ void load_scores(uint32_t t, int from, float (&x)[8]) {
     tmem_ld8(t, x);
@@ -396,8 +413,8 @@ __device__ __forceinline__ bool few_item(const RoleState &r, const Item &it, uin
     const int key = r.quarter * 32 + lane;
     const uint32_t lanes = (uint32_t)(r.quarter * 32) << 16, tS = r.tmem + 256 * s + lanes, tO = tS + 128, tL = tS + 192;
     const float sc = a.scale_log2;
-    // P[row][key] with keys contiguous, 64 a 128-byte swizzled line
-    const uint32_t pt = ptx::smem_u32(r.pt) + (key >> 6) * FEW_SUB, pk = (key & 63) * 2;
+    // P[row][key] with keys contiguous, 64 a 128-byte swizzled line; rows g .. g + 7 at lines 2g .. 2g + 7, their rests behind
+    const uint32_t pt = ptx::smem_u32(r.pt) + (key >> 6) * FEW_P_SUB, pk = (key & 63) * 2;
 #pragma unroll 1
     for (int j = s; j < nt; j += 2, ++steps) {
         if (!wait_bar(&c.s_full[s], steps & 1, a.err, kErrWaitSoftmax)) return false;
@@ -446,17 +463,18 @@ __device__ __forceinline__ bool few_item(const RoleState &r, const Item &it, uin
                 ptx::tc_fence_after();
 #pragma unroll 1
                 for (int g = 0; g < rows; g += 8) {
-                    float o[8], l[8], alpha[8];
+                    float o[16], l[8], alpha[8];
                     load8(&c.few.alpha[s][g], alpha);
-                    tmem_ld8(tO + g, o);
+                    ptx::tmem_ld16(tO + 2 * g, reinterpret_cast<uint32_t(&)[16]>(o));
                     tmem_ld8(tL + g, l);
                     ptx::tmem_ld_wait();
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         o[e] *= alpha[e];
+                        o[e + 8] *= alpha[e];
                         l[e] *= alpha[e];
                     }
-                    tmem_st8(tO + g, o);
+                    ptx::tmem_st16(tO + 2 * g, reinterpret_cast<uint32_t(&)[16]>(o));
                     tmem_st8(tL + g, l);
                 }
                 ptx::tmem_st_wait();
@@ -477,12 +495,19 @@ __device__ __forceinline__ bool few_item(const RoleState &r, const Item &it, uin
                 l[e] = first ? x[e] : l[e] + x[e];
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) w[e] = pack2(x[2 * e], x[2 * e + 1]);
-            const uint32_t row = pt + g * 128;
+            for (int e = 0; e < 4; ++e) w[e] = __byte_perm(__float_as_uint(x[2 * e]), __float_as_uint(x[2 * e + 1]), 0x7632);
+            const uint32_t row = pt + g * 256;
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                asm volatile("st.shared.b16 [%0], %1;" ::"r"(row + e * 128 + (pk ^ (e << 4))),
-                             "h"((uint16_t)(w[e / 2] >> (e & 1 ? 16 : 0))));
+            for (int part = 0; part < 2; ++part) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    asm volatile("st.shared.b16 [%0], %1;" ::"r"(row + part * 1024 + e * 128 + (pk ^ (e << 4))),
+                                 "h"((uint16_t)(w[e / 2] >> (e & 1 ? 16 : 0))));
+                if (part == 0) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w[e] = pack2(rest(x[2 * e]), rest(x[2 * e + 1]));
+                }
+            }
             tmem_st8(tL + g, l);
         }
         ptx::tc_fence_before();
@@ -531,12 +556,13 @@ __device__ __forceinline__ bool few_item(const RoleState &r, const Item &it, uin
 #pragma unroll 1
             for (int e = 0; e < rows; ++e) {
                 uint32_t o;
-                asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(o) : "r"(tO + e));
+                const uint32_t at = tO + 2 * (e & ~7) + (e & 7);  // row e's column
+                asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(o) : "r"(at));
                 ptx::tmem_ld_wait();
                 const int last = min(it.pos0 + (e * r.p->inv_group >> 16), it.ke * TKF - 1);
                 o = __float_as_uint(__uint_as_float(o) + poison_sum(a, it.table, it.kvh, max(it.kb * TKF, it.pos0 + 1), last,
                                                                     TKF, it.kb + s, 2, key));
-                asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(tO + e), "r"(o) : "memory");
+                asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(at), "r"(o) : "memory");
             }
         ptx::tmem_st_wait();
         ptx::tc_fence_before();
@@ -573,15 +599,16 @@ __device__ __forceinline__ bool few_item(const RoleState &r, const Item &it, uin
     // Every other eight rows are this warpgroup's to write; thread = dim.
 #pragma unroll 1
     for (int g = 8 * s; g < rows; g += 16) {
-        float o[8], o1[8];
-        tmem_ld8(r.tmem + lanes + 128 + g, o);
-        if (two) tmem_ld8(r.tmem + lanes + 256 + 128 + g, o1);
+        float o[16], o1[16];
+        ptx::tmem_ld16(r.tmem + lanes + 128 + 2 * g, reinterpret_cast<uint32_t(&)[16]>(o));
+        if (two) ptx::tmem_ld16(r.tmem + lanes + 256 + 128 + 2 * g, reinterpret_cast<uint32_t(&)[16]>(o1));
         ptx::tmem_ld_wait();
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
+            o[e] += o[e + 8];  // the rests' share
             o[e] *= __shfl_sync(0xffffffffu, w0, g + e);
             const float v1 = __shfl_sync(0xffffffffu, w1, g + e);
-            if (two) o[e] = fmaf(o1[e], v1, o[e]);
+            if (two) o[e] = fmaf(o1[e] + o1[e + 8], v1, o[e]);
             const int64_t to = __shfl_sync(0xffffffffu, at, g + e) + key;
             if (g + e < rows) {
                 if (it.dest < 0)
@@ -934,9 +961,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (lane == 0) ptx::mbar_arrive(&c.item_empty[k % ITEMS]);
                 if (ntok == 0) break;
                 const bool wide = ntok > p.tt, few = ntok * p.group <= kFewRows;
-                // few: S^T = K Q^T (128 keys x 16 or 32 rows) and O^T = V^T P^T (128 dims x rows)
-                const int nrow = ntok * p.group <= 16 ? 16 : 32;
-                const uint32_t idesc_s = ptx::idesc_bf16_f32(128, nrow), idesc_o = idesc_s | 1u << 15;  // A (V) MN-major
+                // few: S^T = K Q^T (128 keys x 16 or 32 rows) and O^T = V^T P^T (128 dims x rows, twice)
+                const int nrow = ntok * p.group <= 16 ? 16 : 32, np = (ntok * p.group + 7) / 8 * 16;
+                const uint32_t idesc_s = ptx::idesc_bf16_f32(128, nrow);
+                const uint32_t idesc_o = ptx::idesc_bf16_f32(128, np) | 1u << 15;  // A (V) MN-major
                 // Product n's slot is n & 1. S lies beside P, so the next S of a slot is computed as soon as its softmax
                 // has taken this one, and waits there for it; only P V waits for P.
                 const int count = wide ? 2 * nt : nt;
@@ -1053,11 +1081,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 if (m - 2 >= dirty && !wait_clean(m - 2)) break;
                                 const uint32_t v = bKV + vt * (TILE >> 4), keep = m >= 4 ? 1u : 0u;
                                 if (few) {
-                                    const uint32_t pt = bQ + ((TILE + s * 2 * FEW_SUB) >> 4);
+                                    const uint32_t pt = bQ + ((TILE + s * FEW_P) >> 4);
 #pragma unroll
                                     for (int kk = 0; kk < 8; ++kk)
                                         ptx::mma_bf16(tS + 128, mnmajor(v + kk * (2048 >> 4)),
-                                                      kmajor(pt + (((kk >> 2) * FEW_SUB + (kk & 3) * 32) >> 4)), idesc_o,
+                                                      kmajor(pt + (((kk >> 2) * FEW_P_SUB + (kk & 3) * 32) >> 4)), idesc_o,
                                                       kk > 0 ? 1u : keep);
                                 } else {
 #pragma unroll
@@ -1103,7 +1131,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (lane == 0) ptx::mbar_arrive(&c.item_empty[k % ITEMS]);
             if (it.ntok == 0) break;
             if (it.ntok * p.group <= kFewRows) {
-                const RoleState r = {&c, &p, sQ + TILE + s * 2 * FEW_SUB, tmem, s, quarter, lane, cta, k};
+                const RoleState r = {&c, &p, sQ + TILE + s * FEW_P, tmem, s, quarter, lane, cta, k};
                 // the sums of p go where a narrow item's O is: both warpgroups have read that out behind this
                 if (narrow_before) ptx::named_barrier(1, 256);
                 narrow_before = false;
