@@ -58,7 +58,7 @@
 namespace lrm {
 namespace {
 
-constexpr int TK = sched::kTileKeys, TKF = sched::kFewTileKeys, KV_ST = 5, SLOTS = 2, ITEMS = 4, DIRTY = 8;
+constexpr int TK = sched::kTileKeys, TKF = sched::kFewTileKeys, KV_ST = sched::kRing, SLOTS = 2, ITEMS = 4, DIRTY = 8;
 constexpr int P_COL = 80;  // P's columns in tensor memory, behind S's (two bf16 a column): 80 + 40 of the slot's first 128
 constexpr int SUB = 128 * 64 * 2;  // one [128 rows][64] bf16 swizzled sub-tile
 constexpr int TILE = 2 * SUB;      // [128 rows][128]
@@ -90,11 +90,6 @@ struct alignas(16) Record {
     int tok0, ntok, kvh, follow;
 };
 
-// The ring order of an item's tiles is the order in which the issuer first uses them. In step t it issues S = Q K^T of tile t
-// (wide: for both slots) and O += P V of an earlier one. Wide: S of slot 0, P V of slot 1 and tile t - 2, S of slot 1, P V of
-// slot 0 and tile t - 1; else tile t is slot t & 1's, and P V is of tile t - 2. So K_t comes before V_{t - lead + 1}, lead
-// being 2 (wide) or 3, and V_t is ring item t + min(nt, t + lead) of an item of nt tiles.
-
 // A value that is the same in all lanes, so that the compiler knows it is.
 __device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
 
@@ -120,7 +115,9 @@ struct Control {
     uint64_t s_full[SLOTS], s_free[SLOTS], p_full[SLOTS], o_done[SLOTS];  // a phase each product of the slot
     uint64_t item_full[ITEMS], item_empty[ITEMS];
     uint64_t v_clean[DIRTY];  // dirty tile n's v is clean: barrier n % DIRTY
-    int z[2][32], z_pad[8];  // the producers': z coordinates of a window of pages
+    int z[2][32];  // the producers': z coordinates of a window of pages (one int behind it is read, and not used)
+    int kv_issued[KV_ST], q_issued[2];  // the last ring item copied to a stage, the last item's q to a place; from 1, 0: none
+    int gave_up;                        // the issuer did not get to the end of the items
     Item items[ITEMS];
     uint64_t warp_sum[kThreads / 32];
     uint64_t started;
@@ -695,6 +692,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 ptx::mbar_init(&c.o_done[s], 1);
             }
             for (int s = 0; s < 4; ++s) c.poison[s] = 0;
+            for (int s = 0; s < KV_ST; ++s) c.kv_issued[s] = 0;
+            c.q_issued[0] = c.q_issued[1] = c.gave_up = 0;
             for (int s = 0; s < DIRTY; ++s) ptx::mbar_init(&c.v_clean[s], 1);
             for (int s = 0; s < ITEMS; ++s) {
                 ptx::mbar_init(&c.item_full[s], 1);
@@ -858,6 +857,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     few_before = few;
                     if (ptx::elect_one()) {
                         uint64_t *bar = &c.q_full[k & 1];
+                        c.q_issued[k & 1] = k + 1;
                         if (few) {
                             uint8_t *dst = sQ + (k & 1) * 2 * FEW_SUB;
                             ptx::mbar_arrive_expect_tx(bar, p.few_tok * p.group * 256);
@@ -874,11 +874,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     __syncwarp();
                 }
-                const int lead = wide ? 2 : 3, dirty = kv ? uniform(item_dirty) : nt;
+                const int lead = wide ? sched::kLeadWide : sched::kLead, dirty = kv ? uniform(item_dirty) : nt;
                 // Dirty tile j's keys that the first token does not see. (Those past the request's pages are zeros.)
                 auto clean = [&](int j) {
-                    const int x = ring + j + min(nt, j + lead), key0 = (kb + j) * tile_pages * kPageTokens;
-                    if (!wait_bar(&c.kv_full[x % KV_ST], (x / KV_ST) & 1, err, kErrWaitProducer)) ok = false;
+                    const int x = ring + sched::v_place(j, nt, lead), key0 = (kb + j) * tile_pages * kPageTokens;
+                    if (!wait_bar(&c.kv_full[x % KV_ST], sched::fill_parity(x), err, kErrWaitProducer)) ok = false;
                     clean_v(sKV + (x % KV_ST) * TILE, max(0, pos0 + 1 - key0),
                             min(tile_pages * kPageTokens, npages * kPageTokens - key0), lane, pos0 + ntok - 1 - key0,
                             &c.poison[k & 3], k + 1);
@@ -902,13 +902,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                             const int *zt = c.z[kv] + (ta - t0) * tile_pages;
 #pragma unroll 1
                             for (int t = ta; t < t1; ++t, zt += tile_pages) {
-                                const int x = ring + t + (kv ? min(nt, t + lead) : max(0, t - lead + 1)), st = x % KV_ST;
+                                const int x = ring + (kv ? sched::v_place(t, nt, lead) : sched::k_place(t, lead)), st = x % KV_ST;
                                 const uint32_t bar = ptx::smem_u32(&c.kv_full[st]), dst = ptx::smem_u32(sKV) + st * TILE;
                                 int zp[8];
 #pragma unroll
                                 for (int u = 0; u < 8; ++u) zp[u] = zt[u];  // (the array behind z is read past a window's end)
-                                ok = wait_bar(&c.kv_empty[st], ((x / KV_ST) & 1) ^ 1, err, kErrWaitProducer);
+                                ok = wait_bar(&c.kv_empty[st], sched::fill_parity(x) ^ 1, err, kErrWaitProducer);
                                 if (!ok) break;
+                                c.kv_issued[st] = x + 1;
                                 ptx::mbar_arrive_expect_tx(&c.kv_full[st], tile_pages * 4096);
 #pragma unroll
                                 for (int u = 0; u < 5; ++u) {
@@ -922,11 +923,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                                         tma_3d(dst + SUB + u * 2048, &tkv, bar, 64, zp[u]);
                                     }
                                 }
-                            }
-                            // on the error path, the copies in flight must land before the CTA exits
-                            for (int y = ok ? t1 : 0; y < t1; ++y) {
-                                const int x = ring + y + (kv ? min(nt, y + lead) : max(0, y - lead + 1));
-                                wait_bar(&c.kv_full[x % KV_ST], (x / KV_ST) & 1, err, kErrWaitProducer);
                             }
                         }
                         __syncwarp();
@@ -951,6 +947,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             int ring = 0;                // ring items of the items before this one
             uint32_t before0 = 0, before1 = 0;  // products of the items before, a slot
             uint32_t cleaned = 0;               // dirty tiles of the items before
+            bool ended = false;
             for (int k = 0;; ++k) {
                 bool ok = wait_bar(&c.item_full[k % ITEMS], (k / ITEMS) & 1, err, kErrWaitIssuer);
                 if (!__all_sync(0xffffffffu, ok)) break;
@@ -959,7 +956,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int dirty = uniform(c.items[k % ITEMS].dirty);
                 __syncwarp();
                 if (lane == 0) ptx::mbar_arrive(&c.item_empty[k % ITEMS]);
-                if (ntok == 0) break;
+                if ((ended = ntok == 0)) break;
                 const bool wide = ntok > p.tt, few = ntok * p.group <= kFewRows;
                 // few: S^T = K Q^T (128 keys x 16 or 32 rows) and O^T = V^T P^T (128 dims x rows, twice)
                 const int nrow = ntok * p.group <= 16 ? 16 : 32, np = (ntok * p.group + 7) / 8 * 16;
@@ -1106,6 +1103,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 before1 += count / 2;
                 cleaned += (uint32_t)max(0, nt - dirty);
             }
+            if (!ended && lane == 0) c.gave_up = 1;
             // No MMA may still be writing TMEM when it is freed (this matters on the error path).
             if (ptx::elect_one()) ptx::mma_commit(&c.fin);
             wait_bar(&c.fin, 0, err, kErrWaitIssuer);
@@ -1351,6 +1349,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     ptx::tc_fence_after();
     if (warp == 1) ptx::tmem_dealloc(tmem, 512);
+    // Copies in flight must land before the CTA exits. An issuer that got to the end has waited for all of them. Else, since
+    // every role has returned, a stage's last copy is the only one of it that can be on its way: the one before was used
+    // before the stage was given out again, and nothing refills it now.
+    if (tid == 0 && c.gave_up) {
+        for (int s = 0; s < KV_ST; ++s)
+            if (const int x = c.kv_issued[s]) wait_bar(&c.kv_full[s], sched::fill_parity(x - 1), err, kErrWaitProducer);
+        for (int s = 0; s < 2; ++s)
+            if (const int k = c.q_issued[s]) wait_bar(&c.q_full[s], (k - 1) >> 1 & 1, err, kErrWaitProducer);
+    }
 }
 
 // Merges the partial results of the items that a cut passes through: o = sum 2^(m_i - m) o_i / sum 2^(m_i - m) l_i in the

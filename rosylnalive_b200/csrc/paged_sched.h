@@ -130,5 +130,16 @@ LRM_HD int cta_of(const Cut &k, uint64_t u) {
     return u < longer ? (int)quotient(u, k.share + 1) : (int)(k.more + quotient(u - longer, k.share));
 }
 
+// ---- the ring of K and V tiles ----
+//
+// The ring order of an item's tiles is the order in which the issuer first uses them. In step t it issues S = Q K^T of tile t
+// (wide: for both slots) and O += P V of an earlier one. Wide: S of slot 0, P V of slot 1 and tile t - 2, S of slot 1, P V of
+// slot 0 and tile t - 1; else tile t is slot t & 1's, and P V is of tile t - 2. So K_t comes before V_{t - lead + 1}, lead
+// being 2 (wide) or 3. Ring item x (counted from the CTA's first) is fill x / kRing of stage x % kRing.
+constexpr int kRing = 5, kLeadWide = 2, kLead = 3;
+LRM_HD int k_place(int t, int lead) { return t + (t >= lead ? t - lead + 1 : 0); }            // of K_t in its item
+LRM_HD int v_place(int t, int nt, int lead) { return t + (t + lead < nt ? t + lead : nt); }  // of V_t, nt tiles
+LRM_HD uint32_t fill_parity(int x) { return (uint32_t)(x / kRing) & 1; }
+
 }  // namespace sched
 }  // namespace lrm
