@@ -138,6 +138,7 @@ struct Control {
     };
 };
 static_assert(kLeastUnits > sched::kWide.tile, "a share within an item holds a tile");
+static_assert(sched::kSoftmaxPolls > sched::kIssuerWaits * sched::kPolls, "the softmax's warps give up together");
 static_assert(offsetof(Control, few) % 16 == 0, "few.max is read as float4");
 constexpr int SMEM_BYTES = (SLOTS + KV_ST) * TILE + (int)sizeof(Control);
 static_assert(SMEM_BYTES <= 227 * 1024, "shared memory of one CTA");
@@ -171,7 +172,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // ptx::mbar_wait with the first poll (which by itself waits some time) on the straight path and the loop behind it out of
 // the way. Three roles' code shares an SM sub-partition's instruction buffers, so code that is not straight costs some 5
 // cycles an instruction in fetches: with the polls unrolled (60 KB of code for thirty waits) every role stalled on them.
-constexpr uint32_t kPolls = 1u << 20;  // a second or so; waits are microseconds
 __device__ __forceinline__ bool try_wait(uint32_t bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
@@ -185,8 +185,9 @@ __device__ __forceinline__ bool try_wait(uint32_t bar, uint32_t parity) {
 }
 __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, uint32_t *err, uint32_t code) {
     if (__builtin_expect(try_wait(bar, parity), 1)) return true;
+    const uint32_t polls = code == kErrWaitSoftmax ? sched::kSoftmaxPolls : sched::kPolls;
 #pragma unroll 1
-    for (uint32_t i = 0; i < kPolls; ++i)
+    for (uint32_t i = 0; i < polls; ++i)
         if (try_wait(bar, parity)) return true;
     atomicCAS(err, 0u, code);
     return false;

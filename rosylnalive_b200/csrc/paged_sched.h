@@ -139,6 +139,10 @@ LRM_HD int cta_of(const Cut &k, uint64_t u) {
 constexpr int kRing = 5, kLeadWide = 2, kLead = 3;
 LRM_HD int k_place(int t, int lead) { return t + (t >= lead ? t - lead + 1 : 0); }            // of K_t in its item
 LRM_HD int v_place(int t, int nt, int lead) { return t + (t + lead < nt ? t + lead : nt); }  // of V_t, nt tiles
+// Waits end after so many polls (a second or so; waits are microseconds). The softmax's warps meet at barriers that have no such
+// limit, so they must agree on whether a wait failed: theirs end long after the issuer, which makes at most ten waits from one
+// commit to the next of a slot, has either committed or given up for good, so nothing arrives while some have left.
+constexpr uint32_t kPolls = 1u << 20, kIssuerWaits = 10, kSoftmaxPolls = 16 * kPolls;
 LRM_HD uint32_t fill_parity(int x) { return (uint32_t)(x / kRing) & 1; }
 
 }  // namespace sched

@@ -69,6 +69,11 @@ class Cta:
         self.o_free, self.q_empty, self.cleaned = 0, 0, 0
         self.mark, self.reading, self.ahead = [0] * self.MARKS, 0, 0
         self.ended = False
+        self.waits, self.last, self.most = 0, [0, 0], 0  # the issuer's waits, and the most from a slot's commit to its next
+
+    def commit(self, s):
+        self.most = max(self.most, self.waits - self.last[s])
+        self.last[s] = self.waits
 
     def item(self, role, k):
         """Until the scheduler has handed out item k: four items on from one that all have taken."""
@@ -122,22 +127,28 @@ class Cta:
         x, cleaned, before = 0, 0, [0, 0]
         for k, (nt, wide, dirty, marked) in enumerate(self.items):
             yield from self.item("issuer", k)
+            self.waits += 2  # the item and its q
 
             def tile():
                 nonlocal x
+                self.waits += 1
                 yield from self.wait(self.full[x % self.R], self.lib.parity_of(x), x // self.R + 1)
                 x += 1
                 return (x - 1) % self.R
 
             def product(s, n):
+                self.waits += 1
                 while self.p_full[s] < before[s] + n + 1:
                     yield
                 self.o_done[s] += 1
+                self.commit(s)
 
             def score(s, n):
+                self.waits += 1
                 while self.s_free[s] < before[s] + n:
                     yield
                 self.s_full[s] += 1
+                self.commit(s)
 
             vt = None
             for t in range(nt + 2):
@@ -154,6 +165,7 @@ class Cta:
                         self.q_empty += t == nt - 1
                     if 1 <= t <= nt:
                         vt = yield from tile()
+                        self.waits += (t == 1) + (t > dirty)
                         while t == 1 and self.o_free < 2 * k:
                             yield
                         while t > dirty and self.cleaned < cleaned + t - dirty:
@@ -168,6 +180,7 @@ class Cta:
                         self.q_empty += t == nt - 1
                     if t >= 2:
                         vt = yield from tile()
+                        self.waits += (t == 2) + (t - 2 >= dirty)
                         while t == 2 and self.o_free < 2 * k:
                             yield
                         while t - 2 >= dirty and self.cleaned < cleaned + t - 1 - dirty:
@@ -257,3 +270,16 @@ def test_what_is_waited_for_after_giving_up_is_what_is_in_flight(sched):
         for st, x in cta.issued.items():
             assert cta.full[st].passes(sched.parity_of(x))
     assert in_flight > 50
+
+
+def test_the_issuer_commits_or_gives_up_before_a_wait_of_the_softmax_ends(sched):
+    # The softmax's warps wait for a slot's next commit; an issuer that never waits longer than its limit has made it, or has
+    # returned, by the time theirs ends. (Items of one tile leave slot 1 out, so whole runs of them stand between its commits,
+    # but then slot 1's warps wait for slot 0's.)
+    for seed in range(60):
+        rng = random.Random(2000 + seed)
+        items = [(max(2, nt), wide, dirty, marked) for nt, wide, dirty, marked in some_items(rng, 12)]
+        cta = Cta(sched, items, rng)
+        cta.run()
+        assert cta.most <= sched.issuer_waits()
+    assert sched.polls(1) > sched.issuer_waits() * sched.polls(0)
