@@ -123,9 +123,7 @@ struct Control {
     uint64_t started;
     Walk walk;  // of the scheduler, behind the range's last item
     uint32_t tmem;
-    // The item (counted from 1) in which v of a visible key was zeroed, by item: its tiles, two at least, are in the ring of
-    // five when they are cleaned, so that is at most two items ahead of the epilogue that reads this.
-    int poison[4];
+    int poison[sched::kMarks];  // the item (counted from 1) in which v of a visible key was zeroed, by item % kMarks
     union {
         float ml[SLOTS][128][2];  // narrow: the slots' states
         struct {                  // few
@@ -549,7 +547,7 @@ __device__ __forceinline__ bool few_item(const RoleState &r, const Item &it, uin
     if (ok && nt > 1 - s) ok = wait_bar(&c.o_done[1 - s], (done[1 - s] - 1) & 1, a.err, kErrWaitSoftmax);
     if (!ok) return false;
     ptx::tc_fence_after();
-    if (c.poison[r.k & 3] == r.k + 1) {
+    if (c.poison[r.k % sched::kMarks] == r.k + 1) {
         if (nt > s)
 #pragma unroll 1
             for (int e = 0; e < rows; ++e) {
@@ -692,7 +690,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 ptx::mbar_init(&c.p_full[s], 4);
                 ptx::mbar_init(&c.o_done[s], 1);
             }
-            for (int s = 0; s < 4; ++s) c.poison[s] = 0;
+            for (int s = 0; s < sched::kMarks; ++s) c.poison[s] = 0;
             for (int s = 0; s < KV_ST; ++s) c.kv_issued[s] = 0;
             c.q_issued[0] = c.q_issued[1] = c.gave_up = 0;
             for (int s = 0; s < DIRTY; ++s) ptx::mbar_init(&c.v_clean[s], 1);
@@ -882,7 +880,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (!wait_bar(&c.kv_full[x % KV_ST], sched::fill_parity(x), err, kErrWaitProducer)) ok = false;
                     clean_v(sKV + (x % KV_ST) * TILE, max(0, pos0 + 1 - key0),
                             min(tile_pages * kPageTokens, npages * kPageTokens - key0), lane, pos0 + ntok - 1 - key0,
-                            &c.poison[k & 3], k + 1);
+                            &c.poison[k % sched::kMarks], k + 1);
                     __syncwarp();
                     if (lane == 0) ptx::mbar_arrive(&c.v_clean[cleaned % DIRTY]);
                     ++cleaned;
@@ -1268,7 +1266,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 l = (l0 == 0.f ? 0.f : w[0] * l0) + (l1 == 0.f ? 0.f : w[1] * l1);
                 ptx::named_barrier(1, 256);  // read by both before either may write there again
             }
-            const bool poisoned = c.poison[k & 3] == k + 1;
+            const bool poisoned = c.poison[k % sched::kMarks] == k + 1;
             if (active) {
                 // o = w[0] O_0 + w[1] O_1 (wide: this slot's O alone), 32 dims at a time
                 const uint32_t tO = (wide ? tS : tmem + lanes) + 128;

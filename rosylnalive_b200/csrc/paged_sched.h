@@ -139,6 +139,12 @@ LRM_HD int cta_of(const Cut &k, uint64_t u) {
 constexpr int kRing = 5, kLeadWide = 2, kLead = 3;
 LRM_HD int k_place(int t, int lead) { return t + (t >= lead ? t - lead + 1 : 0); }            // of K_t in its item
 LRM_HD int v_place(int t, int nt, int lead) { return t + (t + lead < nt ? t + lead : nt); }  // of V_t, nt tiles
+// The cleaning of V marks an item (kMarks places, by item) and the item's epilogue reads the mark. While the epilogue of item k
+// runs, the P V of item k + 1 waits for it, so the last tile that has been freed is K of k + 1. Of items of one tile (with
+// more the ring holds fewer items) that is ring item 2k + 2, its stage's next one is 2k + 2 + kRing, and V of item k + j is
+// 2k + 2j + 1: V can be there, and be cleaned, up to (kRing + 1) / 2 items ahead of the mark that is still to be read.
+constexpr int kMarks = (kRing + 1) / 2 + 1;
+
 // Waits end after so many polls (a second or so; waits are microseconds). The softmax's warps meet at barriers that have no such
 // limit, so they must agree on whether a wait failed: theirs end long after the issuer, which makes at most ten waits from one
 // commit to the next of a slot, has either committed or given up for good, so nothing arrives while some have left.

@@ -57,7 +57,7 @@ class Cta:
     """The roles of a CTA that fill, use and free the ring, as generators that yield what they wait for. MMAs complete when
     they are issued; a copy lands when the memory's turn comes. Every wait that passes is checked to be the phase meant."""
 
-    ITEMS, MARKS = 4, 4
+    ITEMS = 4
 
     def __init__(self, lib, items, rng):
         self.lib, self.items, self.rng = lib, items, rng  # items: (tiles, wide, dirty tile, whether a key is marked)
@@ -67,7 +67,8 @@ class Cta:
         self.picked = {r: -1 for r in ("K", "V", "issuer", "softmax")}
         self.s_full, self.p_full, self.o_done, self.s_free = [0, 0], [0, 0], [0, 0], [0, 0]
         self.o_free, self.q_empty, self.cleaned = 0, 0, 0
-        self.mark, self.reading, self.ahead = [0] * self.MARKS, 0, 0
+        self.MARKS = lib.marks()
+        self.mark, self.read, self.ahead = [0] * self.MARKS, [0, 0], 0  # read: items whose mark has been read, a slot
         self.ended = False
         self.waits, self.last, self.most = 0, [0, 0], 0  # the issuer's waits, and the most from a slot's commit to its next
 
@@ -99,7 +100,7 @@ class Cta:
                 yield from self.wait(self.full[x % self.R], self.lib.parity_of(x), x // self.R + 1)
                 if marked and j == nt - 1:
                     self.mark[k % self.MARKS] = k + 1
-                    self.ahead = max(self.ahead, k - self.reading)
+                    self.ahead = max(self.ahead, k - min(self.read))
                 self.cleaned += 1
 
             for t in range(nt):
@@ -208,10 +209,9 @@ class Cta:
             done[1] += nt if wide else nt // 2
             while self.o_done[s] < done[s] or (not wide and self.o_done[1 - s] < done[1 - s]):
                 yield
-            if s == 0:
-                self.reading = k
             yield
             assert (self.mark[k % self.MARKS] == k + 1) == bool(marked), "a mark was lost"
+            self.read[s] = k + 1
             self.o_free += 1
 
     def run(self, steps=None):
@@ -246,6 +246,17 @@ def test_the_roles_get_through_and_lose_no_mark(sched):
         cta = Cta(sched, some_items(rng, rng.randint(1, 14)), rng)
         cta.run()
         assert cta.ended and not cta.flying
+
+
+def test_the_cleaning_runs_as_far_ahead_as_there_are_marks(sched):
+    # Items of one tile whose epilogues are slow: the mark of the item farthest ahead takes the last place that is free.
+    most = 0
+    for seed in range(300):
+        rng = random.Random(3000 + seed)
+        cta = Cta(sched, [(1, 0, 0, 1)] * 12, rng)
+        cta.run()
+        most = max(most, cta.ahead)
+    assert most == sched.marks() - 1
 
 
 def test_what_is_waited_for_after_giving_up_is_what_is_in_flight(sched):
