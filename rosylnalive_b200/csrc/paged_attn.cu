@@ -68,7 +68,6 @@ constexpr int kRegsLaunch = 168;  // 65536 / 384, rounded down to the allocation
 constexpr int kRegsControl = 72, kRegsSoftmax = 216;
 static_assert(128 * kRegsControl + 256 * kRegsSoftmax <= kThreads * kRegsLaunch, "register split exceeds the launch");
 constexpr float kRescaleThreshold = 8.0f;  // log2 units: the reference maximum moves only when a tile exceeds it by more
-constexpr int kLeastUnits = 12;  // of a CTA (900 keys, 8 KV heads: 11.7 us, 14.1 with 30; more CTAs than that do not help)
 constexpr int kFewRows = sched::kFewRows;  // items of up to this many rows run with keys and rows swapped
 constexpr int FEW_SUB = kFewRows * 128;  // half of the dims of up to 32 rows of q
 constexpr int FEW_P_SUB = 2 * FEW_SUB, FEW_P = 2 * FEW_P_SUB;  // half of the keys (all) of P, two lines a row, in a slot
@@ -135,7 +134,6 @@ struct Control {
         } few;
     };
 };
-static_assert(kLeastUnits > sched::kWide.tile, "a share within an item holds a tile");
 static_assert(sched::kSoftmaxPolls > sched::kIssuerWaits * sched::kPolls, "the softmax's warps give up together");
 static_assert(offsetof(Control, few) % 16 == 0, "few.max is read as float4");
 constexpr int SMEM_BYTES = (SLOTS + KV_ST) * TILE + (int)sizeof(Control);
@@ -623,10 +621,10 @@ __device__ __forceinline__ bool few_item(const RoleState &r, const Item &it, uin
 // The share of the walk's item that lies in the range, taken off its units.
 __device__ __forceinline__ Item take_share(const Params &p, const sched::Cut &cut, uint64_t u1, int cta, Walk &w) {
     Item it;
-    const int begin = (uint64_t)w.end > w.left ? w.end - (int)w.left : 0, span = SLOTS * p.tt;
-    const int tk = w.cost.tile == sched::kFew.tile ? TKF : TK;
-    it.kb = sched::tile_at(w.cost, begin);
-    it.ke = sched::tile_at(w.cost, w.end);
+    const sched::Share share = sched::share_of(w.cost, w.end, w.left);
+    const int span = SLOTS * p.tt, tk = w.cost.tile == sched::kFew.tile ? TKF : TK;
+    it.kb = share.kb;
+    it.ke = share.ke;
     it.table = (int64_t)w.q.slot * p.a.pages_per_seq;
     if (it.ke > it.kb)  // the producers' first load of page ids would miss otherwise
         asm volatile("prefetch.global.L2 [%0];" ::"l"(p.a.page_table + it.table + it.kb * (tk / kPageTokens)));
@@ -636,10 +634,10 @@ __device__ __forceinline__ Item take_share(const Params &p, const sched::Cut &cu
     it.pos0 = w.q.kv - w.q.n + w.i * span;
     it.npages = (w.q.kv + kPageTokens - 1) / kPageTokens;
     it.dirty = max(0, (tk == TK ? (it.pos0 + 1) / TK : (it.pos0 + 1) / TKF) - it.kb);
-    it.dest = it.kb == 0 && it.ke == w.cost.tiles ? -1 : (it.kb == 0 ? 1 : 0);
+    it.dest = share.dest;
     if (it.dest == 1 && it.ke > it.kb)  // the range's last item, begun here: the rest of it lies behind the range
         w.rec = Record{it.tok0, it.ntok, w.h, sched::cta_of(cut, u1 - 1 + (uint64_t)(w.cost.units - w.end)) - cta};
-    w.left -= (uint64_t)(w.end - begin);
+    w.left -= (uint64_t)(w.end - share.begin);
     return it;
 }
 
@@ -736,7 +734,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         units += c.warp_sum[w];
     }
     const uint32_t tmem = __shfl_sync(0xffffffffu, c.tmem, 0);
-    const sched::Cut cut = sched::make_cut(units, (int)gridDim.x, kLeastUnits);
+    const sched::Cut cut = sched::make_cut(units, (int)gridDim.x, sched::kLeastUnits);
     const bool idle = cta >= cut.ctas;
     const uint64_t u0 = sched::begin(cut, cta), u1 = sched::begin(cut, cta + 1);
     if (!idle && before <= u1 - 1 && u1 - 1 < before + own) {

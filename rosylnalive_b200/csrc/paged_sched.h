@@ -1,5 +1,5 @@
-// paged_sched.h -- how the paged attention's work is counted and cut (host and device: the kernels use it, and it can
-// be checked on the CPU).
+// paged_sched.h -- how the paged attention's work is counted and cut, and the order of its ring of tiles (host and device:
+// the kernels use it, and tests/test_paged_sched.py checks it on the CPU).
 //
 // A request has n new tokens, the last of its kv keys, and `group` query heads a KV head. An item is up to `span`
 // consecutive tokens of one request and KV head, all their query heads, and reads the keys that its last token sees in
@@ -48,6 +48,7 @@ struct Cost {
     int own, tile;
 };
 constexpr Cost kFew = {13, 6}, kNarrow = {22, 7}, kWide = {30, 10};
+static_assert(kFew.tile != kNarrow.tile && kFew.tile != kWide.tile && kNarrow.tile != kWide.tile, "tile_at goes by them");
 
 // Units of the items before item i of a head: all of them are whole spans, and so of two slots' rows.
 LRM_HD uint64_t units_before(const Shape &s, int n, int kv, int i) {
@@ -104,9 +105,25 @@ LRM_HD uint64_t quotient(uint64_t a, uint64_t b) {
     return (a | b) >> 32 ? a / b : (uint64_t)((uint32_t)a / (uint32_t)b);
 }
 
+// The share of an item that lies in a range which ends at unit `end` of the item and has `left` units from there back: key
+// tiles [kb, ke) (none when it is of the item's own cost alone), from unit `begin` on. dest: -1 the whole item, else which of
+// the CTA's two partial results it is, 1 when it has the item's first tile. So a CTA has at most one of each: 1 is its
+// range's last item, cut at the range's end, and 0 its first, cut before it.
+struct Share {
+    int begin, kb, ke, dest;
+};
+LRM_HD Share share_of(const Item &t, int end, uint64_t left) {
+    const int begin = (uint64_t)end > left ? end - (int)left : 0, kb = tile_at(t, begin), ke = tile_at(t, end);
+    return Share{begin, kb, ke, kb == 0 && ke == t.tiles ? -1 : (kb == 0 ? 1 : 0)};
+}
+
 // The cut of all units: CTA c's range is [begin(c), begin(c + 1)). CTAs that take part have at least `least` units each
 // (more than kWide.tile, so that a share within an item holds a tile): short work is not cut into pieces that cost more
-// to merge than they save.
+// to merge than they save. (One token over 900 keys, 8 KV heads: 10.6 us, with 20 units 12.1; 4 tokens over up to 1700 keys, 4
+// KV heads 13.4, 14.7; 26 requests with chunks of up to 250 tokens, 2 KV heads 18.4, 18.8, with 30 20.5. Calls that fill the
+// SMs are alike.)
+constexpr int kLeastUnits = 12;
+static_assert(kLeastUnits > kWide.tile, "a share within an item holds a tile");
 struct Cut {
     int ctas;
     uint32_t more;   // the first ranges that are one unit longer

@@ -22,6 +22,29 @@ def sched(tmp_path_factory):
     return ctypes.CDLL(lib)
 
 
+# ---- the cut of a call's work ---------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("group", [1, 2, 3, 5, 8, 16, 31, 32, 33, 64, 65, 128])
+def test_items_of_a_request(sched, group):
+    sched.check_items.argtypes = [ctypes.c_uint64] + [ctypes.c_int] * 3
+    rng = random.Random(group)
+    span = 2 * (128 // group)
+    most = 1 << 24  # tokens of a call, and keys of a request
+    new = [1, 2, span - 1, span, span + 1, 3 * span, 5 * span + 1, most - 1, most] + [rng.randint(1, 5000) for _ in range(40)]
+    for n in new:
+        if n < 1:
+            continue
+        for kv in {n, min(most, n + 1), min(most, n + rng.randint(0, 300)), min(most, n + rng.randint(0, 1 << 23)), most}:
+            assert sched.check_items(n * 31 + kv, group, n, kv) == 0, (n, kv)
+
+
+@pytest.mark.parametrize("most", [1, 2, 16, 148, 200])
+def test_every_tile_of_a_call_is_computed_once_and_merged_once(sched, most):
+    sched.check_call.argtypes = [ctypes.c_uint64, ctypes.c_int]
+    for seed in range(400):
+        assert sched.check_call(seed * 1000 + most, most) == 0, seed
+
+
 # ---- the ring of K and V tiles ---------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("wide", [0, 1])
