@@ -310,7 +310,8 @@ lrm_status lrm_op_decode_attention_static(void *stream, const lrm_decode_attn_de
  *   seq_len_out      int32 [max_seqs]: the new lengths of the slots in slots (others stay); may be seq_len itself
  *   free_count_out   int32 [1]; may be free_count itself.
  * All or nothing: on a broken rule the error word gets its code, cu_seqlens and kv_len are all 0, tok_pos 0, slot_map
- * -1 (so the step's other calls do nothing), and the lengths, the table and the count stay as they were. Codes:
+ * -1 (so the step's other calls do nothing), and the lengths, the table and the count stay as they were: separate outputs get
+ * the old count and the old lengths of the listed slots that exist, so they hold the state all the same. Codes:
  *   0x5001 a slot outside 0 .. max_seqs - 1 or listed twice, a negative new_len, or a length (old or new) outside 0 ..
  *          16 * pages_per_seq;  0x5002 not enough free pages;  0x5003 more than max_tokens tokens;  0x5004 free_count
  *          outside 0 .. kv_pages, or a page id to be taken outside 0 .. kv_pages - 1.
@@ -326,7 +327,8 @@ lrm_status lrm_op_page_plan(void *stream, const lrm_page_plan_desc *desc);
 
 /* The plan's inverse: slot slots[i] keeps its first keep_len[i] tokens (0 .. its length; 0 frees the slot), and the
  * pages behind them go back on top of the free list, in request and then page order. slots[i] = -1 is padding.
- * seq_len_out and free_count_out as in the plan. All or nothing: on a broken rule nothing is written but the code:
+ * seq_len_out and free_count_out as in the plan, on a broken rule too. All or nothing: then nothing else is written but the
+ * code, and no length, page or count changes:
  *   0x5011 a slot outside 0 .. max_seqs - 1 or listed twice, a length outside 0 .. 16 * pages_per_seq, or a keep_len
  *          outside 0 .. the slot's length;  0x5012 free_count outside 0 .. kv_pages or more pages than the list holds;
  *          0x5014 a page id to be given back outside 0 .. kv_pages - 1. */

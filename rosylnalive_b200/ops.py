@@ -258,7 +258,8 @@ def page_plan(slots, new_len, seq_len, page_table, free_list, free_count, cu_seq
     tok_pos and slot_map [max_tokens]; int32 tensors throughout. slots [requests] (-1: padding) with new_len tokens
     each; seq_len [max_seqs], page_table [max_seqs, pages_per_seq], free_list [kv_pages] and free_count [1] are the
     cache's state, updated in place unless seq_len_out / free_count_out are given. All or nothing: a step that breaks a
-    rule (error_word 0x5001 .. 0x5004) takes no page and becomes a step of no tokens."""
+    rule (error_word 0x5001 .. 0x5004) takes no page and becomes a step of no tokens, and seq_len_out / free_count_out
+    get the old lengths of its slots and the old count."""
     if seq_len_out is None:
         seq_len_out = seq_len
     if free_count_out is None:
@@ -285,7 +286,8 @@ def page_release(slots, keep_len, seq_len, page_table, free_list, free_count, se
                  stream=None):
     """Cuts slots [requests] (-1: padding) back to their first keep_len tokens (0 frees a slot) and puts the pages
     behind them back on top of the free list. State and outputs as in page_plan. All or nothing: a call that breaks a
-    rule (error_word 0x5011, 0x5012, 0x5014) changes nothing."""
+    rule (error_word 0x5011, 0x5012, 0x5014) changes no length, page or count; seq_len_out / free_count_out get the old
+    ones, as in page_plan."""
     if seq_len_out is None:
         seq_len_out = seq_len
     if free_count_out is None:
