@@ -364,8 +364,9 @@ lrm_status lrm_op_qkv_append(void *stream, const lrm_qkv_append_desc *desc);
  * request's tokens are taken in pieces of 2 * floor(128 / group), group = q_heads / kv_heads. In a piece of at most 32 rows
  * (tokens * group), so for single tokens and short drafts, the weights that multiply v keep 16 bits (off by 2^-15 at most);
  * in larger ones they are rounded to bf16, as in lrm_op_prefill_attention (off by 2^-8 at most).
- * A request whose rows fall outside the tokens, whose slot is outside 0 .. max_seqs - 1, or whose kv_len is below its
- * tokens or above 16 * pages_per_seq is not computed: its rows are left as they were and the error word gets 0x4001. A
+ * A request whose rows fall outside the tokens or run backwards, whose slot is outside 0 .. max_seqs - 1, or whose kv_len is
+ * below its tokens or above 16 * pages_per_seq is not computed: its rows are left as they were and the error word gets
+ * 0x4001. (A row that two sound requests share, which takes a cu_seqlens that falls, gets the result of either.) A
  * page id outside the pool is never read: its keys count as zeros and the error word gets 0x4002. `workspace`:
  * workspace_bytes, at least lrm_op_paged_attention_workspace's, 16-byte aligned, any contents; calls that can run at the
  * same time need one each. scale must be positive and finite; ld_q and ld_out multiples of 8; q, pool and out 16-byte aligned.
