@@ -745,7 +745,12 @@ uint64_t lrm_op_paged_attention_workspace(int32_t tokens, int32_t q_heads, int32
     if (!in(tokens, 1, kMaxStepTokens) || !in(kv_heads, 1, 65535) || !in(q_heads, 1, 65535) || q_heads % kv_heads ||
         q_heads / kv_heads > 128)
         return 0;
-    return paged_attention_workspace(tokens, q_heads, kv_heads, device_sms());
+    uint64_t bytes = 0;
+    guarded([&] {  // without a device the message of that may not be allocated
+        bytes = paged_attention_workspace(tokens, q_heads, kv_heads, device_sms());
+        return LRM_OK;
+    });
+    return bytes;
 }
 
 lrm_status lrm_op_paged_attention(void *stream, const lrm_paged_attn_desc *d) {
