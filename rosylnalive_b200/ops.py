@@ -191,7 +191,9 @@ def decode_attention_static(q, pool, page_table, seq_len, slots, out, pages_per_
 #
 # plan -> append -> attention -> release, with lengths, page table and free pages kept on the device and no copy to or
 # from the host. These take tensors of any CUDA device (all of a call on one) and launch on `stream`, or on that
-# device's current stream. What only the device knows (slots, lengths, page ids) is checked there: error_word().
+# device's current stream. What only the device knows (slots, lengths, page ids) is checked there: error_word(). Arrays
+# without elements are refused (ValueError), as by the operators above: a step has one request and one row at least, which
+# may be padding (slot -1, slot_map -1).
 
 # A call is a few microseconds on the device, so the checks are kept to a few as well: one loop over its tensors, and the
 # descriptor packed in one go (the layouts of PagePlanDesc and its like above).
@@ -361,7 +363,8 @@ def qkv_append(qkv, q_norm, k_norm, eps, cos, sin, tok_pos, slot_map, q_out, poo
 
 
 def paged_attention_workspace(tokens, q_heads, kv_heads) -> int:
-    """Bytes of workspace for paged_attention calls of up to `tokens` rows, on the current device."""
+    """Bytes of workspace for paged_attention calls of up to `tokens` rows, on the current device; 0 for sizes that no
+    call has."""
     return int(N.lib().lrm_op_paged_attention_workspace(tokens, q_heads, kv_heads))
 
 
