@@ -381,11 +381,11 @@ __device__ __forceinline__ void load8(const float *shared, float (&x)[8]) {
     x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
 }
 
-// What is left of p beside its first 16 bits (the difference is exact); above 0 where p is, so that it times an infinite v is
-// that infinity and no NaN.
+// What is left of p beside its first 16 bits (the difference is exact). Where p is above 0 this is at least bf16's smallest
+// number, so that it times an infinite v is that infinity and no NaN.
 __device__ __forceinline__ float rest(float p) {
     const float hi = __uint_as_float(__float_as_uint(p) & 0xFFFF0000u);
-    return fmaxf(p - hi, fminf(p, 0x1p-126f));
+    return fmaxf(p - hi, fminf(p, 0x1p-133f));
 }
 
 // Eight rows' scores of this thread's key; rows that do not see it (those before `from`) as -inf.

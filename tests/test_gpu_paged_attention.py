@@ -63,6 +63,27 @@ def test_values_that_are_not_finite_in_keys_that_every_row_sees(value, heads):
     c.check(c.run(), before)
 
 
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), 3e38])
+@pytest.mark.parametrize("heads", [(16, 8), (4, 4), (10, 1)])
+def test_weights_of_one_bit_times_large_values(value, heads):
+    # q = 0: all weights are equal and p is 1, whose second bf16 has nothing left to hold. q_0 k_0 = -83: p is about 2^-120.
+    c = Cache([(1, 1), (1, 2), (3, 90), (1, 300), (40, 500), (1, 64)], *heads, seed=47)
+    c.q.zero_()
+    c.q[-1, :, 0] = 1
+    own, slots = c.table.cpu().numpy(), c.slots.tolist()
+    for i, (n, kv) in enumerate(c.reqs):
+        key = 0
+        pg = int(own[slots[i], key // PAGE])
+        c.pool[pg, :, 1, key % PAGE, 1::4] = value
+        c.v[i][key, :, 1::4] = value
+    c.k[5][0, :, 0] = -83 / SCALE
+    c.k[5][1:, :, 0] = 0
+    for key in range(64):
+        c.pool[int(own[slots[5], key // PAGE]), :, 0, key % PAGE, 0] = c.k[5][key, :, 0]
+    before = c.out.clone()
+    c.check(c.run(), before)
+
+
 def by_slot(c, i):
     return int(c.slots[i])
 
