@@ -41,9 +41,9 @@ namespace {
 //   4. write the part's outputs, tokens, pages and lengths.
 // A slot is listed once, so no CTA reads a length that another writes, and the new lengths may take the old ones' place;
 // free_count is read by all before the second barrier and written after it. What bounds it is latency: two dependent
-// loads, three barriers and the stores: 2.9 us for 64 requests of one token, 8.9 us for 1024 of 64 (a cluster in which
-// every CTA scans all requests took 15 us for 2000 requests and 36 thousand tokens, this one 10). A step that fits one
-// pass of one CTA (kCluster false) leaves out the exchange between the CTAs.
+// loads, three barriers and the stores: 3.2 us for 64 requests of one token (3.9 with lengths of their own), 9.2 us for 1024
+// of 64 (a cluster in which every CTA scans all requests took 15 us for 2000 requests and 36 thousand tokens, this one 10).
+// A step that fits one pass of one CTA (kCluster false) leaves out the exchange between the CTAs.
 // Sums saturate at 2^30 (min(a + b, 2^30) is associative for non-negative terms), far above every limit.
 constexpr int kPlanThreads = 1024, kPlanCtas = 8;
 constexpr uint32_t kSat = 1u << 30;
@@ -602,10 +602,13 @@ bool in(int64_t v, int64_t lo, int64_t hi) { return v >= lo && v <= hi; }
 }  // namespace
 
 cudaError_t launch_page_step(const PageStepArgs &a, cudaStream_t st) {
-    // Up to a size one CTA is faster, above it a cluster of 8 (times in us, one CTA against the cluster). Plans of 64
-    // requests and tokens 2.9, 5.9; of 1024 4.5, 6.5; of 512 requests and 4096 tokens 5.3, 6.4, and 6144 tokens 6.5, 6.2.
-    // Releases of 64 requests 3.0, 5.9; of 768 6.2, 6.5; of 1024 8.0, 6.6.
-    const bool big = a.keep_len ? a.requests > 768 : a.requests > kPlanThreads || a.max_tokens > 5 * 1024;
+    // Up to a size one CTA is faster, above it a cluster of 8. Times in us, one CTA against the cluster, with 1000 cached
+    // tokens a request: plans of 64 requests and tokens 3.2, 6.1; of 1024 4.6, 6.1; of 512 requests and 4096 tokens 5.5, 6.4,
+    // and 6144 tokens 8.4, 7.1; of 64 requests and 4096 tokens 6.3, 7.1. A release's time goes by its pages, which only the
+    // device knows; the host knows how many there can be. All of 40 requests' 2520 pages 4.6, 6.3; of 64's 4032 5.0, 6.4; of
+    // 256's 16,128 12.7, 6.7; of 768's 48,384 33.5, 9.1. A release of few pages is 3 us faster on one CTA, whatever it could be.
+    const int64_t most_pages = std::min<int64_t>((int64_t)a.requests * a.pages_per_seq, a.kv_pages);
+    const bool big = a.keep_len ? a.requests > 768 || most_pages > 8192 : a.requests > kPlanThreads || a.max_tokens > 5 * 1024;
     const unsigned ctas = big ? kPlanCtas : 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas);
