@@ -16,7 +16,8 @@
 //   few     (up to 32 rows): as narrow, with keys and rows swapped (below).
 // Tiles of wide and narrow items have 80 keys: S (80 columns) and P (40, two bf16 a column) then lie side by side in the
 // 128 that O leaves of a slot, so the next S is computed while the softmax still works on this one. With 128 keys, P over
-// S, every S waited for the P V before it: 1,000 rows over 121,000 keys took 1.68 million cycles, with 80 keys 1.25.
+// S, every S waited for the P V before it: 1,000 rows over 121,000 keys took 1.465 million cycles, with 80 keys 1.383 (and
+// 1.25 with what came after).
 // Warps of a CTA:
 //   0, 3    TMA producers: q of an item and K's tiles, and V's tiles, in the order of their use through a ring of five
 //           32 KiB stages (5 or 8 pages of 16 tokens, one box a page and 64 dims), running ahead into the next item;
@@ -35,11 +36,13 @@
 //
 // What bounds it and what it measured (device time, both kernels; 8 KV heads, two query heads each unless said):
 //   HBM       64 single tokens over 4096 to 4352 keys: 171 us, 6.48 TB/s, 0.99 of a copy's rate.
-//   HBM and the start: 32 x 5 tokens over 100 to 6000 keys, 32 query heads: 39.2 us, 4.35 TB/s. 3.5 us pass before the first
-//             load (the lengths' and page table's loads, the cut, and code that no CTA has fetched yet), 4 after the last.
-//   softmax and power: 1,000 tokens over 121,000 keys: 1.25 million cycles, tensor pipe active in 67 percent of them, the
-//             exponentials' unit in 67; 820 us at the 1.53 GHz that 1000 W allow, 1 PFLOP/s over seconds.
-//   the same and what an item costs beside its tiles (9,000 cycles of 36,000): 16 x 2048 tokens without a past 311 us.
+//   HBM and the start: 32 x 5 tokens over 100 to 6000 keys, 32 query heads: 39.4 to 41 us by the board, 4.2 TB/s. 3.5 us pass
+//             before the first load (the lengths' and page table's loads, the cut, and code that no CTA has fetched yet), 4
+//             after the last; every item's own 4,000 cycles are there too.
+//   softmax   1,000 tokens over 121,000 keys: 1.25 million cycles, tensor pipe active in 67 percent of them, the
+//             exponentials' unit in 67; 820 us at 1.53 GHz. Over seconds the board's 1000 W allow 1.36 GHz and it takes 1,010:
+//             a GEMM's sustained rate, at the same clock, would be 701.
+//   the same and what an item costs beside its tiles (9,000 cycles of 36,000): 16 x 2048 tokens without a past 320 us.
 //   latency   one token over 900 keys: 10.7 us.
 // Tried and slower: two issuing warps (their MMAs interleave badly); four softmax warpgroups (spills); a part of the
 // exponentials as polynomials on the FMA pipes (the warps' issue is as full as that unit).
@@ -320,8 +323,8 @@ __device__ __forceinline__ void quad_transpose(uint4 (&v)[4], int lane) {
 // single token is as precise as with lrm_op_decode_attention, whose p is fp32. Groups of eight rows alternate (eight rows,
 // the eight rests, ...), so O^T's columns do too, and up to eight rows still make one MMA of 16 columns. (p rounded to bf16
 // alone: 64 single tokens over 4096 keys off by 2.3e-3 in norm instead of 1.66e-3, which is the output's own rounding; 32 x 5
-// drafted tokens 40.4 us instead of 41.2, 8 x 511 among 56 decodes 55.1 instead of 58.3, single tokens alike. The rests in
-// eight MMAs of their own: 42.7, and 64 x 4096 173.9 instead of 172.5.)
+// drafted tokens 39.2 us instead of 39.4, on another board 40.0 and 41.0, 8 x 511 among 56 decodes 54.4 instead of 54.9,
+// single tokens alike. The rests in eight MMAs of their own: 32 x 5 42.7 us where it is 41.2, 64 x 4096 173.9 and 172.5.)
 struct RoleState {
     Control *c;
     const Params *p;

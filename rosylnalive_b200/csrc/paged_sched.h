@@ -41,9 +41,12 @@ LRM_HD Shape make_shape(int group) {
 LRM_HD int items_of(const Shape &s, int n) { return (int)(((uint64_t)(uint32_t)(n + s.span - 1) * s.inv_span) >> 38); }
 
 // An item's units: `own` for its start and end, then `tile` a tile. A unit is about 300 cycles. Alone, items of few rows
-// take 4,000 cycles + 1,400 a tile, of one slot's rows 6,700 + 1,400, of two slots' 9,000 + 1,950; where the memory's queues
-// are full, as in most mixtures, tiles take longer and part of `own` hides behind them. The weights are from mixtures (8
-// chunks of 511 tokens among 56 single ones: 56 us, 61 with 13 + 5 for few rows and 40 + 10 for two slots').
+// took 4,000 cycles + 1,400 a tile (with p in one bf16), of one slot's rows 6,700 + 1,400, of two slots' 9,000 + 1,950; where
+// the memory's queues are full, as in most mixtures, tiles take longer and part of `own` hides behind them. So the weights are
+// from mixtures, and a mixture's best ones are not another's: with kFew 11 + 6, 13 + 6, 15 + 6 and 18 + 7, 8 chunks of 511
+// tokens among 56 single ones (8 KV heads) took 63.9, 57.9, 60.1 and 59.3 us, 26 requests with 12 chunks of up to 250 (2 KV
+// heads) 19.5, 18.5, 19.6 and 18.3, 15 short requests (8 KV heads) 13.7, 13.1, 13.3 and 13.3; kWide at 40 + 10 with kFew 13 + 5
+// left the first at 61 where it was 56.
 struct Cost {
     int own, tile;
 };
