@@ -165,10 +165,11 @@ LRM_HD int v_place(int t, int nt, int lead) { return t + (t + lead < nt ? t + le
 // 2k + 2j + 1: V can be there, and be cleaned, up to (kRing + 1) / 2 items ahead of the mark that is still to be read.
 constexpr int kMarks = (kRing + 1) / 2 + 1;
 
-// Waits end after so many polls (a second or so; waits are microseconds). The softmax's warps meet at barriers that have no such
-// limit, so they must agree on whether a wait failed: theirs end long after the issuer, which makes at most ten waits from one
-// commit to the next of a slot, has either committed or given up for good, so nothing arrives while some have left.
-constexpr uint32_t kPolls = 1u << 20, kIssuerWaits = 10, kSoftmaxPolls = 16 * kPolls;
+// Waits end after so many polls: 2 s, at 4 us a poll that fails. They are microseconds, but for the scheduler's, which waits
+// for a whole item, 0.3 s of the longest that a call can have (2^24 keys). The softmax's warps meet at barriers that have no
+// such limit, so they must agree on whether a wait failed: theirs end long after the issuer, which makes at most ten waits
+// from one commit to the next of a slot, has either committed or given up for good, so nothing arrives while some have left.
+constexpr uint32_t kPolls = 1u << 19, kIssuerWaits = 10, kSoftmaxPolls = 12 * kPolls;
 LRM_HD uint32_t fill_parity(int x) { return (uint32_t)(x / kRing) & 1; }
 
 }  // namespace sched
